@@ -55,7 +55,8 @@ enum {
 enum {
     RESS_STATUS_HESS_NO_CONVERGENCE = 1, /* adjust_attention_selection max_iters hit */
     RESS_STATUS_ATTN_WAIT_TIMEOUT = 2,   /* a bounded mbarrier wait expired */
-    RESS_STATUS_LIST_OVERFLOW = 4        /* a keep list would exceed list_width */
+    RESS_STATUS_LIST_OVERFLOW = 4,       /* a keep list would exceed list_width */
+    RESS_STATUS_CACHE_RANGE = 8          /* a cache length or page number out of range */
 };
 
 enum { RESS_F32 = 0, RESS_BF16 = 1 };
@@ -340,6 +341,95 @@ int ress_dense_attn(const uint16_t *q, const uint16_t *k, const uint16_t *v, int
                     void *out, int out_bf16, int out_heads, long long out_sb, long long out_sh,
                     long long out_st, int out_group, long long out_period, int out_off, int32_t *status,
                     ress_stream_t stream);
+
+/*
+ * Streaming: a paged key/value cache in 8 bits.  No counterpart in the
+ * reference, whose global attention takes all views at once; here views
+ * arrive one after another and attend to those before them.
+ *
+ * A page holds 64 tokens.  Its block of one key/value head is 64 x 64 e4m3
+ * codes, token-major and contiguous (4096 bytes); the block of page p, head h
+ * begins at pages + p*page_stride + h*head_stride (bytes, multiples of 16).
+ * The block's scale is one e8m0 byte at scale + p*scale_stride + h: code u
+ * means 2^(u - 127), 255 means NaN.  Value = e4m3 code * scale.
+ * Stream b's token i lies in slot i % 64 of page table[b*table_stride + i/64];
+ * table entries past table_width pages do not exist, entries of pages that
+ * hold no token are never read.  Two streams may read a shared page; a page
+ * that receives tokens belongs to one stream.
+ *
+ * ress_cache_append: new tokens behind the lens[b] that stream b holds.
+ *   q (optional), k, v: head dim 64 contiguous, element (b, t, head) at
+ *   b*sb + t*st + head*sh (elements; rows 16-byte aligned), RESS_F32 or
+ *   RESS_BF16.  B streams, T tokens each, of which n_new[b] count (NULL: T);
+ *   Hkv heads of k and v, Hq of q (a multiple of Hkv).
+ *   q and k: LayerNorm over the head dims where weight and bias are given
+ *   (fp32; NULL: none), then the 2-D rotary embedding as in
+ *   ress_qkv_prologue when rope_cos is given (tables (rope_len, 32) in the
+ *   input's type, pos (B, T, 2) int64), all in fp32 without intermediate
+ *   rounding.  q_out (B, T, Hq, 64) contiguous in the input's type, padding
+ *   tokens included.  k and v go into their pages: the block's scale is the
+ *   smallest power of two that brings its new values to 448 or less (and no
+ *   smaller than the one of tokens it holds already, whose codes move to the
+ *   new scale); codes round to nearest even.  A value that is not finite
+ *   makes its block's scale NaN.  Slots that get no token keep their bytes.
+ *   lens is not changed.  Tokens whose page is missing (past table_width, or a
+ *   page number outside [0, n_pages)) are not stored, and set
+ *   RESS_STATUS_CACHE_RANGE.
+ */
+int ress_cache_append(const void *q, const void *k, const void *v, int dtype, int B, int T, int Hq, int Hkv,
+                      long long q_sb, long long q_st, long long q_sh, long long k_sb, long long k_st,
+                      long long k_sh, long long v_sb, long long v_st, long long v_sh, const float *qn_weight,
+                      const float *qn_bias, const float *kn_weight, const float *kn_bias, float eps,
+                      const long long *pos, const void *rope_cos, const void *rope_sin, int rope_len,
+                      const int32_t *table, long long table_stride, int table_width, const int32_t *lens,
+                      const int32_t *n_new, int n_pages, uint8_t *k_pages, uint8_t *v_pages, uint8_t *k_scale,
+                      uint8_t *v_scale, long long page_stride, long long head_stride, long long scale_stride,
+                      void *q_out, int32_t *status, ress_stream_t stream);
+
+/*
+ * Attention of the queries q (bf16; element (b, t, head) at b*q_sb + t*q_st +
+ * head*q_sh, rows 16-byte aligned) over the cache: softmax(q k^T * sm_scale) v
+ * over stream b's tokens below min(lens[b], limits[b*Tq + t]) (limits NULL:
+ * lens[b] for all).  Query heads are consecutive groups of Hq / Hkv per
+ * key/value head.  Sums and softmax statistics are fp32.  A query that sees no
+ * token gives zeros.  out (strides in elements, rows 16-byte aligned): bf16
+ * when out_bf16, else fp32.
+ * A length outside [0, 64*table_width] is clamped, a page number outside
+ * [0, n_pages) counts as a page of NaN; both set RESS_STATUS_CACHE_RANGE.
+ */
+int ress_cache_attn(const uint16_t *q, int B, int Tq, int Hq, int Hkv, long long q_sb, long long q_st,
+                    long long q_sh, const int32_t *table, long long table_stride, int table_width,
+                    const int32_t *lens, const int32_t *limits, int n_pages, const uint8_t *k_pages,
+                    const uint8_t *v_pages, const uint8_t *k_scale, const uint8_t *v_scale,
+                    long long page_stride, long long head_stride, long long scale_stride, float sm_scale,
+                    void *out, int out_bf16, long long o_sb, long long o_st, long long o_sh, int32_t *status,
+                    ress_stream_t stream);
+
+/*
+ * Rows to int8: scale[m] = max|x[m]| * RN(1/127), x8 = rint(x / scale) (zeros
+ * where the scale is 0; a row that is not finite gets a NaN scale).  x (M, K)
+ * RESS_F32 or RESS_BF16, rows x_st elements apart and 16-byte aligned, K a
+ * multiple of 16 and at most 2^17; x8 (M, K) contiguous.  Lays out the weights
+ * of ress_int8_linear as well.
+ */
+int ress_int8_quant_rows(const void *x, int dtype, int M, int K, long long x_st, int8_t *x8, float *scale,
+                         ress_stream_t stream);
+
+/*
+ * A Linear layer in 8-bit integers (no counterpart in the reference, whose
+ * Linears run in the model's type): x is quantised per row as by
+ * ress_int8_quant_rows, then
+ *   out[m][n] = (x8[m] . w8[n]) * scale[m] * w_scale[n] + bias[n]
+ * with exact int32 sums, the rest in fp32, an exact (erf) GELU when gelu is
+ * set, one rounding to out's type (RESS_F32 or RESS_BF16).  w8 (N, K)
+ * contiguous, 16-byte aligned; bias may be NULL; out rows out_st apart.
+ * workspace: ress_int8_linear_workspace(M, K) bytes, 16-byte aligned (NULL if
+ * that is 0).
+ */
+size_t ress_int8_linear_workspace(int M, int K);
+int ress_int8_linear(const void *x, int dtype, int M, int N, int K, long long x_st, const int8_t *w8,
+                     const float *w_scale, const float *bias, int gelu, void *out, int out_dtype,
+                     long long out_st, void *workspace, int32_t *status, ress_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -25,6 +25,7 @@ RESS_F32, RESS_BF16 = 0, 1
 STATUS_HESS_NO_CONVERGENCE = 1
 STATUS_ATTN_WAIT_TIMEOUT = 2
 STATUS_LIST_OVERFLOW = 4
+STATUS_CACHE_RANGE = 8
 
 # every symbol include/ress_sm100.h declares, with its ctypes signature
 _P = ctypes.c_void_p
@@ -64,6 +65,13 @@ SIGNATURES = {
                                     _I, _P, _P, _I, _P, _P, _P]),
     "ress_dense_attn": (_I, [_P, _P, _P, _I, _I, _I, _L, _L, _L, _L, _F, _P, _I, _I, _L, _L, _L, _I, _L, _I,
                              _P, _P]),
+    "ress_cache_append": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, *[_L] * 9, _P, _P, _P, _P, _F, _P, _P, _P, _I,
+                               _P, _L, _I, _P, _P, _I, _P, _P, _P, _P, _L, _L, _L, _P, _P, _P]),
+    "ress_cache_attn": (_I, [_P, _I, _I, _I, _I, _L, _L, _L, _P, _L, _I, _P, _P, _I, _P, _P, _P, _P, _L, _L, _L, _F,
+                             _P, _I, _L, _L, _L, _P, _P]),
+    "ress_int8_quant_rows": (_I, [_P, _I, _I, _I, _L, _P, _P, _P]),
+    "ress_int8_linear_workspace": (ctypes.c_size_t, [_I, _I]),
+    "ress_int8_linear": (_I, [_P, _I, _I, _I, _I, _L, _P, _P, _P, _I, _P, _I, _L, _P, _P, _P]),
 }
 
 _lib = None

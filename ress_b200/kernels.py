@@ -70,6 +70,8 @@ def check_status(device=None, reset: bool = True) -> int:
         raise RessError("sparse attention kernel: a bounded wait expired (result invalid)")
     if v & _lib.STATUS_LIST_OVERFLOW:
         raise RessError("keep list longer than its buffer")
+    if v & _lib.STATUS_CACHE_RANGE:
+        raise RessError("cache: a stream's length or a page number is out of range")
     return v
 
 
@@ -541,3 +543,206 @@ def qkv_prologue(qkv, H, qn_weight=None, qn_bias=None, kn_weight=None, kn_bias=N
                                         _ptr(kb), ctypes.c_float(eps), _ptr(pos), _ptr(rope_cos), _ptr(rope_sin),
                                         rope_len, _ptr(q), _ptr(k), _ptr(v), _stream(dev)), "ress_qkv_prologue")
     return q, k, v
+
+
+# ----------------------------------------------------------------- streaming
+PAGE = 64  # tokens per cache page
+
+
+def _cache_args(k_pages, v_pages, k_scale, v_scale, table, lens, B):
+    """Checks the cache's tensors; their common strides."""
+    n, Hkv = k_pages.shape[:2]
+    if k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn:
+        raise RessError("cache pages are float8_e4m3fn")
+    if k_scale.dtype != torch.float8_e8m0fnu or v_scale.dtype != torch.float8_e8m0fnu:
+        raise RessError("cache scales are float8_e8m0fnu")
+    if k_pages.shape != (n, Hkv, PAGE, HD) or v_pages.shape != k_pages.shape:
+        raise RessError("cache pages are (pages, heads, 64, 64), alike for k and v")
+    ps, hs, ts, ds = k_pages.stride()
+    if ts != HD or ds != 1 or v_pages.stride() != (ps, hs, ts, ds):
+        raise RessError("a page's block of one head is contiguous, and k and v pages share strides")
+    if k_scale.shape != (n, Hkv) or v_scale.shape != (n, Hkv):
+        raise RessError("cache scales are (pages, heads)")
+    ss, one = k_scale.stride()
+    if (one != 1 and Hkv > 1) or v_scale.stride() != (ss, one):
+        raise RessError("cache scales have contiguous heads, and k and v scales share strides")
+    if table.dtype != torch.int32 or lens.dtype != torch.int32:
+        raise RessError("the page table and the lengths are int32")
+    if table.dim() != 2 or table.shape[0] != B or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise RessError("the page table is (streams, pages) with contiguous rows")
+    if lens.shape != (B,) or not lens.is_contiguous():
+        raise RessError("lens holds one contiguous length per stream")
+    if n == 1:  # strides of a single page are never used
+        ps, ss = max(ps, hs, PAGE * HD), max(ss, Hkv)
+    if Hkv == 1:
+        hs = PAGE * HD
+    return n, Hkv, ps, hs, max(ss, Hkv)
+
+
+def _head_rows(x, what):
+    if x.dim() != 4 or x.shape[-1] != HD or x.stride(-1) != 1:
+        raise RessError(f"{what} must be (B, T, heads, 64) with a contiguous last dim")
+    (B, T, H, _), (sb, st, sh, _) = x.shape, x.stride()
+    return sb if B > 1 else 0, st if T > 1 else 0, sh if H > 1 else 0  # strides of a single row are never used
+
+
+def _same_device(dev, *ts):
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise RessError("all tensors of a call are on one CUDA device")
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def cache_append(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, *, q=None, n_new=None, qn_weight=None,
+                 qn_bias=None, kn_weight=None, kn_bias=None, eps=1e-5, pos=None, rope_cos=None, rope_sin=None):
+    """New tokens into a paged 8-bit cache (ress_cache_append).  k, v (B, T,
+    Hkv, 64) and q (B, T, Hq, 64) bf16 or fp32, any strides with a contiguous
+    last dim (views of a qkv Linear's output); lens (B,) int32 tokens that the
+    streams hold (not changed), n_new (B,) int32 of the T tokens that count.
+    q and k are normalised over the head dims where weight and bias are given
+    and rotated where rope_cos, rope_sin (positions, 32) and pos (B, T, 2) are;
+    k and v are quantised into their pages.  Returns q's rows (B, T, Hq, 64),
+    or None without q."""
+    _dev_ok(k)
+    dev = k.device
+    _same_device(dev, v, q, k_pages, v_pages, k_scale, v_scale, table, lens, n_new, qn_weight, qn_bias, kn_weight,
+                 kn_bias, pos, rope_cos, rope_sin)
+    ksb, kst, ksh = _head_rows(k, "k")
+    vsb, vst, vsh = _head_rows(v, "v")
+    B, T = k.shape[:2]
+    n, Hkv, ps, hs, ss = _cache_args(k_pages, v_pages, k_scale, v_scale, table, lens, B)
+    if k.shape != v.shape or k.shape[2] != Hkv or k.dtype != v.dtype:
+        raise RessError("k and v must be alike, with the cache's heads")
+    dt = _dtype_code(k.dtype)
+    q_out, Hq, qsb, qst, qsh = None, 0, 0, 0, 0
+    if q is not None:
+        qsb, qst, qsh = _head_rows(q, "q")
+        Hq = q.shape[2]
+        if q.shape[:2] != k.shape[:2] or q.dtype != k.dtype or Hq % Hkv:
+            raise RessError("q must have k's tokens and type, and a multiple of its heads")
+    if n_new is not None and (n_new.dtype != torch.int32 or n_new.shape != (B,) or not n_new.is_contiguous()):
+        raise RessError("n_new holds one contiguous int32 per stream")
+    for w, b in ((qn_weight, qn_bias), (kn_weight, kn_bias)):
+        if (w is None) != (b is None):
+            raise RessError("a norm has both weight and bias")
+        for x in (w, b):
+            if x is not None and (x.dtype != torch.float32 or x.shape != (HD,) or not x.is_contiguous()):
+                raise RessError("norm weights and biases are contiguous fp32 (64,)")
+    rope_len = 0
+    if (rope_cos is None) != (rope_sin is None):
+        raise RessError("the rotary embedding has both tables")
+    if rope_cos is not None:
+        if pos is None or pos.dtype != torch.int64 or pos.shape != (B, T, 2):
+            raise RessError("pos must be (B, T, 2) int64")
+        if rope_cos.dtype != k.dtype or rope_cos.shape[-1] != 32 or rope_cos.shape != rope_sin.shape or \
+                rope_sin.dtype != k.dtype or rope_cos.dim() != 2:
+            raise RessError("rotary tables must be (max_pos, 32) in k's dtype")
+        rope_cos, rope_sin, pos = rope_cos.contiguous(), rope_sin.contiguous(), pos.contiguous()
+        rope_len = rope_cos.shape[0]
+    if q is not None:
+        q_out = torch.empty(B, T, Hq, HD, dtype=q.dtype, device=dev)
+    if T == 0 or B == 0:
+        return q_out
+    code = _lib.load().ress_cache_append(
+        _p(q), k.data_ptr(), v.data_ptr(), dt, B, T, Hq, Hkv, qsb, qst, qsh, ksb, kst, ksh, vsb, vst, vsh,
+        _p(qn_weight), _p(qn_bias), _p(kn_weight), _p(kn_bias), eps, _p(pos) if rope_len else None, _p(rope_cos),
+        _p(rope_sin), rope_len, table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(), _p(n_new), n,
+        k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ps, hs, ss, _p(q_out),
+        status_word(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+    check(code, "ress_cache_append")
+    return q_out
+
+
+def cache_attn(q, k_pages, v_pages, k_scale, v_scale, table, lens, *, limits=None, sm_scale=None, out=None,
+               out_bf16=True):
+    """Attention of q (B, T, Hq, 64) bf16 over a paged 8-bit cache
+    (ress_cache_attn): query t of stream b sees the tokens below lens[b], or
+    below min(lens[b], limits[b, t]) with limits (B, T) int32 (a causal or
+    frame-wise mask, a prefix).  A query that sees none gives zeros.  out: a
+    (B, T, Hq, 64) tensor, bf16 or fp32; by default a new one."""
+    _dev_ok(q)
+    dev = q.device
+    _same_device(dev, k_pages, v_pages, k_scale, v_scale, table, lens, limits, out)
+    if q.dtype != torch.bfloat16:
+        raise RessError("cache_attn takes bf16 q")
+    sb, st, sh = _head_rows(q, "q")
+    B, T, Hq, _ = q.shape
+    n, Hkv, ps, hs, ss = _cache_args(k_pages, v_pages, k_scale, v_scale, table, lens, B)
+    if Hq % Hkv:
+        raise RessError("q's heads must be a multiple of the cache's")
+    if limits is not None and (limits.dtype != torch.int32 or limits.shape != (B, T) or not limits.is_contiguous()):
+        raise RessError("limits must be contiguous (B, T) int32")
+    if out is None:
+        out = torch.empty(B, T, Hq, HD, dtype=torch.bfloat16 if out_bf16 else torch.float32, device=dev)
+    elif out.shape != q.shape or out.dtype not in (torch.bfloat16, torch.float32):
+        raise RessError("cache_attn output must have q's shape, bf16 or fp32")
+    osb, ost, osh = _head_rows(out, "out")
+    if T == 0 or B == 0:
+        return out
+    code = _lib.load().ress_cache_attn(
+        q.data_ptr(), B, T, Hq, Hkv, sb, st, sh, table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(),
+        _p(limits), n, k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ps, hs, ss,
+        1.0 / math.sqrt(HD) if sm_scale is None else sm_scale, out.data_ptr(), int(out.dtype == torch.bfloat16), osb,
+        ost, osh, status_word(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+    check(code, "ress_cache_attn")
+    return out
+
+
+def _rows2d(x):
+    """x as (M, K) rows with one stride; a copy only where its strides do not allow that."""
+    if x.dim() == 2 and x.stride(1) == 1:
+        return x
+    x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 else x.contiguous()
+
+
+def int8_quant_rows(x):
+    """(..., K) bf16 or fp32 -> int8 of the same shape and one fp32 scale per
+    row (ress_int8_quant_rows): tokens, or the output channels of a weight."""
+    _dev_ok(x)
+    x2 = _rows2d(x)
+    M, K = x2.shape
+    x8 = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if M:
+        check(_lib.load().ress_int8_quant_rows(_p(x2), _dtype_code(x.dtype), M, K, x2.stride(0) if M > 1 else K, _p(x8),
+                                               _p(scale), torch.cuda.current_stream(x.device).cuda_stream),
+              "ress_int8_quant_rows")
+    return x8, scale
+
+
+def int8_linear(x, w8, w_scale, bias=None, *, act=None, out_dtype=None):
+    """A Linear layer in 8-bit integers (ress_int8_linear): x (..., K) bf16 or
+    fp32 is quantised per token, w8 (N, K) int8 and w_scale (N,) fp32 are the
+    weight's (int8_quant_rows lays them out once).  act: None or "gelu".
+    Returns (..., N) in x's type, or out_dtype."""
+    _dev_ok(x)
+    dev = x.device
+    _same_device(dev, w8, w_scale, bias)
+    if w8.dtype != torch.int8 or w8.dim() != 2 or not w8.is_contiguous():
+        raise RessError("w8 must be contiguous int8 (N, K)")
+    N, K = w8.shape
+    if x.shape[-1] != K:
+        raise RessError(f"x has {x.shape[-1]} features, the weight {K}")
+    for t in (w_scale, bias):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (N,) or not t.is_contiguous()):
+            raise RessError("w_scale and bias are contiguous fp32 (N,)")
+    if act not in (None, "gelu"):
+        raise RessError(f"unknown activation {act!r}")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    x2 = _rows2d(x)
+    M = x2.shape[0]
+    out = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype, device=dev)
+    if M == 0:
+        return out
+    lib = _lib.load()
+    need = lib.ress_int8_linear_workspace(M, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(lib.ress_int8_linear(x2.data_ptr(), _dtype_code(x.dtype), M, N, K, x2.stride(0) if M > 1 else K, w8.data_ptr(),
+                               w_scale.data_ptr(), _p(bias), int(act == "gelu"), out.data_ptr(),
+                               _dtype_code(out_dtype), N, _p(ws), status_word(dev).data_ptr(),
+                               torch.cuda.current_stream(dev).cuda_stream), "ress_int8_linear")
+    return out
