@@ -9,6 +9,7 @@
 // once to the output's type.
 #include "common.cuh"
 #include "prologue.cuh"
+#include "tcgen05.cuh"
 
 namespace ress {
 namespace i8 {
@@ -23,6 +24,7 @@ struct LinArgs {
     long long out_st;
     int M, N, K;
     int gelu;
+    int vec;              // w_scale and bias can be read four at a time
 };
 
 // The scale of a row from the bits of its largest magnitude; a row that is
@@ -50,7 +52,7 @@ __device__ __forceinline__ uint32_t amax8(const float (&x)[8]) {
 }
 
 __device__ __forceinline__ float finish(int acc, float sx, float sw, float bias, int gelu) {
-    float y = __fadd_rn(__fmul_rn(__fmul_rn((float)acc, sx), sw), bias);
+    float y = __fmaf_rn(__fmul_rn((float)acc, sx), sw, bias);
     if (gelu) y = 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
     return y;
 }
@@ -152,11 +154,403 @@ __global__ void __launch_bounds__(FEW_NT) few_kernel(const T *__restrict__ x, lo
 template <typename T, typename O>
 static int launch_few(const void *x, long long x_st, const LinArgs &a, cudaStream_t s) {
     const size_t smem = (size_t)FEW_M * (((a.K + 63) & ~63) + 16);
-    if (smem > 220 * 1024 || (a.M + FEW_M - 1) / FEW_M > 65535) return RESS_E_SHAPE;
     set_smem_attr((const void *)few_kernel<T, O>, smem);
     const dim3 grid((a.N + 31) / 32, (a.M + FEW_M - 1) / FEW_M);
     few_kernel<T, O><<<grid, FEW_NT, smem, s>>>((const T *)x, x_st, a);
     return cudaGetLastError() == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
+}
+
+// ----------------------------------------------------------------- many rows
+// Tiles of 128*CG tokens x BN channels on the tensor cores (tcgen05.mma
+// kind::i8, int32 accumulators in tensor memory).  CG = 2 pairs two CTAs of a
+// cluster on one tile: each loads its half of the tokens and of the channels,
+// so a tile's operands cross from L2 once per pair.  Persistent CTAs (pairs)
+// take tiles in turn, channel tiles fastest, so that the CTAs that run
+// together share token rows in L2.  Eight warps:
+//   warp 0     loads K slices of 128 bytes (TMA, 128B swizzle) into a ring;
+//   warp 1     issues the MMAs (the pair's first CTA only, when paired);
+//   warp 2     allocates tensor memory;
+//   warps 4-7  epilogue: accumulators of one of two buffers to registers,
+//              scales, bias, GELU, one rounding, shared memory, TMA store,
+//              while the next tile is accumulated into the other buffer.
+using namespace tc;
+
+template <int CG, int BN, typename O> struct Tile {
+    static constexpr int NT = 256, BK = 128;
+    static constexpr int A_BYTES = 128 * BK, B_ROWS = BN / CG, B_BYTES = B_ROWS * BK;
+    static constexpr int STAGE = A_BYTES + B_BYTES;
+    static constexpr int OUT_COLS = 128 / (int)sizeof(O);  // one 128-byte swizzled row
+    static constexpr int OUT_BYTES = 32 * 128;             // of a warp: 32 rows
+    static constexpr int RING = 196608;
+    static constexpr int NS = RING / STAGE < 8 ? RING / STAGE : 8;
+    static constexpr int OFF_OUT = NS * STAGE;
+    static constexpr int SMEM = OFF_OUT + 4 * 2 * OUT_BYTES + 1024;
+    static constexpr uint32_t COLS = 2 * BN;  // two accumulators
+    static constexpr uint32_t IDESC =
+        (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((128 * CG) >> 4) << 24);
+    static_assert(SMEM <= 227 * 1024 && COLS <= 512 && NS >= 2, "tile does not fit");
+};
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"((uint64_t)map),
+                 "r"(src), "r"(x), "r"(y)
+                 : "memory");
+}
+template <int CG> __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::
+                "r"(dst),
+            "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::
+                "r"(dst),
+            "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y)
+            : "memory");
+}
+template <int CG> __device__ __forceinline__ void mma_int8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(acc));
+    else
+        mma_i8(d, a, b, idesc, acc);
+}
+// arrives on the barrier at this offset in every CTA of the pair
+template <int CG> __device__ __forceinline__ void commit(uint64_t *bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                smem_u32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        mma_commit(bar);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t leader_addr(uint32_t a) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(a));
+    return r;
+}
+template <int CG> __device__ __forceinline__ void pair_sync() {
+    if constexpr (CG == 2) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+
+struct GemmBars {
+    uint64_t full[8], empty[8], acc_full[2], acc_free[2];
+    uint32_t tmem;
+    int abort_flag;
+};
+
+template <int CG, int BN, typename O>
+__global__ void __launch_bounds__(256, 1) gemm_kernel(const __grid_constant__ CUtensorMap tm_x,
+                                                      const __grid_constant__ CUtensorMap tm_w,
+                                                      const __grid_constant__ CUtensorMap tm_o, const LinArgs a,
+                                                      const float *__restrict__ sx, int tma_out, int32_t *status) {
+    using C = Tile<CG, BN, O>;
+    extern __shared__ unsigned char raw[];
+    __shared__ GemmBars B;
+    unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t ring = smem_u32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CG == 2 ? (int)cluster_rank() : 0;
+    volatile int *abort_flag = &B.abort_flag;
+    const int tiles_n = (a.N + BN - 1) / BN, tiles_m = (a.M + 128 * CG - 1) / (128 * CG);
+    const int tiles = tiles_n * tiles_m;
+    const int first = blockIdx.x / CG, step = gridDim.x / CG;
+    const int nk = (a.K + C::BK - 1) / C::BK;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::NS; ++i) {
+            mbar_init(&B.full[i], 1);
+            mbar_init(&B.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&B.acc_full[i], 1);
+            mbar_init(&B.acc_free[i], 4 * CG);
+        }
+        B.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        if constexpr (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)),
+                         "r"(C::COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)),
+                         "r"(C::COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    fence_before();
+    __syncthreads();
+    pair_sync<CG>();  // the peer's barriers exist before anything arrives on them
+    fence_after();
+    const uint32_t tmem = B.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int tile = first; ok && tile < tiles; tile += step) {
+                const int m0 = (tile / tiles_n) * 128 * CG + rank * 128, n0 = (tile % tiles_n) * BN + rank * C::B_ROWS;
+                for (int k = 0; k < nk; ++k, ++it) {
+                    const int s = it % C::NS;
+                    if (it >= C::NS && !wait_bar(&B.empty[s], (it / C::NS - 1) & 1, abort_flag, status)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = ring + s * C::STAGE;
+                    const uint32_t bar = CG == 2 ? leader_addr(smem_u32(&B.full[s])) : smem_u32(&B.full[s]);
+                    if (rank == 0) mbar_expect_tx(&B.full[s], CG * C::STAGE);
+                    tma_load_2d<CG>(dst, &tm_x, bar, k * C::BK, m0);
+                    tma_load_2d<CG>(dst + C::A_BYTES, &tm_w, bar, k * C::BK, n0);
+                }
+            }
+            // the last loads of each stage are seen to have landed (and been
+            // consumed, both CTAs') before this CTA may exit
+            for (int s = 0; s < C::NS && s < it; ++s) {
+                const int last = it - 1 - ((it - 1 - s) % C::NS);
+                const uint64_t t0 = globaltimer();
+                while (!mbar_try_wait_sleep(smem_u32(&B.empty[s]), (last / C::NS) & 1) &&
+                       globaltimer() - t0 < TIMEOUT_NS) {
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int it = 0, n = 0;
+            bool ok = true;
+            for (int tile = first; ok && tile < tiles; tile += step, ++n) {
+                const int buf = n & 1;
+                if (n >= 2 && !wait_bar(&B.acc_free[buf], ((n >> 1) - 1) & 1, abort_flag, status)) break;
+                fence_after();
+                for (int k = 0; k < nk; ++k, ++it) {
+                    const int s = it % C::NS;
+                    if (!wait_bar(&B.full[s], (it / C::NS) & 1, abort_flag, status)) {
+                        ok = false;
+                        break;
+                    }
+                    fence_after();
+                    const uint32_t sa = ring + s * C::STAGE, sb = sa + C::A_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_int8<CG>(tmem + buf * BN, make_desc(sa + kk * 32, 16, 1024, LAYOUT_SW128),
+                                     make_desc(sb + kk * 32, 16, 1024, LAYOUT_SW128), C::IDESC, (k | kk) ? 1u : 0u);
+                    commit<CG>(&B.empty[s]);
+                }
+                if (ok) commit<CG>(&B.acc_full[buf]);
+            }
+        }
+    } else if (warp >= 4) {
+        const int quad = warp & 3;
+        unsigned char *out_s = smem + C::OFF_OUT + quad * 2 * C::OUT_BYTES;
+        const uint32_t out_a = smem_u32(out_s);
+        int n = 0, ob = 0;
+        for (int tile = first; tile < tiles; tile += step, ++n) {
+            const int buf = n & 1;
+            const int m0 = (tile / tiles_n) * 128 * CG + rank * 128 + quad * 32, n0 = (tile % tiles_n) * BN;
+            const int m = m0 + lane;
+            const float s_row = m < a.M ? sx[m] : 0.0f;
+            if (!wait_bar_warp(&B.acc_full[buf], (n >> 1) & 1, abort_flag, status)) break;
+            fence_after();
+            const uint32_t tq = tmem + buf * BN + ((uint32_t)(quad * 32) << 16);
+#pragma unroll 1
+            for (int c = 0; c < BN; c += C::OUT_COLS, ob ^= 1) {
+                if (n0 + c >= a.N) break;
+                // the buffer written two pieces ago has been read by its store
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                __syncwarp();
+#pragma unroll
+                for (int part = 0; part < C::OUT_COLS; part += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(tq + c + part, v);
+                    tmem_wait_ld();
+                    const int col = n0 + c + part;
+                    const bool full = a.vec && col + 32 <= a.N;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float w[4], bb[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (full) {
+                            const float4 w4 = __ldg(reinterpret_cast<const float4 *>(a.w_scale + col + i));
+                            w[0] = w4.x; w[1] = w4.y; w[2] = w4.z; w[3] = w4.w;
+                            if (a.bias != nullptr) {
+                                const float4 b4 = __ldg(reinterpret_cast<const float4 *>(a.bias + col + i));
+                                bb[0] = b4.x; bb[1] = b4.y; bb[2] = b4.z; bb[3] = b4.w;
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const bool in = col + i + j < a.N;
+                                w[j] = in ? a.w_scale[col + i + j] : 0.0f;
+                                if (in && a.bias != nullptr) bb[j] = a.bias[col + i + j];
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            v[i + j] = __float_as_uint(finish((int)v[i + j], s_row, w[j], bb[j], a.gelu));
+                    }
+                    if (tma_out) {
+                        // 16-byte pieces of the lane's row, 128B-swizzled
+                        constexpr int PER = 16 / (int)sizeof(O);
+#pragma unroll
+                        for (int i = 0; i < 32; i += PER) {
+                            uint4 w;
+                            if constexpr (sizeof(O) == 2) {
+                                uint32_t x[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const __nv_bfloat162 h =
+                                        __floats2bfloat162_rn(__uint_as_float(v[i + 2 * j]), __uint_as_float(v[i + 2 * j + 1]));
+                                    x[j] = *reinterpret_cast<const uint32_t *>(&h);
+                                }
+                                w = make_uint4(x[0], x[1], x[2], x[3]);
+                            } else {
+                                w = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                            }
+                            const int piece = (part + i) / PER;
+                            *reinterpret_cast<uint4 *>(out_s + ob * C::OUT_BYTES + lane * 128 + ((piece ^ (lane & 7)) << 4)) = w;
+                        }
+                    } else if (m < a.M) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (col + i < a.N)
+                                DT<O>::store(reinterpret_cast<O *>(a.out), (size_t)(m * a.out_st + col + i),
+                                             __uint_as_float(v[i]));
+                    }
+                }
+                if (tma_out) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0 && m0 < a.M) {
+                        tma_store_2d(&tm_o, out_a + ob * C::OUT_BYTES, n0 + c, m0);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
+            }
+            // the accumulator is read: the issuer may overwrite it
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2)
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                     leader_addr(smem_u32(&B.acc_free[buf])))
+                                 : "memory");
+                else
+                    mbar_arrive(&B.acc_free[buf]);
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    pair_sync<CG>();  // neither CTA leaves while the other may still touch its memory
+    fence_after();
+    if (warp == 2) {
+        if constexpr (CG == 2)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
+    }
+}
+
+// Rows of `cols` elements, `stride` bytes apart, in boxes of 128 bytes x box_rows.
+static bool map_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem, long long cols, long long rows,
+                   long long stride, int box_rows) {
+    auto enc = get_encode();
+    if (!enc) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / elem), (cuuint32_t)box_rows}, es[2] = {1, 1};
+    return enc(m, dt, 2, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int CG, int BN, typename O>
+static int launch_gemm(const int8_t *x8, const float *sx, const LinArgs &a, int32_t *status, cudaStream_t s) {
+    using C = Tile<CG, BN, O>;
+    CUtensorMap tx, tw, to;
+    if (!map_2d(&tx, x8, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, a.K, 128) ||
+        !map_2d(&tw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.N, a.K, C::B_ROWS))
+        return RESS_E_NO_DEVICE;
+    const int size = (int)sizeof(O);
+    // rows whose stride or start a TMA store cannot take are stored by plain instructions
+    const int tma_out = !((uintptr_t)a.out & 15) && !((a.out_st * size) & 15);
+    to = tx;
+    if (tma_out && !map_2d(&to, a.out, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                           size, a.N, a.M, a.out_st * size, 32))
+        return RESS_E_NO_DEVICE;
+    const long long tiles = (long long)((a.N + BN - 1) / BN) * ((a.M + 128 * CG - 1) / (128 * CG));
+    const int slots = 148 / CG;
+    auto kern = gemm_kernel<CG, BN, O>;
+    set_smem_attr((const void *)kern, C::SMEM);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(CG * (tiles < slots ? tiles : slots)));
+    cfg.blockDim = dim3(C::NT);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, tx, tw, to, a, sx, tma_out, status) == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
+}
+
+template <typename T>
+static int launch_quant(const T *x, long long x_st, int M, int K, int8_t *x8, float *scale, cudaStream_t s) {
+    const unsigned blocks = (unsigned)(((long long)M * 32 + QUANT_NT - 1) / QUANT_NT);
+    quant_rows_kernel<<<blocks, QUANT_NT, 0, s>>>(x, x_st, M, K, x8, scale);
+    return cudaGetLastError() == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
+}
+
+// Rows up to which the weights' bytes bound the call and sixteen-row tiles do.
+constexpr int FEW_MAX_M = 16, FEW_MAX_K = 8192;
+static bool use_few(int M, int K) { return M <= FEW_MAX_M && K <= FEW_MAX_K; }
+static size_t workspace(int M, int K) {
+    return use_few(M, K) ? 0 : ((size_t)M * K + 255) / 256 * 256 + (size_t)M * sizeof(float);
+}
+
+template <typename T, typename O>
+static int linear(const void *x, long long x_st, const LinArgs &a, void *ws, int32_t *status, cudaStream_t s) {
+    if (use_few(a.M, a.K)) return launch_few<T, O>(x, x_st, a, s);
+    if (!ws) return RESS_E_ARG;
+    int8_t *x8 = reinterpret_cast<int8_t *>(ws);
+    float *sx = reinterpret_cast<float *>(x8 + ((size_t)a.M * a.K + 255) / 256 * 256);
+    const int rc = launch_quant((const T *)x, x_st, a.M, a.K, x8, sx, s);
+    if (rc != RESS_OK) return rc;
+    const long long pairs = (long long)((a.M + 255) / 256) * ((a.N + 255) / 256);
+    if (pairs >= 74) return launch_gemm<2, 256, O>(x8, sx, a, status, s);
+    const long long ones = (long long)((a.M + 127) / 128) * ((a.N + 127) / 128);
+    if (ones >= 100) return launch_gemm<1, 128, O>(x8, sx, a, status, s);
+    return launch_gemm<1, 64, O>(x8, sx, a, status, s);
 }
 
 }  // namespace i8
@@ -171,19 +565,13 @@ extern "C" int ress_int8_quant_rows(const void *x, int dtype, int M, int K, long
     if (K % 16 != 0 || K > (1 << 17)) return RESS_E_SHAPE;
     const int size = dtype == RESS_BF16 ? 2 : 4;
     if ((((uintptr_t)x | (uintptr_t)x8) & 15) || ((x_st * size) & 15)) return RESS_E_ARG;
-    const unsigned blocks = (unsigned)(((long long)M * 32 + i8::QUANT_NT - 1) / i8::QUANT_NT);
     if (dtype == RESS_BF16)
-        i8::quant_rows_kernel<<<blocks, i8::QUANT_NT, 0, (cudaStream_t)stream>>>((const __nv_bfloat16 *)x, x_st, M, K, x8,
-                                                                                 scale);
-    else
-        i8::quant_rows_kernel<<<blocks, i8::QUANT_NT, 0, (cudaStream_t)stream>>>((const float *)x, x_st, M, K, x8, scale);
-    return cudaGetLastError() == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
+        return i8::launch_quant((const __nv_bfloat16 *)x, x_st, M, K, x8, scale, (cudaStream_t)stream);
+    return i8::launch_quant((const float *)x, x_st, M, K, x8, scale, (cudaStream_t)stream);
 }
 
 extern "C" size_t ress_int8_linear_workspace(int M, int K) {
-    (void)M;
-    (void)K;
-    return 0;
+    return M > 0 && K > 0 ? i8::workspace(M, K) : 0;
 }
 
 extern "C" int ress_int8_linear(const void *x, int dtype, int M, int N, int K, long long x_st, const int8_t *w8,
@@ -196,12 +584,13 @@ extern "C" int ress_int8_linear(const void *x, int dtype, int M, int N, int K, l
     if (K % 16 != 0 || K > (1 << 17)) return RESS_E_SHAPE;
     const int size = dtype == RESS_BF16 ? 2 : 4;
     if ((((uintptr_t)x | (uintptr_t)w8) & 15) || ((x_st * size) & 15)) return RESS_E_ARG;
-    (void)workspace;
-    const i8::LinArgs a{w8, w_scale, bias, out, out_st, M, N, K, gelu};
+    if (((uintptr_t)workspace & 15) || M > (1 << 26)) return RESS_E_ARG;
+    const int vec = (((uintptr_t)w_scale | (uintptr_t)bias) & 15) == 0;
+    const i8::LinArgs a{w8, w_scale, bias, out, out_st, M, N, K, gelu, vec};
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == RESS_BF16)
-        return out_dtype == RESS_BF16 ? i8::launch_few<__nv_bfloat16, __nv_bfloat16>(x, x_st, a, s)
-                                      : i8::launch_few<__nv_bfloat16, float>(x, x_st, a, s);
-    return out_dtype == RESS_BF16 ? i8::launch_few<float, __nv_bfloat16>(x, x_st, a, s)
-                                  : i8::launch_few<float, float>(x, x_st, a, s);
+        return out_dtype == RESS_BF16 ? i8::linear<__nv_bfloat16, __nv_bfloat16>(x, x_st, a, workspace, status, s)
+                                      : i8::linear<__nv_bfloat16, float>(x, x_st, a, workspace, status, s);
+    return out_dtype == RESS_BF16 ? i8::linear<float, __nv_bfloat16>(x, x_st, a, workspace, status, s)
+                                  : i8::linear<float, float>(x, x_st, a, workspace, status, s);
 }
