@@ -356,54 +356,79 @@ int ress_dense_attn(const uint16_t *q, const uint16_t *k, const uint16_t *v, int
  * table entries past table_width pages do not exist, entries of pages that
  * hold no token are never read.  Two streams may read a shared page; a page
  * that receives tokens belongs to one stream.
- *
- * ress_cache_append: new tokens behind the lens[b] that stream b holds.
+ * The structs hold 8-byte fields only, so that a binding can pack them as
+ * arrays; sizes and strides are int64_t.
+ */
+typedef struct {
+    uint8_t *k_pages, *v_pages, *k_scale, *v_scale;
+    int64_t n_pages, heads;                           /* of the pool */
+    int64_t page_stride, head_stride, scale_stride;   /* bytes, alike for k and v */
+    const int32_t *table;
+    int64_t table_stride, table_width;                /* entries */
+    const int32_t *lens;                              /* tokens that each stream holds */
+    int64_t streams;
+} ress_cache;
+
+/*
+ * ress_cache_append: `tokens` new tokens per stream, behind the lens[b] that
+ * stream b holds; n_new[b] of them count (NULL: all).
  *   q (optional), k, v: head dim 64 contiguous, element (b, t, head) at
  *   b*sb + t*st + head*sh (elements; rows 16-byte aligned), RESS_F32 or
- *   RESS_BF16.  B streams, T tokens each, of which n_new[b] count (NULL: T);
- *   Hkv heads of k and v, Hq of q (a multiple of Hkv).
+ *   RESS_BF16; k and v have the cache's heads, q a multiple of them.
  *   q and k: LayerNorm over the head dims where weight and bias are given
  *   (fp32; NULL: none), then the 2-D rotary embedding as in
  *   ress_qkv_prologue when rope_cos is given (tables (rope_len, 32) in the
- *   input's type, pos (B, T, 2) int64), all in fp32 without intermediate
- *   rounding.  q_out (B, T, Hq, 64) contiguous in the input's type, padding
- *   tokens included.  k and v go into their pages: the block's scale is the
- *   smallest power of two that brings its new values to 448 or less (and no
- *   smaller than the one of tokens it holds already, whose codes move to the
- *   new scale); codes round to nearest even.  A value that is not finite
- *   makes its block's scale NaN.  Slots that get no token keep their bytes.
- *   lens is not changed.  Tokens whose page is missing (past table_width, or a
- *   page number outside [0, n_pages)) are not stored, and set
- *   RESS_STATUS_CACHE_RANGE.
+ *   input's type, pos (streams, tokens, 2) int64), all in fp32 without
+ *   intermediate rounding.  q_out (streams, tokens, q_heads, 64) contiguous in
+ *   the input's type, padding tokens included.  k and v go into their pages:
+ *   the block's scale is the smallest power of two that brings its new values
+ *   to 448 or less (and no smaller than the one of tokens it holds already,
+ *   whose codes move to the new scale); codes round to nearest even.  A value
+ *   that is not finite makes its block's scale NaN.  Slots that get no token
+ *   keep their bytes.  lens is not changed.  Tokens whose page is missing (past
+ *   table_width, or a page number outside [0, n_pages)) are not stored, and
+ *   set RESS_STATUS_CACHE_RANGE.
  */
-int ress_cache_append(const void *q, const void *k, const void *v, int dtype, int B, int T, int Hq, int Hkv,
-                      long long q_sb, long long q_st, long long q_sh, long long k_sb, long long k_st,
-                      long long k_sh, long long v_sb, long long v_st, long long v_sh, const float *qn_weight,
-                      const float *qn_bias, const float *kn_weight, const float *kn_bias, float eps,
-                      const long long *pos, const void *rope_cos, const void *rope_sin, int rope_len,
-                      const int32_t *table, long long table_stride, int table_width, const int32_t *lens,
-                      const int32_t *n_new, int n_pages, uint8_t *k_pages, uint8_t *v_pages, uint8_t *k_scale,
-                      uint8_t *v_scale, long long page_stride, long long head_stride, long long scale_stride,
-                      void *q_out, int32_t *status, ress_stream_t stream);
+typedef struct {
+    const void *q, *k, *v;
+    void *q_out;
+    int64_t dtype, tokens, q_heads;
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+    const float *qn_weight, *qn_bias, *kn_weight, *kn_bias;
+    double eps;
+    const int64_t *pos;
+    const void *rope_cos, *rope_sin;
+    int64_t rope_len;
+    const int32_t *n_new;
+} ress_append_args;
+int ress_cache_append(const ress_cache *cache, const ress_append_args *args, int32_t *status, ress_stream_t stream);
 
 /*
- * Attention of the queries q (bf16; element (b, t, head) at b*q_sb + t*q_st +
- * head*q_sh, rows 16-byte aligned) over the cache: softmax(q k^T * sm_scale) v
- * over stream b's tokens below min(lens[b], limits[b*Tq + t]) (limits NULL:
- * lens[b] for all).  Query heads are consecutive groups of Hq / Hkv per
- * key/value head.  Sums and softmax statistics are fp32.  A query that sees no
- * token gives zeros.  out (strides in elements, rows 16-byte aligned): bf16
- * when out_bf16, else fp32.
- * A length outside [0, 64*table_width] is clamped, a page number outside
- * [0, n_pages) counts as a page of NaN; both set RESS_STATUS_CACHE_RANGE.
+ * ress_cache_attn: queries q (bf16, `tokens` per stream and q_heads heads,
+ * element (b, t, head) at b*q_sb + t*q_st + head*q_sh, rows 16-byte aligned)
+ * over the cache: softmax(q k^T * sm_scale) v over stream b's tokens below
+ * min(lens[b], limits[b*tokens + t]) (limits NULL: lens[b] for all).  Query
+ * heads are consecutive groups of q_heads / heads per key/value head.  Sums
+ * and softmax statistics are fp32.  A query that sees no token gives zeros.
+ * out (strides in elements, rows 16-byte aligned): bf16 when out_bf16, else
+ * fp32.  A length outside [0, 64*table_width] is clamped, a page number
+ * outside [0, n_pages) counts as a page of NaN; both set
+ * RESS_STATUS_CACHE_RANGE.
+ * workspace: ress_cache_attn_workspace(streams, heads, rows, table_width) bytes
+ * with rows = tokens * q_heads / heads, 16-byte aligned (NULL if that is 0).
  */
-int ress_cache_attn(const uint16_t *q, int B, int Tq, int Hq, int Hkv, long long q_sb, long long q_st,
-                    long long q_sh, const int32_t *table, long long table_stride, int table_width,
-                    const int32_t *lens, const int32_t *limits, int n_pages, const uint8_t *k_pages,
-                    const uint8_t *v_pages, const uint8_t *k_scale, const uint8_t *v_scale,
-                    long long page_stride, long long head_stride, long long scale_stride, float sm_scale,
-                    void *out, int out_bf16, long long o_sb, long long o_st, long long o_sh, int32_t *status,
-                    ress_stream_t stream);
+typedef struct {
+    const uint16_t *q;
+    void *out;
+    int64_t tokens, q_heads;
+    int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
+    int64_t out_bf16;
+    const int32_t *limits;
+    double sm_scale;
+    void *workspace;
+} ress_attn_args;
+size_t ress_cache_attn_workspace(int64_t streams, int64_t heads, int64_t rows, int64_t table_width);
+int ress_cache_attn(const ress_cache *cache, const ress_attn_args *args, int32_t *status, ress_stream_t stream);
 
 /*
  * Rows to int8: scale[m] = max|x[m]| * RN(1/127), x8 = rint(x / scale) (zeros

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libress_sm100.so")
@@ -32,6 +33,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_longlong
 _F = ctypes.c_float
+_S = ctypes.c_char_p  # a struct, packed as bytes
 SIGNATURES = {
     "ress_version": (_I, []),
     "ress_check_scale_division": (_I, [_P, _P]),
@@ -65,14 +67,18 @@ SIGNATURES = {
                                     _I, _P, _P, _I, _P, _P, _P]),
     "ress_dense_attn": (_I, [_P, _P, _P, _I, _I, _I, _L, _L, _L, _L, _F, _P, _I, _I, _L, _L, _L, _I, _L, _I,
                              _P, _P]),
-    "ress_cache_append": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, *[_L] * 9, _P, _P, _P, _P, _F, _P, _P, _P, _I,
-                               _P, _L, _I, _P, _P, _I, _P, _P, _P, _P, _L, _L, _L, _P, _P, _P]),
-    "ress_cache_attn": (_I, [_P, _I, _I, _I, _I, _L, _L, _L, _P, _L, _I, _P, _P, _I, _P, _P, _P, _P, _L, _L, _L, _F,
-                             _P, _I, _L, _L, _L, _P, _P]),
+    "ress_cache_append": (_I, [_S, _S, _P, _P]),
+    "ress_cache_attn_workspace": (ctypes.c_size_t, [_L, _L, _L, _L]),
+    "ress_cache_attn": (_I, [_S, _S, _P, _P]),
     "ress_int8_quant_rows": (_I, [_P, _I, _I, _I, _L, _P, _P, _P]),
     "ress_int8_linear_workspace": (ctypes.c_size_t, [_I, _I]),
     "ress_int8_linear": (_I, [_P, _I, _I, _I, _I, _L, _P, _P, _P, _I, _P, _I, _L, _P, _P, _P]),
 }
+
+# the structs of include/ress_sm100.h, every field 8 bytes (P: pointer, q: int64, d: double)
+CACHE = struct.Struct("PPPPqqqqqPqqPq")
+APPEND_ARGS = struct.Struct("PPPPqqqqqqqqqqqqPPPPdPPPqP")
+ATTN_ARGS = struct.Struct("PPqqqqqqqqqPdP")
 
 _lib = None
 

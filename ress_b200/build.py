@@ -13,7 +13,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRC = [os.path.join(HERE, "csrc", f) for f in ("capi.cu", "score.cu", "select.cu", "attn.cu", "noalloc.cu",
-                                                "prologue.cu", "cache.cu", "cache_attn.cu", "int8.cu")]
+                                                "prologue.cu", "cache.cu", "cache_attn.cu", "cache_attn_tc.cu", "int8.cu")]
 OUT = os.path.join(HERE, "libress_sm100.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
@@ -28,7 +28,8 @@ def needs_build() -> bool:
     if not os.path.exists(OUT):
         return True
     t = os.path.getmtime(OUT)
-    deps = SRC + [os.path.join(HERE, "csrc", h) for h in ("common.cuh", "prologue.cuh", "tcgen05.cuh", "cache.cuh")]
+    deps = SRC + [os.path.join(HERE, "csrc", h) for h in ("common.cuh", "prologue.cuh", "tcgen05.cuh", "cache.cuh",
+                                                       "cache_attn.cuh")]
     deps.append(os.path.join(ROOT, "include", "ress_sm100.h"))
     return any(os.path.getmtime(p) > t for p in deps)
 

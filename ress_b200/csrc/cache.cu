@@ -175,52 +175,47 @@ __global__ void __launch_bounds__(APP_NT) append_kernel(const AppendArgs a) {
 
 using namespace ress;
 
-extern "C" int ress_cache_append(const void *q, const void *k, const void *v, int dtype, int B, int T, int Hq, int Hkv,
-                                 long long q_sb, long long q_st, long long q_sh, long long k_sb, long long k_st,
-                                 long long k_sh, long long v_sb, long long v_st, long long v_sh,
-                                 const float *qn_weight, const float *qn_bias, const float *kn_weight,
-                                 const float *kn_bias, float eps, const long long *pos, const void *rope_cos,
-                                 const void *rope_sin, int rope_len, const int32_t *table, long long table_stride,
-                                 int table_width, const int32_t *lens, const int32_t *n_new, int n_pages,
-                                 uint8_t *k_pages, uint8_t *v_pages, uint8_t *k_scale, uint8_t *v_scale,
-                                 long long page_stride, long long head_stride, long long scale_stride, void *q_out,
-                                 int32_t *status, ress_stream_t stream) {
-    if (!k || !v || !table || !lens || !k_pages || !v_pages || !k_scale || !v_scale || !status) return RESS_E_ARG;
-    if (B <= 0 || T <= 0 || Hkv <= 0 || n_pages <= 0 || table_width <= 0 || table_stride < 0) return RESS_E_ARG;
-    if ((q != nullptr) != (q_out != nullptr) || (q && (Hq <= 0 || Hq % Hkv != 0))) return RESS_E_ARG;
-    if ((qn_weight == nullptr) != (qn_bias == nullptr) || (kn_weight == nullptr) != (kn_bias == nullptr))
+extern "C" int ress_cache_append(const ress_cache *cache, const ress_append_args *args, int32_t *status,
+                                 ress_stream_t stream) {
+    const int rc = cache::check_cache(cache);
+    if (rc != RESS_OK) return rc;
+    if (!args || !status || !args->k || !args->v || args->tokens <= 0) return RESS_E_ARG;
+    const ress_append_args &g = *args;
+    if ((g.q != nullptr) != (g.q_out != nullptr) || (g.q && (g.q_heads <= 0 || g.q_heads % cache->heads != 0)))
         return RESS_E_ARG;
-    if ((rope_cos == nullptr) != (rope_sin == nullptr) || (rope_cos != nullptr && (!pos || rope_len <= 0)))
+    if ((g.qn_weight == nullptr) != (g.qn_bias == nullptr) || (g.kn_weight == nullptr) != (g.kn_bias == nullptr))
         return RESS_E_ARG;
-    if (dtype != RESS_BF16 && dtype != RESS_F32) return RESS_E_DTYPE;
+    if ((g.rope_cos == nullptr) != (g.rope_sin == nullptr) || (g.rope_cos != nullptr && (!g.pos || g.rope_len <= 0)))
+        return RESS_E_ARG;
+    if (g.dtype != RESS_BF16 && g.dtype != RESS_F32) return RESS_E_DTYPE;
     // 16-byte loads of eight elements
-    const int size = dtype == RESS_BF16 ? 2 : 4;
-    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)rope_cos | (uintptr_t)rope_sin) & 15)
+    const int size = g.dtype == RESS_BF16 ? 2 : 4;
+    if (((uintptr_t)g.q | (uintptr_t)g.k | (uintptr_t)g.v | (uintptr_t)g.q_out | (uintptr_t)g.rope_cos |
+         (uintptr_t)g.rope_sin) & 15)
         return RESS_E_ARG;
-    if (((k_sb | k_st | k_sh | v_sb | v_st | v_sh) * size) & 15) return RESS_E_ARG;
-    if (q && ((q_sb | q_st | q_sh) * size) & 15) return RESS_E_ARG;
-    if ((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) || ((page_stride | head_stride) & 15)) return RESS_E_ARG;
-    if (head_stride < cache::BLOCK_BYTES || page_stride < cache::BLOCK_BYTES || scale_stride < Hkv) return RESS_E_ARG;
-    const long long pages = ((long long)T + cache::PAGE - 2) / cache::PAGE + 1;  // that T tokens can reach into
-    if (pages > 65535 || B > 65535) return RESS_E_SHAPE;
+    if (((g.k_sb | g.k_st | g.k_sh | g.v_sb | g.v_st | g.v_sh) * size) & 15) return RESS_E_ARG;
+    if (g.q && ((g.q_sb | g.q_st | g.q_sh) * size) & 15) return RESS_E_ARG;
+    const int64_t pages = (g.tokens + cache::PAGE - 2) / cache::PAGE + 1;  // that the tokens can reach into
+    if (pages > 65535 || g.rope_len > (1 << 30) || g.q_heads > (1 << 20)) return RESS_E_SHAPE;
     cache::AppendArgs a;
-    a.q = q; a.k = k; a.v = v;
-    a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
-    a.k_sb = k_sb; a.k_st = k_st; a.k_sh = k_sh;
-    a.v_sb = v_sb; a.v_st = v_st; a.v_sh = v_sh;
-    a.q_out = q_out;
-    a.T = T;
-    a.group = q ? Hq / Hkv : 0;
-    a.qw = qn_weight; a.qb = qn_bias; a.kw = kn_weight; a.kb = kn_bias;
-    a.eps = eps;
-    a.pos = pos; a.cos = rope_cos; a.sin = rope_sin; a.rope_len = rope_len;
-    a.table = table; a.lens = lens; a.n_new = n_new;
-    a.table_stride = table_stride; a.table_width = table_width; a.n_pages = n_pages;
-    a.K = {k_pages, k_scale, page_stride, head_stride, scale_stride};
-    a.V = {v_pages, v_scale, page_stride, head_stride, scale_stride};
+    a.q = g.q; a.k = g.k; a.v = g.v;
+    a.q_sb = g.q_sb; a.q_st = g.q_st; a.q_sh = g.q_sh;
+    a.k_sb = g.k_sb; a.k_st = g.k_st; a.k_sh = g.k_sh;
+    a.v_sb = g.v_sb; a.v_st = g.v_st; a.v_sh = g.v_sh;
+    a.q_out = g.q_out;
+    a.T = (int)g.tokens;
+    a.group = g.q ? (int)(g.q_heads / cache->heads) : 0;
+    a.qw = g.qn_weight; a.qb = g.qn_bias; a.kw = g.kn_weight; a.kb = g.kn_bias;
+    a.eps = (float)g.eps;
+    a.pos = reinterpret_cast<const long long *>(g.pos);
+    a.cos = g.rope_cos; a.sin = g.rope_sin; a.rope_len = (int)g.rope_len;
+    a.table = cache->table; a.lens = cache->lens; a.n_new = g.n_new;
+    a.table_stride = cache->table_stride; a.table_width = (int)cache->table_width; a.n_pages = (int)cache->n_pages;
+    a.K = {cache->k_pages, cache->k_scale, cache->page_stride, cache->head_stride, cache->scale_stride};
+    a.V = {cache->v_pages, cache->v_scale, cache->page_stride, cache->head_stride, cache->scale_stride};
     a.status = status;
-    const dim3 grid((unsigned)Hkv, (unsigned)pages, (unsigned)B);
-    if (dtype == RESS_BF16)
+    const dim3 grid((unsigned)cache->heads, (unsigned)pages, (unsigned)cache->streams);
+    if (g.dtype == RESS_BF16)
         cache::append_kernel<__nv_bfloat16><<<grid, cache::APP_NT, 0, (cudaStream_t)stream>>>(a);
     else
         cache::append_kernel<float><<<grid, cache::APP_NT, 0, (cudaStream_t)stream>>>(a);

@@ -27,6 +27,19 @@ struct Pages {
     long long scale_stride;              // of a page's scales; heads are contiguous
 };
 
+// The host-side checks of a cache that its calls share.
+inline int check_cache(const ress_cache *c) {
+    if (!c || !c->k_pages || !c->v_pages || !c->k_scale || !c->v_scale || !c->table || !c->lens) return RESS_E_ARG;
+    if (c->n_pages <= 0 || c->heads <= 0 || c->streams <= 0 || c->table_width <= 0 || c->table_stride < 0)
+        return RESS_E_ARG;
+    if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages | (uintptr_t)c->page_stride | (uintptr_t)c->head_stride) & 15)
+        return RESS_E_ARG;
+    if (c->head_stride < BLOCK_BYTES || c->page_stride < BLOCK_BYTES || c->scale_stride < c->heads) return RESS_E_ARG;
+    if (c->n_pages > (1 << 30) || c->heads > 65535 || c->streams > 65535 || c->table_width > (1 << 24))
+        return RESS_E_SHAPE;
+    return RESS_OK;
+}
+
 __device__ __forceinline__ float scale_value(int u) {
     return __uint_as_float(u == 255 ? 0x7FC00000u : (u == 0 ? 0x00400000u : (uint32_t)u << 23));
 }

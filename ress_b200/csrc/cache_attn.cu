@@ -1,47 +1,11 @@
-// cache_attn.cu -- attention of a few or many queries over the paged 8-bit
-// cache (cache.cuh).
-//
-//     S = q k^T sm_scale,  P = softmax(S over the tokens a query sees),  O = P V
-//
-// with k = code * 2^(u - 127) and v likewise.  Query t of stream b sees the
-// tokens below min(lens[b], limits[b][t]); a query that sees none gives
-// zeros.  Query heads that share a key/value head are rows of one tile: row
-// r of (stream, key/value head) is query r / group, head r % group of its
-// group.
-#include <climits>
-
-#include "cache.cuh"
-#include "tcgen05.cuh"
+// cache_attn.cu -- attention of a few queries over the paged 8-bit cache, and
+// the C entry for any number (cache_attn.cuh has the definition).
+#include "cache_attn.cuh"
 
 namespace ress {
 namespace cache {
 
 using namespace tc;
-
-struct AttnArgs {
-    const uint16_t *q;  // bf16
-    long long q_sb, q_st, q_sh;
-    void *out;
-    long long o_sb, o_st, o_sh;
-    int out_bf16;
-    int Tq, group, rows;  // rows = Tq * group
-    Pages K, V;
-    const int32_t *table, *lens, *limits;
-    long long table_stride;
-    int table_width, n_pages;
-    float scale_log2;  // sm_scale * log2(e)
-    int32_t *status;
-};
-
-// Tokens that the queries of stream b may see at most.
-__device__ __forceinline__ int stream_len(const AttnArgs &a, int b) {
-    const int len = a.lens[b];
-    const long long cap = (long long)a.table_width * PAGE;
-    return len < 0 ? 0 : (len > cap ? (int)cap : len);
-}
-__device__ __forceinline__ bool bad_len(const AttnArgs &a, int b) {
-    return a.lens[b] < 0 || a.lens[b] > (long long)a.table_width * PAGE;
-}
 
 // ------------------------------------------------------------------ few rows
 // Up to 16 rows a tile, on mma.sync.m16n8k16: with so few rows the bound is
@@ -68,6 +32,8 @@ constexpr int FEW_ROWS = 16, FEW_WARPS = 4, FEW_STAGES = 3;
 constexpr int FEW_NT = FEW_WARPS * 32;
 constexpr int FEW_SMEM = FEW_WARPS * FEW_STAGES * 2 * BLOCK_BYTES;
 constexpr int P_SHIFT = 14;
+// Rows of a (stream, key/value head) up to which this kernel runs.
+constexpr int FEW_MAX_ROWS = 32;
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -121,9 +87,7 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ float load_q16(const AttnArgs &a, int b, int h, int r, int t, uint32_t (&w)[8]) {
     float x[16] = {};
     if (r < a.rows) {
-        const int tq = r / a.group, g = r - tq * a.group;
-        const uint4 *p = reinterpret_cast<const uint4 *>(a.q + b * a.q_sb + tq * a.q_st +
-                                                         (long long)(h * a.group + g) * a.q_sh + t * 16);
+        const uint4 *p = reinterpret_cast<const uint4 *>(a.q + row_at(a, b, h, r, a.q_sb, a.q_st, a.q_sh) + t * 16);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint4 u = __ldg(p + i);
@@ -174,10 +138,8 @@ __global__ void __launch_bounds__(FEW_NT) few_kernel(const AttnArgs a, int kv_he
     int lim[2], lo = INT_MAX, hi = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int r = r0 + g + 8 * i;
-        lim[i] = -1;
-        if (r < a.rows) {
-            lim[i] = a.limits != nullptr ? max(0, min(len, a.limits[(long long)b * a.Tq + r / a.group])) : len;
+        lim[i] = row_limit(a, b, len, r0 + g + 8 * i);
+        if (lim[i] >= 0) {
             lo = min(lo, lim[i]);
             hi = max(hi, lim[i]);
         }
@@ -436,8 +398,7 @@ __global__ void __launch_bounds__(FEW_NT) few_kernel(const AttnArgs a, int kv_he
             l = cta_l[r];
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no token seen: zeros
-        const int tq = (r0 + r) / a.group, gq = (r0 + r) - tq * a.group;
-        const long long at = b * a.o_sb + tq * a.o_st + (long long)(h * a.group + gq) * a.o_sh + d;
+        const long long at = row_at(a, b, h, r0 + r, a.o_sb, a.o_st, a.o_sh) + d;
         if (a.out_bf16) {
             const __nv_bfloat162 x = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
             const __nv_bfloat162 y = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
@@ -451,6 +412,17 @@ __global__ void __launch_bounds__(FEW_NT) few_kernel(const AttnArgs a, int kv_he
     if (splits > 1) cluster_sync();  // peers read this CTA's shared memory until here
 }
 
+// Clusters of more than eight CTAs, once per device and kernel.
+static bool allow_wide_clusters(const void *kern, int which) {
+    static thread_local uint64_t done[2] = {0, 0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 64 && (done[which] >> dev) & 1) return true;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+    if (dev < 64) done[which] |= 1ull << dev;
+    return true;
+}
+
 static int launch_few(const AttnArgs &a, int B, int Hkv, cudaStream_t stream) {
     const int tiles = (a.rows + FEW_ROWS - 1) / FEW_ROWS;
     const long long groups = (long long)tiles * Hkv * B;
@@ -459,9 +431,7 @@ static int launch_few(const AttnArgs &a, int B, int Hkv, cudaStream_t stream) {
     while (splits < 16 && groups * splits * 2 <= 148 * 2 && splits * 2 * FEW_WARPS * 2 <= a.table_width) splits *= 2;
     auto kern = a.rows <= 8 ? few_kernel<true> : few_kernel<false>;
     set_smem_attr((const void *)kern, FEW_SMEM);
-    if (splits > 8 &&
-        cudaFuncSetAttribute((const void *)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        return RESS_E_LAUNCH;
+    if (splits > 8 && !allow_wide_clusters((const void *)kern, a.rows <= 8)) return RESS_E_LAUNCH;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, (unsigned)(tiles * Hkv), (unsigned)B);
     cfg.blockDim = dim3(FEW_NT);
@@ -481,38 +451,43 @@ static int launch_few(const AttnArgs &a, int B, int Hkv, cudaStream_t stream) {
 
 using namespace ress;
 
-extern "C" int ress_cache_attn(const uint16_t *q, int B, int Tq, int Hq, int Hkv, long long q_sb, long long q_st,
-                               long long q_sh, const int32_t *table, long long table_stride, int table_width,
-                               const int32_t *lens, const int32_t *limits, int n_pages, const uint8_t *k_pages,
-                               const uint8_t *v_pages, const uint8_t *k_scale, const uint8_t *v_scale,
-                               long long page_stride, long long head_stride, long long scale_stride, float sm_scale,
-                               void *out, int out_bf16, long long o_sb, long long o_st, long long o_sh,
-                               int32_t *status, ress_stream_t stream) {
-    if (!q || !table || !lens || !k_pages || !v_pages || !k_scale || !v_scale || !out || !status) return RESS_E_ARG;
-    if (B <= 0 || Tq <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0) return RESS_E_ARG;
-    if (n_pages <= 0 || table_width <= 0 || table_stride < 0) return RESS_E_ARG;
-    if (((uintptr_t)q & 15) || ((q_sb | q_st | q_sh) & 7)) return RESS_E_ARG;
-    if ((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) || ((page_stride | head_stride) & 15)) return RESS_E_ARG;
-    if (head_stride < cache::BLOCK_BYTES || page_stride < cache::BLOCK_BYTES || scale_stride < Hkv) return RESS_E_ARG;
-    const int size = out_bf16 ? 2 : 4;
-    if (((uintptr_t)out & 15) || (((o_sb | o_st | o_sh) * size) & 15)) return RESS_E_ARG;
-    const long long rows = (long long)Tq * (Hq / Hkv);
-    if (rows > (1 << 30) || table_width > (1 << 24) || B > 65535) return RESS_E_SHAPE;
-    if (((rows + cache::FEW_ROWS - 1) / cache::FEW_ROWS) * Hkv > 65535) return RESS_E_SHAPE;
+extern "C" size_t ress_cache_attn_workspace(int64_t streams, int64_t heads, int64_t rows, int64_t table_width) {
+    if (streams <= 0 || heads <= 0 || rows <= cache::FEW_MAX_ROWS || table_width <= 0) return 0;
+    return cache::many_workspace((int)streams, (int)heads, rows, table_width);
+}
+
+extern "C" int ress_cache_attn(const ress_cache *cache, const ress_attn_args *args, int32_t *status,
+                               ress_stream_t stream) {
+    const int rc = cache::check_cache(cache);
+    if (rc != RESS_OK) return rc;
+    if (!args || !status || !args->q || !args->out || args->tokens <= 0) return RESS_E_ARG;
+    const ress_attn_args &g = *args;
+    const int64_t H = cache->heads;
+    if (g.q_heads <= 0 || g.q_heads % H != 0) return RESS_E_ARG;
+    if (((uintptr_t)g.q & 15) || ((g.q_sb | g.q_st | g.q_sh) & 7)) return RESS_E_ARG;
+    const int size = g.out_bf16 ? 2 : 4;
+    if (((uintptr_t)g.out & 15) || (((g.o_sb | g.o_st | g.o_sh) * size) & 15)) return RESS_E_ARG;
+    if (g.tokens > (1 << 30) || g.q_heads > (1 << 20)) return RESS_E_SHAPE;
+    const int64_t rows = g.tokens * (g.q_heads / H);
+    if (rows > (1 << 30)) return RESS_E_SHAPE;
     cache::AttnArgs a;
-    a.q = q;
-    a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
-    a.out = out;
-    a.o_sb = o_sb; a.o_st = o_st; a.o_sh = o_sh;
-    a.out_bf16 = out_bf16;
-    a.Tq = Tq;
-    a.group = Hq / Hkv;
+    a.q = g.q;
+    a.q_sb = g.q_sb; a.q_st = g.q_st; a.q_sh = g.q_sh;
+    a.out = g.out;
+    a.o_sb = g.o_sb; a.o_st = g.o_st; a.o_sh = g.o_sh;
+    a.out_bf16 = g.out_bf16 != 0;
+    a.Tq = (int)g.tokens;
+    a.group = (int)(g.q_heads / H);
     a.rows = (int)rows;
-    a.K = {const_cast<uint8_t *>(k_pages), const_cast<uint8_t *>(k_scale), page_stride, head_stride, scale_stride};
-    a.V = {const_cast<uint8_t *>(v_pages), const_cast<uint8_t *>(v_scale), page_stride, head_stride, scale_stride};
-    a.table = table; a.lens = lens; a.limits = limits;
-    a.table_stride = table_stride; a.table_width = table_width; a.n_pages = n_pages;
-    a.scale_log2 = sm_scale * 1.4426950408889634f;
+    a.K = {cache->k_pages, cache->k_scale, cache->page_stride, cache->head_stride, cache->scale_stride};
+    a.V = {cache->v_pages, cache->v_scale, cache->page_stride, cache->head_stride, cache->scale_stride};
+    a.table = cache->table; a.lens = cache->lens; a.limits = g.limits;
+    a.table_stride = cache->table_stride; a.table_width = (int)cache->table_width; a.n_pages = (int)cache->n_pages;
+    a.scale_log2 = (float)(g.sm_scale * 1.4426950408889634);
     a.status = status;
-    return cache::launch_few(a, B, Hkv, (cudaStream_t)stream);
+    a.partial = nullptr;
+    a.arrived = nullptr;
+    if (rows > cache::FEW_MAX_ROWS)
+        return cache::launch_many(a, (int)cache->streams, (int)H, args->workspace, (cudaStream_t)stream);
+    return cache::launch_few(a, (int)cache->streams, (int)H, (cudaStream_t)stream);
 }

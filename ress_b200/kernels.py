@@ -546,54 +546,69 @@ def qkv_prologue(qkv, H, qn_weight=None, qn_bias=None, kn_weight=None, kn_bias=N
 
 
 # ----------------------------------------------------------------- streaming
+# These calls are made per token: their checks read each tensor's attributes
+# once, and structs and raw pointers keep the host's share of a call small.
 PAGE = 64  # tokens per cache page
+_E4M3, _E8M0, _BF16, _F32, _I32 = (torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.bfloat16, torch.float32,
+                                   torch.int32)
+_status_ptr = {}
 
 
-def _cache_args(k_pages, v_pages, k_scale, v_scale, table, lens, B):
-    """Checks the cache's tensors; their common strides."""
-    n, Hkv = k_pages.shape[:2]
-    if k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn:
-        raise RessError("cache pages are float8_e4m3fn")
-    if k_scale.dtype != torch.float8_e8m0fnu or v_scale.dtype != torch.float8_e8m0fnu:
-        raise RessError("cache scales are float8_e8m0fnu")
-    if k_pages.shape != (n, Hkv, PAGE, HD) or v_pages.shape != k_pages.shape:
-        raise RessError("cache pages are (pages, heads, 64, 64), alike for k and v")
-    ps, hs, ts, ds = k_pages.stride()
-    if ts != HD or ds != 1 or v_pages.stride() != (ps, hs, ts, ds):
-        raise RessError("a page's block of one head is contiguous, and k and v pages share strides")
-    if k_scale.shape != (n, Hkv) or v_scale.shape != (n, Hkv):
-        raise RessError("cache scales are (pages, heads)")
-    ss, one = k_scale.stride()
-    if (one != 1 and Hkv > 1) or v_scale.stride() != (ss, one):
-        raise RessError("cache scales have contiguous heads, and k and v scales share strides")
-    if table.dtype != torch.int32 or lens.dtype != torch.int32:
-        raise RessError("the page table and the lengths are int32")
-    if table.dim() != 2 or table.shape[0] != B or (table.stride(1) != 1 and table.shape[1] > 1):
-        raise RessError("the page table is (streams, pages) with contiguous rows")
-    if lens.shape != (B,) or not lens.is_contiguous():
-        raise RessError("lens holds one contiguous length per stream")
-    if n == 1:  # strides of a single page are never used
-        ps, ss = max(ps, hs, PAGE * HD), max(ss, Hkv)
-    if Hkv == 1:
-        hs = PAGE * HD
-    return n, Hkv, ps, hs, max(ss, Hkv)
+def _dev_status(i: int) -> int:
+    """Address of device i's status word (it lives as long as the process)."""
+    p = _status_ptr.get(i)
+    if p is None:
+        p = _status_ptr[i] = status_word(torch.device("cuda", i)).data_ptr()
+    return p
 
 
-def _head_rows(x, what):
-    if x.dim() != 4 or x.shape[-1] != HD or x.stride(-1) != 1:
-        raise RessError(f"{what} must be (B, T, heads, 64) with a contiguous last dim")
-    (B, T, H, _), (sb, st, sh, _) = x.shape, x.stride()
-    return sb if B > 1 else 0, st if T > 1 else 0, sh if H > 1 else 0  # strides of a single row are never used
+def _raw_stream(i: int) -> int:
+    return torch.cuda.current_stream(i).cuda_stream
 
 
-def _same_device(dev, *ts):
+def _on_device(i: int, *ts):
     for t in ts:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != i:
             raise RessError("all tensors of a call are on one CUDA device")
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
+def _pack_cache(i, B, k_pages, v_pages, k_scale, v_scale, table, lens):
+    """Checks the cache's tensors (device i, B streams); the struct and the heads."""
+    if k_pages.dtype is not _E4M3 or v_pages.dtype is not _E4M3:
+        raise RessError("cache pages are float8_e4m3fn")
+    if k_scale.dtype is not _E8M0 or v_scale.dtype is not _E8M0:
+        raise RessError("cache scales are float8_e8m0fnu")
+    if table.dtype is not _I32 or lens.dtype is not _I32:
+        raise RessError("the page table and the lengths are int32")
+    _on_device(i, k_pages, v_pages, k_scale, v_scale, table, lens)
+    shape, strides = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or shape[2:] != (PAGE, HD) or v_pages.shape != shape:
+        raise RessError("cache pages are (pages, heads, 64, 64), alike for k and v")
+    if strides[2:] != (HD, 1) or v_pages.stride() != strides:
+        raise RessError("a page's block of one head is contiguous, and k and v pages share strides")
+    n, H = shape[:2]
+    sstr = k_scale.stride()
+    if k_scale.shape != (n, H) or v_scale.shape != (n, H) or v_scale.stride() != sstr or (sstr[1] != 1 and H > 1):
+        raise RessError("cache scales are (pages, heads) with contiguous heads, alike for k and v")
+    tshape, tstr = table.shape, table.stride()
+    if len(tshape) != 2 or tshape[0] != B or (tstr[1] != 1 and tshape[1] > 1):
+        raise RessError("the page table is (streams, pages) with contiguous rows")
+    if lens.shape != (B,) or not lens.is_contiguous():
+        raise RessError("lens holds one contiguous length per stream")
+    ps, hs, ss = strides[0], strides[1], sstr[0]
+    if n == 1 or H == 1:  # the stride of a single page or head is never used
+        hs = hs if H > 1 else PAGE * HD
+        ps, ss = (ps, ss) if n > 1 else (H * hs, H)
+    return _lib.CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, H, ps,
+                           hs, ss, table.data_ptr(), tstr[0], tshape[1], lens.data_ptr(), B), H
+
+
+def _head_rows(x, what):
+    """Shape and strides of (B, T, heads, 64) rows; 0 for a stride that is never used."""
+    shape, s = x.shape, x.stride()
+    if len(shape) != 4 or shape[3] != HD or s[3] != 1:
+        raise RessError(f"{what} must be (B, T, heads, 64) with a contiguous last dim")
+    return shape, s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0
 
 
 def cache_append(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, *, q=None, n_new=None, qn_weight=None,
@@ -607,52 +622,56 @@ def cache_append(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, *, q=Non
     k and v are quantised into their pages.  Returns q's rows (B, T, Hq, 64),
     or None without q."""
     _dev_ok(k)
-    dev = k.device
-    _same_device(dev, v, q, k_pages, v_pages, k_scale, v_scale, table, lens, n_new, qn_weight, qn_bias, kn_weight,
-                 kn_bias, pos, rope_cos, rope_sin)
-    ksb, kst, ksh = _head_rows(k, "k")
-    vsb, vst, vsh = _head_rows(v, "v")
-    B, T = k.shape[:2]
-    n, Hkv, ps, hs, ss = _cache_args(k_pages, v_pages, k_scale, v_scale, table, lens, B)
-    if k.shape != v.shape or k.shape[2] != Hkv or k.dtype != v.dtype:
+    i, dtype = k.get_device(), k.dtype
+    dt = _dtype_code(dtype)
+    shape, ksb, kst, ksh = _head_rows(k, "k")
+    vshape, vsb, vst, vsh = _head_rows(v, "v")
+    B, T = shape[0], shape[1]
+    cache, Hkv = _pack_cache(i, B, k_pages, v_pages, k_scale, v_scale, table, lens)
+    if vshape != shape or shape[2] != Hkv or v.dtype is not dtype:
         raise RessError("k and v must be alike, with the cache's heads")
-    dt = _dtype_code(k.dtype)
-    q_out, Hq, qsb, qst, qsh = None, 0, 0, 0, 0
+    _on_device(i, v, q, n_new, pos, rope_cos, rope_sin)
+    Hq, qsb, qst, qsh, qp, q_out, q_out_p = 0, 0, 0, 0, 0, None, 0
     if q is not None:
-        qsb, qst, qsh = _head_rows(q, "q")
-        Hq = q.shape[2]
-        if q.shape[:2] != k.shape[:2] or q.dtype != k.dtype or Hq % Hkv:
+        qshape, qsb, qst, qsh = _head_rows(q, "q")
+        Hq, qp = qshape[2], q.data_ptr()
+        if qshape[0] != B or qshape[1] != T or q.dtype is not dtype or Hq % Hkv:
             raise RessError("q must have k's tokens and type, and a multiple of its heads")
-    if n_new is not None and (n_new.dtype != torch.int32 or n_new.shape != (B,) or not n_new.is_contiguous()):
+        q_out = torch.empty((B, T, Hq, HD), dtype=dtype, device=k.device)
+        q_out_p = q_out.data_ptr()
+    if n_new is not None and (n_new.dtype is not _I32 or n_new.shape != (B,) or not n_new.is_contiguous()):
         raise RessError("n_new holds one contiguous int32 per stream")
+    norms = []
     for w, b in ((qn_weight, qn_bias), (kn_weight, kn_bias)):
         if (w is None) != (b is None):
             raise RessError("a norm has both weight and bias")
         for x in (w, b):
-            if x is not None and (x.dtype != torch.float32 or x.shape != (HD,) or not x.is_contiguous()):
-                raise RessError("norm weights and biases are contiguous fp32 (64,)")
-    rope_len = 0
+            if x is None:
+                norms.append(0)
+                continue
+            if x.dtype is not _F32 or x.shape != (HD,) or x.get_device() != i or x.stride(0) != 1:
+                raise RessError("norm weights and biases are contiguous fp32 (64,) on the call's device")
+            norms.append(x.data_ptr())
+    pos_p = cos_p = sin_p = rope_len = 0
     if (rope_cos is None) != (rope_sin is None):
         raise RessError("the rotary embedding has both tables")
     if rope_cos is not None:
-        if pos is None or pos.dtype != torch.int64 or pos.shape != (B, T, 2):
+        if pos is None or pos.dtype is not torch.int64 or pos.shape != (B, T, 2):
             raise RessError("pos must be (B, T, 2) int64")
-        if rope_cos.dtype != k.dtype or rope_cos.shape[-1] != 32 or rope_cos.shape != rope_sin.shape or \
-                rope_sin.dtype != k.dtype or rope_cos.dim() != 2:
+        tshape = rope_cos.shape
+        if rope_cos.dtype is not dtype or rope_sin.dtype is not dtype or len(tshape) != 2 or tshape[1] != 32 or \
+                rope_sin.shape != tshape:
             raise RessError("rotary tables must be (max_pos, 32) in k's dtype")
         rope_cos, rope_sin, pos = rope_cos.contiguous(), rope_sin.contiguous(), pos.contiguous()
-        rope_len = rope_cos.shape[0]
-    if q is not None:
-        q_out = torch.empty(B, T, Hq, HD, dtype=q.dtype, device=dev)
+        pos_p, cos_p, sin_p, rope_len = pos.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), tshape[0]
     if T == 0 or B == 0:
         return q_out
-    code = _lib.load().ress_cache_append(
-        _p(q), k.data_ptr(), v.data_ptr(), dt, B, T, Hq, Hkv, qsb, qst, qsh, ksb, kst, ksh, vsb, vst, vsh,
-        _p(qn_weight), _p(qn_bias), _p(kn_weight), _p(kn_bias), eps, _p(pos) if rope_len else None, _p(rope_cos),
-        _p(rope_sin), rope_len, table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(), _p(n_new), n,
-        k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ps, hs, ss, _p(q_out),
-        status_word(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
-    check(code, "ress_cache_append")
+    args = _lib.APPEND_ARGS.pack(qp, k.data_ptr(), v.data_ptr(), q_out_p, dt, T, Hq, qsb, qst, qsh, ksb, kst, ksh, vsb,
+                                 vst, vsh, *norms, eps, pos_p, cos_p, sin_p, rope_len,
+                                 0 if n_new is None else n_new.data_ptr())
+    code = _lib.load().ress_cache_append(cache, args, _dev_status(i), _raw_stream(i))
+    if code:
+        check(code, "ress_cache_append")
     return q_out
 
 
@@ -664,30 +683,39 @@ def cache_attn(q, k_pages, v_pages, k_scale, v_scale, table, lens, *, limits=Non
     frame-wise mask, a prefix).  A query that sees none gives zeros.  out: a
     (B, T, Hq, 64) tensor, bf16 or fp32; by default a new one."""
     _dev_ok(q)
-    dev = q.device
-    _same_device(dev, k_pages, v_pages, k_scale, v_scale, table, lens, limits, out)
-    if q.dtype != torch.bfloat16:
+    i = q.get_device()
+    if q.dtype is not _BF16:
         raise RessError("cache_attn takes bf16 q")
-    sb, st, sh = _head_rows(q, "q")
-    B, T, Hq, _ = q.shape
-    n, Hkv, ps, hs, ss = _cache_args(k_pages, v_pages, k_scale, v_scale, table, lens, B)
+    shape, sb, st, sh = _head_rows(q, "q")
+    B, T, Hq, _ = shape
+    cache, Hkv = _pack_cache(i, B, k_pages, v_pages, k_scale, v_scale, table, lens)
     if Hq % Hkv:
         raise RessError("q's heads must be a multiple of the cache's")
-    if limits is not None and (limits.dtype != torch.int32 or limits.shape != (B, T) or not limits.is_contiguous()):
-        raise RessError("limits must be contiguous (B, T) int32")
+    lim = 0
+    if limits is not None:
+        if limits.dtype is not _I32 or limits.shape != (B, T) or not limits.is_contiguous() or limits.get_device() != i:
+            raise RessError("limits must be contiguous (B, T) int32 on the call's device")
+        lim = limits.data_ptr()
     if out is None:
-        out = torch.empty(B, T, Hq, HD, dtype=torch.bfloat16 if out_bf16 else torch.float32, device=dev)
-    elif out.shape != q.shape or out.dtype not in (torch.bfloat16, torch.float32):
-        raise RessError("cache_attn output must have q's shape, bf16 or fp32")
-    osb, ost, osh = _head_rows(out, "out")
+        out = torch.empty(shape, dtype=_BF16 if out_bf16 else _F32, device=q.device)
+        osh, ost, osb = HD, Hq * HD, T * Hq * HD
+    else:
+        oshape, osb, ost, osh = _head_rows(out, "out")
+        if oshape != shape or out.dtype not in (_BF16, _F32) or out.get_device() != i:
+            raise RessError("cache_attn output must have q's shape, bf16 or fp32, on the call's device")
+        out_bf16 = out.dtype is _BF16
     if T == 0 or B == 0:
         return out
-    code = _lib.load().ress_cache_attn(
-        q.data_ptr(), B, T, Hq, Hkv, sb, st, sh, table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(),
-        _p(limits), n, k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ps, hs, ss,
-        1.0 / math.sqrt(HD) if sm_scale is None else sm_scale, out.data_ptr(), int(out.dtype == torch.bfloat16), osb,
-        ost, osh, status_word(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
-    check(code, "ress_cache_attn")
+    lib, ws = _lib.load(), None
+    rows = T * (Hq // Hkv)
+    if rows > 16:  # one token needs no workspace
+        need = lib.ress_cache_attn_workspace(B, Hkv, rows, table.shape[1])
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    args = _lib.ATTN_ARGS.pack(q.data_ptr(), out.data_ptr(), T, Hq, sb, st, sh, osb, ost, osh, bool(out_bf16), lim,
+                               0.125 if sm_scale is None else sm_scale, 0 if ws is None else ws.data_ptr())
+    code = lib.ress_cache_attn(cache, args, _dev_status(i), _raw_stream(i))
+    if code:
+        check(code, "ress_cache_attn")
     return out
 
 
@@ -703,14 +731,14 @@ def int8_quant_rows(x):
     """(..., K) bf16 or fp32 -> int8 of the same shape and one fp32 scale per
     row (ress_int8_quant_rows): tokens, or the output channels of a weight."""
     _dev_ok(x)
+    i = x.get_device()
     x2 = _rows2d(x)
     M, K = x2.shape
     x8 = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=_F32, device=x.device)
     if M:
-        check(_lib.load().ress_int8_quant_rows(_p(x2), _dtype_code(x.dtype), M, K, x2.stride(0) if M > 1 else K, _p(x8),
-                                               _p(scale), torch.cuda.current_stream(x.device).cuda_stream),
-              "ress_int8_quant_rows")
+        check(_lib.load().ress_int8_quant_rows(x2.data_ptr(), _dtype_code(x.dtype), M, K, x2.stride(0) if M > 1 else K,
+                                               x8.data_ptr(), scale.data_ptr(), _raw_stream(i)), "ress_int8_quant_rows")
     return x8, scale
 
 
@@ -720,29 +748,33 @@ def int8_linear(x, w8, w_scale, bias=None, *, act=None, out_dtype=None):
     weight's (int8_quant_rows lays them out once).  act: None or "gelu".
     Returns (..., N) in x's type, or out_dtype."""
     _dev_ok(x)
-    dev = x.device
-    _same_device(dev, w8, w_scale, bias)
-    if w8.dtype != torch.int8 or w8.dim() != 2 or not w8.is_contiguous():
+    i, dtype, shape, wshape = x.get_device(), x.dtype, x.shape, w8.shape
+    if w8.dtype is not torch.int8 or len(wshape) != 2 or not w8.is_contiguous():
         raise RessError("w8 must be contiguous int8 (N, K)")
-    N, K = w8.shape
-    if x.shape[-1] != K:
-        raise RessError(f"x has {x.shape[-1]} features, the weight {K}")
+    N, K = wshape
+    if shape[-1] != K:
+        raise RessError(f"x has {shape[-1]} features, the weight {K}")
+    _on_device(i, w8, w_scale, bias)
     for t in (w_scale, bias):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (N,) or not t.is_contiguous()):
+        if t is not None and (t.dtype is not _F32 or t.shape != (N,) or not t.is_contiguous()):
             raise RessError("w_scale and bias are contiguous fp32 (N,)")
-    if act not in (None, "gelu"):
+    if act is not None and act != "gelu":
         raise RessError(f"unknown activation {act!r}")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    x2 = _rows2d(x)
-    M = x2.shape[0]
-    out = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype, device=dev)
+    out_dtype = dtype if out_dtype is None else out_dtype
+    dt, odt = _dtype_code(dtype), _dtype_code(out_dtype)
+    if len(shape) != 2 or x.stride(1) != 1:
+        x = _rows2d(x)
+    M = x.shape[0]
+    out = torch.empty(shape[:-1] + (N,), dtype=out_dtype, device=x.device)
     if M == 0:
         return out
     lib = _lib.load()
     need = lib.ress_int8_linear_workspace(M, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    check(lib.ress_int8_linear(x2.data_ptr(), _dtype_code(x.dtype), M, N, K, x2.stride(0) if M > 1 else K, w8.data_ptr(),
-                               w_scale.data_ptr(), _p(bias), int(act == "gelu"), out.data_ptr(),
-                               _dtype_code(out_dtype), N, _p(ws), status_word(dev).data_ptr(),
-                               torch.cuda.current_stream(dev).cuda_stream), "ress_int8_linear")
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    code = lib.ress_int8_linear(x.data_ptr(), dt, M, N, K, x.stride(0) if M > 1 else K, w8.data_ptr(),
+                                w_scale.data_ptr(), None if bias is None else bias.data_ptr(), act is not None,
+                                out.data_ptr(), odt, N, None if ws is None else ws.data_ptr(), _dev_status(i),
+                                _raw_stream(i))
+    if code:
+        check(code, "ress_int8_linear")
     return out
