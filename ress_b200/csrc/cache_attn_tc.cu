@@ -47,6 +47,7 @@ constexpr int OFF_V = OFF_C + NC * BLOCK_BYTES;
 constexpr int OFF_P = OFF_V + NV * V_BYTES;
 constexpr int OFF_ONES = OFF_P + TILES * NP * P_BYTES;
 constexpr int SMEM = OFF_ONES + ONES_BYTES + 1024;
+static_assert(V_BYTES == 4 * 2048, "four K = 16 slices a page");
 static_assert(SMEM + 4096 <= 227 * 1024, "shared memory");
 constexpr float RESCALE_THRESH = 8.0f;
 constexpr int SPLIT_MAX = 8, PART_ROW = HD + 4;  // a partial row: O, maximum, sum
@@ -85,6 +86,12 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(IDESC_S), "r"(acc));
+}
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -348,64 +355,93 @@ __global__ void __launch_bounds__(NT, 1)
             }
         } else if (warp == 1) {
             // -------------------------------------------------------- S
-            if (lane == 0 && cnt > 0) {
+            // The whole warp runs the loop, so that descriptors stay in uniform
+            // registers; one elected lane issues.
+            if (cnt > 0) {
                 bool ok = true;
+                const bool elected = elect_one();
+                const uint64_t dq = make_desc(sQ, 16, 1024, LAYOUT_SW128), dk = make_desc(sK, 16, 512, LAYOUT_SW64);
+                int ks = 0, kphase = 0, pb = 0;
                 for (int j = 0; ok && j < cnt; ++j) {
-                    const int ks = j % NK, sb = j & 1;
-                    if (!wait_bar(&B.k_full[ks], (j / NK) & 1, abort_flag, a.status)) break;
+                    const int sb = j & 1;
+                    if (!wait_bar_warp(&B.k_full[ks], kphase, abort_flag, a.status)) break;
                     for (int t = 0; t < nt; ++t) {
-                        if (j >= 2 && !wait_bar(&B.s_free[t][sb], ((j - 2) >> 1) & 1, abort_flag, a.status)) {
+                        if (j >= 2 && !wait_bar_warp(&B.s_free[t][sb], ((j - 2) >> 1) & 1, abort_flag, a.status)) {
                             ok = false;
                             break;
                         }
                         // P_j takes the place of P_{j-NP}, whose product must be done
-                        if (j >= NP && !wait_bar(&B.o_full[t][j % NP], ((j - NP) / NP) & 1, abort_flag, a.status)) {
+                        if (j >= NP && !wait_bar_warp(&B.o_full[t][pb], ((j - NP) / NP) & 1, abort_flag, a.status)) {
                             ok = false;
                             break;
                         }
                         fence_after();
+                        if (elected) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)  // hi, hi, lo, lo against K's two halves
-                            mma_e4m3(tmem + t * 128 + sb * 64, make_desc(sQ + t * Q_BYTES + kk * 32, 16, 1024, LAYOUT_SW128),
-                                     make_desc(sK + ks * BLOCK_BYTES + (kk & 1) * 32, 16, 512, LAYOUT_SW64),
-                                     kk > 0 ? 1u : 0u);
-                        mma_commit(&B.s_full[t][sb]);
+                            for (int kk = 0; kk < 4; ++kk)  // hi, hi, lo, lo against K's two halves
+                                mma_e4m3(tmem + t * 128 + sb * 64, dq + t * (Q_BYTES >> 4) + kk * 2,
+                                         dk + ks * (BLOCK_BYTES >> 4) + (kk & 1) * 2, kk > 0 ? 1u : 0u);
+                            mma_commit(&B.s_full[t][sb]);
+                        }
+                        __syncwarp();
                     }
-                    if (ok) mma_commit(&B.k_empty[ks]);
+                    if (ok && elected) mma_commit(&B.k_empty[ks]);
+                    if (++ks == NK) {
+                        ks = 0;
+                        kphase ^= 1;
+                    }
+                    if (++pb == NP) pb = 0;
                 }
-                mma_commit(&B.s_done);  // every MMA of this thread completes before tensor memory is freed
-                const uint64_t t0 = globaltimer();
-                while (!mbar_try_wait(smem_u32(&B.s_done), 0) && globaltimer() - t0 < TIMEOUT_NS) {
+                if (elected) {
+                    mma_commit(&B.s_done);  // every MMA of this thread completes before tensor memory is freed
+                    const uint64_t t0 = globaltimer();
+                    while (!mbar_try_wait(smem_u32(&B.s_done), 0) && globaltimer() - t0 < TIMEOUT_NS) {
+                    }
                 }
             }
         } else if (warp == 2) {
             // -------------------------------------------------------- O
-            if (lane == 0 && cnt > 0) {
+            if (cnt > 0) {
                 bool ok = true;
+                const bool elected = elect_one();
+                // B = [V | ones]: the second 128-byte atom along N lies LBO bytes past the
+                // first; a step of 2048 bytes in V moves the start and the distance
+                const uint64_t dp = make_desc(smem_u32(smem + OFF_P), 16, 1024, LAYOUT_SW128);
+                const uint64_t dv = make_desc(sV, sOnes - sV, 1024, LAYOUT_SW128);
+                constexpr uint64_t V_STEP = (2048 >> 4) - ((uint64_t)(2048 >> 4) << 16);
+                int vs = 0, vphase = 0, pb = 0, pphase = 0;
                 for (int j = 0; ok && j < cnt; ++j) {
-                    const int pb = j % NP, vs = j % NV;
-                    if (!wait_bar(&B.v_full[vs], (j / NV) & 1, abort_flag, a.status)) break;
+                    if (!wait_bar_warp(&B.v_full[vs], vphase, abort_flag, a.status)) break;
                     for (int t = 0; t < nt; ++t) {
-                        if (!wait_bar(&B.p_full[t][pb], (j / NP) & 1, abort_flag, a.status)) {
+                        if (!wait_bar_warp(&B.p_full[t][pb], pphase, abort_flag, a.status)) {
                             ok = false;
                             break;
                         }
                         fence_after();
-                        const uint32_t pa = smem_u32(smem + OFF_P) + (t * NP + pb) * P_BYTES, va = sV + vs * V_BYTES;
+                        if (elected) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
-                            // B = [V | ones]: the second 128-byte atom along N lies LBO bytes past the first
-                            const uint32_t vk = va + kk * 2048;
-                            mma_f16(tmem + 256 + t * 128, make_desc(pa + kk * 32, 16, 1024, LAYOUT_SW128),
-                                    make_desc(vk, sOnes - vk, 1024, LAYOUT_SW128), IDESC_O, (j | kk) ? 1u : 0u);
+                            for (int kk = 0; kk < 4; ++kk)
+                                mma_f16(tmem + 256 + t * 128, dp + (t * NP + pb) * (P_BYTES >> 4) + kk * 2,
+                                        dv + (uint64_t)(vs * 4 + kk) * V_STEP, IDESC_O, (j | kk) ? 1u : 0u);
+                            mma_commit(&B.o_full[t][pb]);
                         }
-                        mma_commit(&B.o_full[t][pb]);
+                        __syncwarp();
                     }
-                    if (ok) mma_commit(&B.v_empty[vs]);
+                    if (ok && elected) mma_commit(&B.v_empty[vs]);
+                    if (++vs == NV) {
+                        vs = 0;
+                        vphase ^= 1;
+                    }
+                    if (++pb == NP) {
+                        pb = 0;
+                        pphase ^= 1;
+                    }
                 }
-                mma_commit(&B.pv_done);
-                const uint64_t t0 = globaltimer();
-                while (!mbar_try_wait(smem_u32(&B.pv_done), 0) && globaltimer() - t0 < TIMEOUT_NS) {
+                if (elected) {
+                    mma_commit(&B.pv_done);
+                    const uint64_t t0 = globaltimer();
+                    while (!mbar_try_wait(smem_u32(&B.pv_done), 0) && globaltimer() - t0 < TIMEOUT_NS) {
+                    }
                 }
             }
         } else if (warp >= 4) {
