@@ -406,7 +406,7 @@ int ress_cache_append(const ress_cache *cache, const ress_append_args *args, int
 /*
  * ress_cache_attn: queries q (bf16, `tokens` per stream and q_heads heads,
  * element (b, t, head) at b*q_sb + t*q_st + head*q_sh, rows 16-byte aligned)
- * over the cache: softmax(q k^T * sm_scale) v over stream b's tokens below
+ * over the cache: softmax(q k^T * sm_scale) v (sm_scale >= 0) over stream b's tokens below
  * min(lens[b], limits[b*tokens + t]) (limits NULL: lens[b] for all).  Query
  * heads are consecutive groups of q_heads / heads per key/value head.  Sums
  * and softmax statistics are fp32.  A query that sees no token gives zeros.

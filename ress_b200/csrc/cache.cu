@@ -1,12 +1,15 @@
 // cache.cu -- new tokens into the paged 8-bit cache: q/k LayerNorm, the 2-D
 // rotary embedding and the quantisation in one pass over the projection.
 //
-// One CTA per (page, key/value head, stream): 512 threads, eight per token
-// slot, so that a thread holds eight head dims of one token's k, v and q
-// (16-byte bf16 loads, all in flight before the first use).  With the page
-// in registers its largest magnitude is one reduction away, and codes are
-// written once.  All math is fp32: LayerNorm (mean, then mean of squared
-// deviations), the rotation x*cos + rotate_half(x)*sin, then
+// A CTA takes one page of a stream and a few of its heads in turn: 512
+// threads, eight per token slot.  Thread i of the eight holds dims d..d+3 and
+// d+16..d+19, d = 32*(i/4) + 4*(i%4): the two halves of a rotated pair meet
+// in one thread, the eight's loads still cover the row, and cos and sin are
+// read once for all heads.  With the page in registers its largest magnitude
+// is one reduction away, and codes are written once.  A head's rows are asked
+// for while the head before is worked on.  All math is fp32, two lanes an
+// instruction: LayerNorm (mean, then mean of squared deviations), the
+// rotation x*cos + rotate_half(x)*sin, then
 //     e = the least integer with max|y| <= 448 * 2^e,  code = e4m3(y / 2^e)
 // over the page's new tokens of that head; a page that holds tokens already
 // keeps the larger of its scale and the new one, and its old codes move by
@@ -15,7 +18,6 @@
 // Heads vary fastest in the grid: CTAs that run together read whole rows of
 // the projection.  q rows of a shared key/value head are taken in turn.
 #include "cache.cuh"
-#include "prologue.cuh"
 
 namespace ress {
 namespace cache {
@@ -39,60 +41,151 @@ struct AppendArgs {
     int32_t *status;
 };
 
-// LayerNorm (where w is given) and rotation of one row spread over eight
-// lanes, unrounded fp32 in and out.  All lanes of the warp take part.
-__device__ __forceinline__ void norm_rotate8(float (&x)[8], int c, float eps, const float *w, const float *b, bool rope,
-                                             const float (&cs)[8], const float (&sn)[8]) {
-    if (w != nullptr) {
-        prologue_row8<float>(x, c, eps, w, b, rope, cs, sn);
-    } else if (rope) {
-        const bool first = (c & 31) < 16;
+// Eight values of a row as loaded: two pieces of four, 16 dims apart.
+template <typename T> struct Raw;
+template <> struct Raw<__nv_bfloat16> {
+    uint2 u[2];
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
+        u[0] = __ldg(reinterpret_cast<const uint2 *>(p));
+        u[1] = __ldg(reinterpret_cast<const uint2 *>(p + 16));
+    }
+    __device__ __forceinline__ void clear() { u[0] = u[1] = make_uint2(0, 0); }
+    __device__ __forceinline__ void get(f32x2 (&x)[4]) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float z = __shfl_xor_sync(0xffffffffu, x[j], 2);  // feature j +- 16
-            x[j] = __fadd_rn(__fmul_rn(x[j], cs[j]), __fmul_rn(first ? -z : z, sn[j]));
+        for (int i = 0; i < 2; ++i) {
+            x[2 * i] = f2_pack(__uint_as_float(u[i].x << 16), __uint_as_float(u[i].x & 0xFFFF0000u));
+            x[2 * i + 1] = f2_pack(__uint_as_float(u[i].y << 16), __uint_as_float(u[i].y & 0xFFFF0000u));
+        }
+    }
+};
+template <> struct Raw<float> {
+    float4 u[2];
+    __device__ __forceinline__ void load(const float *p) {
+        u[0] = __ldg(reinterpret_cast<const float4 *>(p));
+        u[1] = __ldg(reinterpret_cast<const float4 *>(p + 16));
+    }
+    __device__ __forceinline__ void clear() { u[0] = u[1] = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void get(f32x2 (&x)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[2 * i] = f2_pack(u[i].x, u[i].y);
+            x[2 * i + 1] = f2_pack(u[i].z, u[i].w);
+        }
+    }
+};
+__device__ __forceinline__ void put(__nv_bfloat16 *p, const f32x2 (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float a, b, c, d;
+        f2_unpack(x[2 * i], a, b);
+        f2_unpack(x[2 * i + 1], c, d);
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(a, b), hi = __floats2bfloat162_rn(c, d);
+        *reinterpret_cast<uint2 *>(p + 16 * i) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+    }
+}
+__device__ __forceinline__ void put(float *p, const f32x2 (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float4 v;
+        f2_unpack(x[2 * i], v.x, v.y);
+        f2_unpack(x[2 * i + 1], v.z, v.w);
+        *reinterpret_cast<float4 *>(p + 16 * i) = v;
+    }
+}
+// four floats of a norm's weight or bias
+__device__ __forceinline__ void affine4(const float *p, f32x2 &a, f32x2 &b) {
+    const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+    a = f2_pack(v.x, v.y);
+    b = f2_pack(v.z, v.w);
+}
+// the sum of both lanes of x over the eight threads of a row
+__device__ __forceinline__ float row_sum(f32x2 x) {
+    float a, b;
+    f2_unpack(x, a, b);
+    a += b;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    return a;
+}
+__device__ __forceinline__ f32x2 twice(float x) { return f2_pack(x, x); }
+
+// LayerNorm (where w is given) and rotation of a row, unrounded.  All lanes of
+// the warp take part.  sn holds sin of dims 16..19 on, and -sin of dims 0..3.
+__device__ __forceinline__ void norm_rotate(f32x2 (&x)[4], int d, float eps, const float *w, const float *b, bool rope,
+                                            const f32x2 (&cs)[4], const f32x2 (&sn)[4]) {
+    if (w != nullptr) {
+        const f32x2 mean = twice(-row_sum(f2_add_rn(f2_add_rn(x[0], x[1]), f2_add_rn(x[2], x[3]))) * (1.0f / HD));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = f2_add_rn(x[i], mean);
+        f32x2 sq = f2_mul_rn(x[0], x[0]);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) sq = f2_fma_rn(x[i], x[i], sq);
+        const f32x2 rstd = twice(rsqrtf(fmaf(row_sum(sq), 1.0f / HD, eps)));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f32x2 w0, w1, b0, b1;
+            affine4(w + d + 16 * i, w0, w1);
+            affine4(b + d + 16 * i, b0, b1);
+            x[2 * i] = f2_fma_rn(f2_mul_rn(x[2 * i], rstd), w0, b0);
+            x[2 * i + 1] = f2_fma_rn(f2_mul_rn(x[2 * i + 1], rstd), w1, b1);
+        }
+    }
+    if (rope) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x2 lo = x[i], hi = x[2 + i];
+            x[i] = f2_fma_rn(lo, cs[i], f2_mul_rn(hi, sn[i]));
+            x[2 + i] = f2_fma_rn(hi, cs[2 + i], f2_mul_rn(lo, sn[2 + i]));
         }
     }
 }
 
-__device__ __forceinline__ uint32_t amax8(const float (&x)[8]) {
-    uint32_t m = 0;
+// The largest magnitude; NaN if there is one.
+__device__ __forceinline__ uint32_t amax_bits(const f32x2 (&x)[4]) {
+    float m = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);  // NaN and infinity sort last
-    return m;
+    for (int i = 0; i < 4; ++i) {
+        float a, b;
+        f2_unpack(x[i], a, b);
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(a)));
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(b)));
+    }
+    return __float_as_uint(m) & 0x7FFFFFFFu;
 }
 
 // f = 0 (a page of NaN scale) writes zeros whatever x holds, so that no code is ever NaN
-__device__ __forceinline__ void store_codes(uint8_t *dst, const float (&x)[8], float f) {
-    if (f == 0.0f) {
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(0, 0);
-        return;
-    }
-    const uint32_t lo = e4m3x4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
-    const uint32_t hi = e4m3x4(x[4] * f, x[5] * f, x[6] * f, x[7] * f);
-    *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
-}
-
-__device__ __forceinline__ void move_codes(uint8_t *p, float f) {
-    const uint2 old = *reinterpret_cast<const uint2 *>(p);
-    float x[8];
-    const uint32_t w[2] = {old.x, old.y};
+__device__ __forceinline__ void store_codes(uint8_t *p, const f32x2 (&x)[4], float f) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t h = e4m3_to_half2((uint16_t)(w[j >> 1] >> ((j & 1) * 16)));
-        const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-        x[2 * j] = v.x;
-        x[2 * j + 1] = v.y;
+    for (int i = 0; i < 2; ++i) {
+        float a, b, c, d;
+        f2_unpack(f2_mul_rn(x[2 * i], twice(f)), a, b);
+        f2_unpack(f2_mul_rn(x[2 * i + 1], twice(f)), c, d);
+        *reinterpret_cast<uint32_t *>(p + 16 * i) = f == 0.0f ? 0u : e4m3x4(a, b, c, d);
+    }
+}
+__device__ __noinline__ void move_codes(uint8_t *p, float f) {
+    f32x2 x[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(p + 16 * i);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t h = e4m3_to_half2((uint16_t)(w >> (16 * j)));
+            const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+            x[2 * i + j] = f2_pack(v.x, v.y);
+        }
     }
     store_codes(p, x, f);
 }
 
+// heads: of the cache; the CTA takes [blockIdx.x * per, .. + per) of them.
 template <typename T>
-__global__ void __launch_bounds__(APP_NT) append_kernel(const AppendArgs a) {
-    __shared__ uint32_t red[2][APP_NT / 32];
-    const int h = blockIdx.x, b = blockIdx.z;
+__global__ void __launch_bounds__(APP_NT, sizeof(T) == 2 ? 2 : 1) append_kernel(const AppendArgs a, int heads, int per) {
+    __shared__ uint32_t red[2][2][APP_NT / 32];
+    const int b = blockIdx.z;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int slot = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;
+    const int slot = threadIdx.x >> 3, i8 = threadIdx.x & 7, d = (i8 >> 2) * 32 + (i8 & 3) * 4;
     const int len_raw = a.lens[b];
     const int len = max(len_raw, 0);
     const int fill = len % PAGE;
@@ -101,21 +194,38 @@ __global__ void __launch_bounds__(APP_NT) append_kernel(const AppendArgs a) {
     const bool row = t >= 0 && t < a.T;  // there is a q row (written for padding tokens as well)
     const bool fresh = t >= 0 && t < n_new;
     if (blockIdx.y > 0 && (int)blockIdx.y * PAGE - fill >= a.T) return;
+    const int h0 = blockIdx.x * per, h1 = min(h0 + per, heads);
 
-    float xk[8] = {}, xv[8] = {}, xq[8] = {}, cs[8] = {}, sn[8] = {};
-    const bool rope = a.cos != nullptr;
-    if (fresh) {
-        load8(reinterpret_cast<const T *>(a.k) + b * a.k_sb + t * a.k_st + h * a.k_sh + c, xk);
-        load8(reinterpret_cast<const T *>(a.v) + b * a.v_sb + t * a.v_st + h * a.v_sh + c, xv);
-    }
-    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.q_sb + t * a.q_st + (long long)h * a.group * a.q_sh + c;
-    const bool has_q = a.q != nullptr;
-    if (has_q && row) load8(qp, xq);
+    const T *kp = reinterpret_cast<const T *>(a.k) + b * a.k_sb + t * a.k_st + d;
+    const T *vp = reinterpret_cast<const T *>(a.v) + b * a.v_sb + t * a.v_st + d;
+    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.q_sb + t * a.q_st + d;
+    const bool has_q = a.q != nullptr, rope = a.cos != nullptr;
+    Raw<T> rk, rv, rq;
+    rk.clear();
+    rv.clear();
+    rq.clear();
+    auto ask_kv = [&](int h) {
+        if (fresh) {
+            rk.load(kp + h * a.k_sh);
+            rv.load(vp + h * a.v_sh);
+        }
+    };
+    auto ask_q = [&](int h) {
+        if (has_q && row) rq.load(qp + (long long)h * a.group * a.q_sh);
+    };
+    ask_kv(h0);
+    ask_q(h0);
+    f32x2 cs[4] = {}, sn[4] = {};
     if (rope && row) {
-        const long long pa = a.pos[((long long)b * a.T + t) * 2 + (c >> 5)];
+        const long long pa = a.pos[((long long)b * a.T + t) * 2 + (d >> 5)];
         const int p = (int)(pa < 0 ? 0 : (pa >= a.rope_len ? a.rope_len - 1 : pa));
-        load8(reinterpret_cast<const T *>(a.cos) + (size_t)p * 32 + (c & 31), cs);
-        load8(reinterpret_cast<const T *>(a.sin) + (size_t)p * 32 + (c & 31), sn);
+        Raw<T> rc, rs;
+        rc.load(reinterpret_cast<const T *>(a.cos) + (size_t)p * 32 + (d & 31));
+        rs.load(reinterpret_cast<const T *>(a.sin) + (size_t)p * 32 + (d & 31));
+        rc.get(cs);
+        rs.get(sn);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sn[i] ^= 0x8000000080000000ull;
     }
     // the page this CTA writes, if any token falls into it
     const long long at = (long long)(len / PAGE) + blockIdx.y;
@@ -124,49 +234,57 @@ __global__ void __launch_bounds__(APP_NT) append_kernel(const AppendArgs a) {
     if (any && at < a.table_width) page = a.table[b * a.table_stride + at];
     const bool ok = page >= 0 && page < a.n_pages && len_raw >= 0;
     if (any && !ok && threadIdx.x == 0) atomicOr(a.status, RESS_STATUS_CACHE_RANGE);
-
-    norm_rotate8(xk, c, a.eps, a.kw, a.kb, rope, cs, sn);
-    if (!fresh) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) xk[j] = 0.0f;
-    }
-    const uint32_t mk = __reduce_max_sync(0xffffffffu, amax8(xk)), mv = __reduce_max_sync(0xffffffffu, amax8(xv));
-    if (lane == 0) {
-        red[0][warp] = mk;
-        red[1][warp] = mv;
-    }
-    // the scales of a page that holds tokens already, read before anyone writes them
     const bool held = blockIdx.y == 0 && fill > 0;
-    int old_k = 0, old_v = 0;
-    if (ok && held) {
-        old_k = a.K.scale[page * a.K.scale_stride + h];
-        old_v = a.V.scale[page * a.V.scale_stride + h];
-    }
-    __syncthreads();
-    if (ok) {
-        const uint32_t rk = __reduce_max_sync(0xffffffffu, red[0][lane & 15]);
-        const uint32_t rv = __reduce_max_sync(0xffffffffu, red[1][lane & 15]);
-        const int uk = max(scale_code(rk), old_k), uv = max(scale_code(rv), old_v);
-        uint8_t *pk = a.K.codes + page * a.K.page_stride + h * a.K.head_stride + slot * HD + c;
-        uint8_t *pv = a.V.codes + page * a.V.page_stride + h * a.V.head_stride + slot * HD + c;
-        if (fresh) {
-            store_codes(pk, xk, scale_inverse(uk));
-            store_codes(pv, xv, scale_inverse(uv));
-        } else if (held && slot < fill) {
-            if (uk != old_k) move_codes(pk, scale_value(old_k) * scale_inverse(uk));
-            if (uv != old_v) move_codes(pv, scale_value(old_v) * scale_inverse(uv));
+
+    for (int h = h0; h < h1; ++h) {
+        f32x2 xk[4], xv[4];
+        rk.get(xk);
+        const Raw<T> v_now = rv;  // as loaded: half the registers
+        if (h + 1 < h1) ask_kv(h + 1);
+        norm_rotate(xk, d, a.eps, a.kw, a.kb, rope, cs, sn);
+        uint32_t (*r)[APP_NT / 32] = red[h & 1];  // the other one may still be read
+        const uint32_t mk = __reduce_max_sync(0xffffffffu, fresh ? amax_bits(xk) : 0u);
+        v_now.get(xv);
+        const uint32_t mv = __reduce_max_sync(0xffffffffu, fresh ? amax_bits(xv) : 0u);
+        if (lane == 0) {
+            r[0][warp] = mk;
+            r[1][warp] = mv;
         }
-        if (threadIdx.x == 0) {
-            a.K.scale[page * a.K.scale_stride + h] = (uint8_t)uk;
-            a.V.scale[page * a.V.scale_stride + h] = (uint8_t)uv;
+        // the scales of a page that holds tokens already, read before anyone writes them
+        int old_k = 0, old_v = 0;
+        if (ok && held) {
+            old_k = a.K.scale[page * a.K.scale_stride + h];
+            old_v = a.V.scale[page * a.V.scale_stride + h];
         }
-    }
-    if (!has_q) return;
-    T *qo = reinterpret_cast<T *>(a.q_out) + (((long long)b * a.T + t) * gridDim.x + h) * a.group * HD + c;
-    for (int g = 0; g < a.group; ++g) {
-        if (g > 0 && row) load8(qp + g * a.q_sh, xq);
-        norm_rotate8(xq, c, a.eps, a.qw, a.qb, rope, cs, sn);
-        if (row) store8(qo + (long long)g * HD, xq);
+        __syncthreads();
+        if (ok) {
+            const int uk = max(scale_code(__reduce_max_sync(0xffffffffu, r[0][lane & 15])), old_k);
+            const int uv = max(scale_code(__reduce_max_sync(0xffffffffu, r[1][lane & 15])), old_v);
+            uint8_t *pk = a.K.codes + page * a.K.page_stride + h * a.K.head_stride + slot * HD + d;
+            uint8_t *pv = a.V.codes + page * a.V.page_stride + h * a.V.head_stride + slot * HD + d;
+            if (fresh) {
+                store_codes(pk, xk, scale_inverse(uk));
+                v_now.get(xv);
+                store_codes(pv, xv, scale_inverse(uv));
+            } else if (held && slot < fill) {
+                if (uk != old_k) move_codes(pk, scale_value(old_k) * scale_inverse(uk));
+                if (uv != old_v) move_codes(pv, scale_value(old_v) * scale_inverse(uv));
+            }
+            if (threadIdx.x == 0) {
+                a.K.scale[page * a.K.scale_stride + h] = (uint8_t)uk;
+                a.V.scale[page * a.V.scale_stride + h] = (uint8_t)uv;
+            }
+        }
+        if (!has_q) continue;
+        T *qo = reinterpret_cast<T *>(a.q_out) + (((long long)b * a.T + t) * heads + h) * a.group * HD + d;
+        for (int g = 0; g < a.group; ++g) {
+            f32x2 xq[4];
+            if (g > 0 && row) rq.load(qp + ((long long)h * a.group + g) * a.q_sh);
+            rq.get(xq);
+            if (g + 1 == a.group && h + 1 < h1) ask_q(h + 1);
+            norm_rotate(xq, d, a.eps, a.qw, a.qb, rope, cs, sn);
+            if (row) put(qo + (long long)g * HD, xq);
+        }
     }
 }
 
@@ -188,10 +306,11 @@ extern "C" int ress_cache_append(const ress_cache *cache, const ress_append_args
     if ((g.rope_cos == nullptr) != (g.rope_sin == nullptr) || (g.rope_cos != nullptr && (!g.pos || g.rope_len <= 0)))
         return RESS_E_ARG;
     if (g.dtype != RESS_BF16 && g.dtype != RESS_F32) return RESS_E_DTYPE;
-    // 16-byte loads of eight elements
+    // loads of up to 16 bytes
     const int size = g.dtype == RESS_BF16 ? 2 : 4;
     if (((uintptr_t)g.q | (uintptr_t)g.k | (uintptr_t)g.v | (uintptr_t)g.q_out | (uintptr_t)g.rope_cos |
-         (uintptr_t)g.rope_sin) & 15)
+         (uintptr_t)g.rope_sin | (uintptr_t)g.qn_weight | (uintptr_t)g.qn_bias | (uintptr_t)g.kn_weight |
+         (uintptr_t)g.kn_bias) & 15)
         return RESS_E_ARG;
     if (((g.k_sb | g.k_st | g.k_sh | g.v_sb | g.v_st | g.v_sh) * size) & 15) return RESS_E_ARG;
     if (g.q && ((g.q_sb | g.q_st | g.q_sh) * size) & 15) return RESS_E_ARG;
@@ -214,10 +333,16 @@ extern "C" int ress_cache_append(const ress_cache *cache, const ress_append_args
     a.K = {cache->k_pages, cache->k_scale, cache->page_stride, cache->head_stride, cache->scale_stride};
     a.V = {cache->v_pages, cache->v_scale, cache->page_stride, cache->head_stride, cache->scale_stride};
     a.status = status;
-    const dim3 grid((unsigned)cache->heads, (unsigned)pages, (unsigned)cache->streams);
+    // heads a CTA takes in turn: one while the CTAs fit on the GPU at once
+    // (two per SM), up to four beyond that, where it hides a head's loads
+    const int64_t ctas = cache->heads * pages * cache->streams;
+    int per = 1;
+    while (per < 4 && ctas / (2 * per) >= 2 * 148) per *= 2;
+    const int heads = (int)cache->heads;
+    const dim3 grid((unsigned)((heads + per - 1) / per), (unsigned)pages, (unsigned)cache->streams);
     if (g.dtype == RESS_BF16)
-        cache::append_kernel<__nv_bfloat16><<<grid, cache::APP_NT, 0, (cudaStream_t)stream>>>(a);
+        cache::append_kernel<__nv_bfloat16><<<grid, cache::APP_NT, 0, (cudaStream_t)stream>>>(a, heads, per);
     else
-        cache::append_kernel<float><<<grid, cache::APP_NT, 0, (cudaStream_t)stream>>>(a);
+        cache::append_kernel<float><<<grid, cache::APP_NT, 0, (cudaStream_t)stream>>>(a, heads, per);
     return cudaGetLastError() == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
 }

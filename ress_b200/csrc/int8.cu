@@ -37,12 +37,44 @@ __device__ __forceinline__ int round_s8(float x) {
     asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(r) : "f"(x));
     return r;
 }
-// d: the scale, or 1 where it is 0.  |x / d| rounds to 127 at most (a scale
-// among the subnormals can be off by more; the conversion saturates).
-__device__ __forceinline__ uint32_t quant4(float a, float b, float c, float e, float d) {
-    const int q0 = round_s8(__fdiv_rn(a, d)), q1 = round_s8(__fdiv_rn(b, d));
-    const int q2 = round_s8(__fdiv_rn(c, d)), q3 = round_s8(__fdiv_rn(e, d));
-    return __byte_perm(__byte_perm(q0, q1, 0x0040), __byte_perm(q2, q3, 0x0040), 0x5410);
+// How a row's values become codes: x / d rounded to the nearest integer, d
+// the scale or 1 where that is 0 or NaN.  The quotient is the correctly
+// rounded one (div_by in common.cuh, two lanes at a time), the integer the
+// low byte of quotient + 1.5 * 2^23.  Scales so small that the division's
+// remainder would be subnormal take the plain division and a saturating
+// conversion (a subnormal scale can be off by more than a half code).
+struct RowQuant {
+    float d;
+    f32x2 r, nd;
+    bool tiny;
+};
+__device__ __forceinline__ RowQuant row_quant(float scale) {
+    const float d = scale > 0.0f ? scale : 1.0f, r = __frcp_rn(d);
+    return {d, f2_pack(r, r), f2_pack(-d, -d), d < 7.9e-31f};
+}
+__device__ __forceinline__ uint2 quant8(const float (&x)[8], const RowQuant &q) {
+    uint32_t c[8];
+    if (q.tiny) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = (uint32_t)round_s8(__fdiv_rn(x[j], q.d));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const f32x2 a = f2_pack(x[j], x[j + 1]), y = f2_mul_rn(a, q.r);
+            const f32x2 z = f2_fma_rn(f2_fma_rn(y, q.nd, a), q.r, y);
+            float u, v;
+            f2_unpack(f2_add_rn(z, 0x4B4000004B400000ull), u, v);
+            c[j] = __float_as_uint(u);
+            c[j + 1] = __float_as_uint(v);
+        }
+    }
+    return make_uint2(pack_low_bytes(c[0], c[1], c[2], c[3]), pack_low_bytes(c[4], c[5], c[6], c[7]));
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t amax8(const float (&x)[8]) {
     uint32_t m = 0;
@@ -51,16 +83,68 @@ __device__ __forceinline__ uint32_t amax8(const float (&x)[8]) {
     return m;
 }
 
-__device__ __forceinline__ float finish(int acc, float sx, float sw, float bias, int gelu) {
-    float y = __fmaf_rn(__fmul_rn((float)acc, sx), sw, bias);
-    if (gelu) y = 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
-    return y;
+// GELU y Phi(y) by erfc's rational approximation (M. Abramowitz and I. Stegun,
+// Handbook of Mathematical Functions, 7.1.26: |error| <= 1.5e-7):
+// Phi(-|y|) = 1/2 (a1 t + .. + a5 t^5) exp(-y^2/2), t = 1 / (1 + p |y| / sqrt 2).
+__device__ __forceinline__ float gelu(float y) {
+    const float u = fabsf(y);
+    float t, e;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(u, 0.3275911f * 0.70710678f, 1.0f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u * u * (-0.5f * 1.44269504f)));
+    float p = 0.5f * 1.061405429f;
+    p = fmaf(p, t, 0.5f * -1.453152027f);
+    p = fmaf(p, t, 0.5f * 1.421413741f);
+    p = fmaf(p, t, 0.5f * -0.284496736f);
+    p = fmaf(p, t, 0.5f * 0.254829592f);
+    const float g = fminf(u, 1e30f) * (p * t * e);  // |y| Phi(-|y|); 0 for an infinite y
+    return fmaxf(y, 0.0f) - g;
+}
+__device__ __forceinline__ float finish(int acc, float sx, float sw, float bias, int act) {
+    const float y = __fmaf_rn(__fmul_rn((float)acc, sx), sw, bias);
+    return act ? gelu(y) : y;
 }
 
-// Rows to int8 with one scale each: one warp per row, the row read twice
-// (the second time from the caches).
+// Rows to int8 with one scale each: one warp per row, eight values a lane at
+// a time.  CH > 0: the row (at most 256 * CH values) stays in registers
+// between its maximum and its codes; CH = 0: it is read again.
 constexpr int QUANT_NT = 256;
-template <typename T>
+template <typename T> struct Piece;  // eight values as loaded
+template <> struct Piece<__nv_bfloat16> {
+    uint4 u;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { u = __ldg(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void clear() { u = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[2 * j] = __uint_as_float(w[j] << 16);
+            x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        }
+    }
+    // bits of the largest magnitude
+    __device__ __forceinline__ uint32_t amax() const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = max(m, max((w[j] << 16) & 0x7FFFFFFFu, w[j] & 0x7FFF0000u));
+        return m;
+    }
+};
+template <> struct Piece<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float *p) { load8(p, v); }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = v[j];
+    }
+    __device__ __forceinline__ uint32_t amax() const { return amax8(v); }
+};
+
+template <typename T, int CH>
 __global__ void __launch_bounds__(QUANT_NT) quant_rows_kernel(const T *__restrict__ x, long long x_st, int M, int K,
                                                               int8_t *__restrict__ q, float *__restrict__ scale) {
     const int lane = threadIdx.x & 31;
@@ -68,95 +152,151 @@ __global__ void __launch_bounds__(QUANT_NT) quant_rows_kernel(const T *__restric
     if (m >= M) return;
     const T *row = x + m * x_st;
     uint32_t am = 0;
-    for (int k = lane * 8; k < K; k += 256) {
-        float v[8];
-        load8(row + k, v);
-        am = max(am, amax8(v));
+    Piece<T> piece[CH > 0 ? CH : 1];
+    if constexpr (CH > 0) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int k = i * 256 + lane * 8;
+            if (k < K) piece[i].load(row + k);
+            else piece[i].clear();
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) am = max(am, piece[i].amax());
+    } else {
+        for (int k = lane * 8; k < K; k += 256) {
+            piece[0].load(row + k);
+            am = max(am, piece[0].amax());
+        }
     }
     am = __reduce_max_sync(0xffffffffu, am);
-    const float s = row_scale(am), d = s > 0.0f ? s : 1.0f;
-    for (int k = lane * 8; k < K; k += 256) {
-        float v[8];
-        load8(row + k, v);
-        *reinterpret_cast<uint2 *>(q + m * K + k) =
-            make_uint2(quant4(v[0], v[1], v[2], v[3], d), quant4(v[4], v[5], v[6], v[7], d));
-    }
+    const float s = row_scale(am);
+    const RowQuant rq = row_quant(s);
     if (lane == 0) scale[m] = s;
+    int8_t *qr = q + m * K;
+    float v[8];
+    if constexpr (CH > 0) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int k = i * 256 + lane * 8;
+            piece[i].get(v);
+            if (k < K) *reinterpret_cast<uint2 *>(qr + k) = quant8(v, rq);
+        }
+    } else {
+        for (int k = lane * 8; k < K; k += 256) {
+            piece[0].load(row + k);
+            piece[0].get(v);
+            *reinterpret_cast<uint2 *>(qr + k) = quant8(v, rq);
+        }
+    }
 }
 
 // ------------------------------------------------------------------ few rows
-// Sixteen tokens a CTA: they are quantised into shared memory by every CTA
-// (they are few, and no second launch is needed), each warp then streams
-// eight weight rows through mma.sync.m16n8k32 straight from global memory.
-// A lane's 16-byte piece of a row serves two k-steps.
-constexpr int FEW_NT = 128, FEW_M = 16;
+// Up to sixteen tokens: the weights' bytes (and the latency of a launch) are
+// the bound.  A CTA takes 16 channels, its eight warps an eighth of K each, as
+// mma.sync.m16n8k32 on two channel tiles; a lane's 16-byte piece of a weight
+// row serves two k-steps.  The first weights are asked for before anything
+// else; meanwhile every CTA quantises the tokens into shared memory (they
+// are few, and no second launch is needed).  The warps' int32 sums are
+// exact, so their order does not matter.
+constexpr int FEW_NT = 256, FEW_WARPS = 8, FEW_M = 16, FEW_N = 16, FEW_AHEAD = 4;
 template <typename T, typename O>
 __global__ void __launch_bounds__(FEW_NT) few_kernel(const T *__restrict__ x, long long x_st, const LinArgs a) {
     extern __shared__ __align__(16) unsigned char xs[];  // FEW_M rows of Kp + 16 bytes
     __shared__ float sx[FEW_M];
+    __shared__ uint32_t top[FEW_WARPS];
+    __shared__ int sums[FEW_WARPS][FEW_M][FEW_N + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const int m0 = blockIdx.y * FEW_M;
+    const int n0 = blockIdx.x * FEW_N;
     const int Kp = (a.K + 63) & ~63, pitch = Kp + 16;
-    for (int r = warp; r < FEW_M; r += FEW_NT / 32) {
-        const int m = m0 + r;
+    // this warp's 64-wide steps of K
+    const int steps = Kp / 64, s0 = steps * warp / FEW_WARPS, s1 = steps * (warp + 1) / FEW_WARPS;
+    const int8_t *w0 = a.w + (long long)min(n0 + g, a.N - 1) * a.K + t * 16;
+    const int8_t *w1 = a.w + (long long)min(n0 + 8 + g, a.N - 1) * a.K + t * 16;
+    auto weight = [&](const int8_t *w, int s) {
+        return s < s1 && s * 64 + t * 16 < a.K ? __ldg(reinterpret_cast<const uint4 *>(w + s * 64)) : make_uint4(0, 0, 0, 0);
+    };
+    uint4 b0[FEW_AHEAD], b1[FEW_AHEAD];
+#pragma unroll
+    for (int i = 0; i < FEW_AHEAD; ++i) {
+        b0[i] = weight(w0, s0 + i);
+        b1[i] = weight(w1, s0 + i);
+    }
+    // `per` warps share a token
+    const int per = a.M >= 8 ? 1 : a.M >= 4 ? 2 : a.M >= 2 ? 4 : 8, sub = warp % per;
+    for (int r0 = 0; r0 < FEW_M; r0 += FEW_WARPS / per) {
+        const int r = r0 + warp / per;
+        if (r0 >= a.M) {  // rows without a token
+            for (int k = sub * 256 + lane * 8; k < Kp; k += 256 * per)
+                *reinterpret_cast<uint2 *>(xs + r * pitch + k) = make_uint2(0, 0);
+            continue;
+        }
+        const T *row = x + (long long)min(r, a.M - 1) * x_st;
         uint32_t am = 0;
-        const T *row = x + (long long)m * x_st;
-        if (m < a.M)
-            for (int k = lane * 8; k < a.K; k += 256) {
-                float v[8];
-                load8(row + k, v);
-                am = max(am, amax8(v));
-            }
+        Piece<T> p;
+        for (int k = sub * 256 + lane * 8; k < a.K; k += 256 * per) {
+            p.load(row + k);
+            am = max(am, p.amax());
+        }
         am = __reduce_max_sync(0xffffffffu, am);
-        const float s = row_scale(am), d = s > 0.0f ? s : 1.0f;
-        for (int k = lane * 8; k < Kp; k += 256) {
+        if (per > 1) {
+            if (lane == 0) top[warp] = am;
+            __syncthreads();
+            for (int i = 0; i < per; ++i) am = max(am, top[warp - sub + i]);
+            __syncthreads();
+        }
+        const float s = row_scale(am);
+        const RowQuant rq = row_quant(s);
+        for (int k = sub * 256 + lane * 8; k < Kp; k += 256 * per) {
             uint2 w = make_uint2(0, 0);
-            if (m < a.M && k < a.K) {
+            if (k < a.K) {
                 float v[8];
-                load8(row + k, v);
-                w = make_uint2(quant4(v[0], v[1], v[2], v[3], d), quant4(v[4], v[5], v[6], v[7], d));
+                p.load(row + k);
+                p.get(v);
+                w = quant8(v, rq);
             }
             *reinterpret_cast<uint2 *>(xs + r * pitch + k) = w;
         }
-        if (lane == 0) sx[r] = s;
+        if (lane == 0 && sub == 0) sx[r] = s;
     }
     __syncthreads();
-    const int n0 = (blockIdx.x * (FEW_NT / 32) + warp) * 8;
-    if (n0 >= a.N) return;
-    const int n = n0 + g;
-    const int8_t *wr = a.w + (long long)min(n, a.N - 1) * a.K;
-    int c[4] = {};
-#pragma unroll 4
-    for (int k = t * 16; k < Kp; k += 64) {
-        const uint4 b = k < a.K ? __ldg(reinterpret_cast<const uint4 *>(wr + k)) : make_uint4(0, 0, 0, 0);
-        const uint4 p = *reinterpret_cast<const uint4 *>(xs + g * pitch + k);
-        const uint4 q = *reinterpret_cast<const uint4 *>(xs + (g + 8) * pitch + k);
-        asm volatile(
-            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-            : "r"(p.x), "r"(q.x), "r"(p.y), "r"(q.y), "r"(b.x), "r"(b.y));
-        asm volatile(
-            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-            : "r"(p.z), "r"(q.z), "r"(p.w), "r"(q.w), "r"(b.z), "r"(b.w));
+    int c[2][4] = {};
+    for (int s = s0; s < s1; s += FEW_AHEAD) {
+#pragma unroll
+        for (int i = 0; i < FEW_AHEAD; ++i) {
+            if (s + i < s1) {
+                const int k = (s + i) * 64 + t * 16;
+                const uint4 p = *reinterpret_cast<const uint4 *>(xs + g * pitch + k);
+                const uint4 q = *reinterpret_cast<const uint4 *>(xs + (g + 8) * pitch + k);
+                mma_s8(c[0], p.x, q.x, p.y, q.y, b0[i].x, b0[i].y);
+                mma_s8(c[1], p.x, q.x, p.y, q.y, b1[i].x, b1[i].y);
+                mma_s8(c[0], p.z, q.z, p.w, q.w, b0[i].z, b0[i].w);
+                mma_s8(c[1], p.z, q.z, p.w, q.w, b1[i].z, b1[i].w);
+            }
+            b0[i] = weight(w0, s + i + FEW_AHEAD);
+            b1[i] = weight(w1, s + i + FEW_AHEAD);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = g + (i >> 1) * 8, col = n0 + 2 * t + (i & 1);
-        if (m0 + r < a.M && col < a.N) {
-            const float y = finish(c[i], sx[r], a.w_scale[col], a.bias != nullptr ? a.bias[col] : 0.0f, a.gelu);
-            DT<O>::store(reinterpret_cast<O *>(a.out), (size_t)((m0 + r) * a.out_st + col), y);
-        }
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[warp][g + (i >> 1) * 8][u * 8 + 2 * t + (i & 1)] = c[u][i];
+    __syncthreads();
+    const int r = threadIdx.x / FEW_N, col = threadIdx.x % FEW_N, n = n0 + col;
+    if (r < a.M && n < a.N) {
+        int acc = 0;
+#pragma unroll
+        for (int w = 0; w < FEW_WARPS; ++w) acc += sums[w][r][col];
+        const float y = finish(acc, sx[r], a.w_scale[n], a.bias != nullptr ? a.bias[n] : 0.0f, a.gelu);
+        DT<O>::store(reinterpret_cast<O *>(a.out), (size_t)(r * a.out_st + n), y);
     }
 }
 
 template <typename T, typename O>
 static int launch_few(const void *x, long long x_st, const LinArgs &a, cudaStream_t s) {
     const size_t smem = (size_t)FEW_M * (((a.K + 63) & ~63) + 16);
-    set_smem_attr((const void *)few_kernel<T, O>, smem);
-    const dim3 grid((a.N + 31) / 32, (a.M + FEW_M - 1) / FEW_M);
-    few_kernel<T, O><<<grid, FEW_NT, smem, s>>>((const T *)x, x_st, a);
+    if (smem > 32 * 1024) set_smem_attr((const void *)few_kernel<T, O>, smem);
+    few_kernel<T, O><<<(a.N + FEW_N - 1) / FEW_N, FEW_NT, smem, s>>>((const T *)x, x_st, a);
     return cudaGetLastError() == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
 }
 
@@ -166,17 +306,18 @@ static int launch_few(const void *x, long long x_st, const LinArgs &a, cudaStrea
 // cluster on one tile: each loads its half of the tokens and of the channels,
 // so a tile's operands cross from L2 once per pair.  Persistent CTAs (pairs)
 // take tiles in turn, channel tiles fastest, so that the CTAs that run
-// together share token rows in L2.  Eight warps:
+// together share token rows in L2.  Twelve warps:
 //   warp 0     loads K slices of 128 bytes (TMA, 128B swizzle) into a ring;
 //   warp 1     issues the MMAs (the pair's first CTA only, when paired);
 //   warp 2     allocates tensor memory;
-//   warps 4-7  epilogue: accumulators of one of two buffers to registers,
+//   warps 4-11 epilogue: accumulators of one of two buffers to registers,
 //              scales, bias, GELU, one rounding, shared memory, TMA store,
-//              while the next tile is accumulated into the other buffer.
+//              while the next tile is accumulated into the other buffer; two
+//              warps share a quarter of the rows and take its columns in turn.
 using namespace tc;
 
 template <int CG, int BN, typename O> struct Tile {
-    static constexpr int NT = 256, BK = 128;
+    static constexpr int NT = 384, BK = 128;
     static constexpr int A_BYTES = 128 * BK, B_ROWS = BN / CG, B_BYTES = B_ROWS * BK;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int OUT_COLS = 128 / (int)sizeof(O);  // one 128-byte swizzled row
@@ -184,7 +325,7 @@ template <int CG, int BN, typename O> struct Tile {
     static constexpr int RING = 196608;
     static constexpr int NS = RING / STAGE < 8 ? RING / STAGE : 8;
     static constexpr int OFF_OUT = NS * STAGE;
-    static constexpr int SMEM = OFF_OUT + 4 * 2 * OUT_BYTES + 1024;
+    static constexpr int SMEM = OFF_OUT + 8 * OUT_BYTES + 1024;
     static constexpr uint32_t COLS = 2 * BN;  // two accumulators
     static constexpr uint32_t IDESC =
         (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((128 * CG) >> 4) << 24);
@@ -266,7 +407,7 @@ struct GemmBars {
 };
 
 template <int CG, int BN, typename O>
-__global__ void __launch_bounds__(256, 1) gemm_kernel(const __grid_constant__ CUtensorMap tm_x,
+__global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CUtensorMap tm_x,
                                                       const __grid_constant__ CUtensorMap tm_w,
                                                       const __grid_constant__ CUtensorMap tm_o, const LinArgs a,
                                                       const float *__restrict__ sx, int tma_out, int32_t *status) {
@@ -289,7 +430,7 @@ __global__ void __launch_bounds__(256, 1) gemm_kernel(const __grid_constant__ CU
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B.acc_full[i], 1);
-            mbar_init(&B.acc_free[i], 4 * CG);
+            mbar_init(&B.acc_free[i], 8 * CG);
         }
         B.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -368,10 +509,10 @@ __global__ void __launch_bounds__(256, 1) gemm_kernel(const __grid_constant__ CU
             }
         }
     } else if (warp >= 4) {
-        const int quad = warp & 3;
-        unsigned char *out_s = smem + C::OFF_OUT + quad * 2 * C::OUT_BYTES;
+        const int quad = warp & 3, half = (warp >> 2) - 1;
+        unsigned char *out_s = smem + C::OFF_OUT + (warp - 4) * C::OUT_BYTES;
         const uint32_t out_a = smem_u32(out_s);
-        int n = 0, ob = 0;
+        int n = 0;
         for (int tile = first; tile < tiles; tile += step, ++n) {
             const int buf = n & 1;
             const int m0 = (tile / tiles_n) * 128 * CG + rank * 128 + quad * 32, n0 = (tile % tiles_n) * BN;
@@ -381,10 +522,10 @@ __global__ void __launch_bounds__(256, 1) gemm_kernel(const __grid_constant__ CU
             fence_after();
             const uint32_t tq = tmem + buf * BN + ((uint32_t)(quad * 32) << 16);
 #pragma unroll 1
-            for (int c = 0; c < BN; c += C::OUT_COLS, ob ^= 1) {
+            for (int c = half * C::OUT_COLS; c < BN; c += 2 * C::OUT_COLS) {
                 if (n0 + c >= a.N) break;
-                // the buffer written two pieces ago has been read by its store
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                // the piece written before has been read by its store
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 __syncwarp();
 #pragma unroll
                 for (int part = 0; part < C::OUT_COLS; part += 32) {
@@ -434,7 +575,7 @@ __global__ void __launch_bounds__(256, 1) gemm_kernel(const __grid_constant__ CU
                                 w = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                             }
                             const int piece = (part + i) / PER;
-                            *reinterpret_cast<uint4 *>(out_s + ob * C::OUT_BYTES + lane * 128 + ((piece ^ (lane & 7)) << 4)) = w;
+                            *reinterpret_cast<uint4 *>(out_s + lane * 128 + ((piece ^ (lane & 7)) << 4)) = w;
                         }
                     } else if (m < a.M) {
 #pragma unroll
@@ -448,7 +589,7 @@ __global__ void __launch_bounds__(256, 1) gemm_kernel(const __grid_constant__ CU
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0 && m0 < a.M) {
-                        tma_store_2d(&tm_o, out_a + ob * C::OUT_BYTES, n0 + c, m0);
+                        tma_store_2d(&tm_o, out_a, n0 + c, m0);
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                 }
@@ -527,7 +668,12 @@ static int launch_gemm(const int8_t *x8, const float *sx, const LinArgs &a, int3
 template <typename T>
 static int launch_quant(const T *x, long long x_st, int M, int K, int8_t *x8, float *scale, cudaStream_t s) {
     const unsigned blocks = (unsigned)(((long long)M * 32 + QUANT_NT - 1) / QUANT_NT);
-    quant_rows_kernel<<<blocks, QUANT_NT, 0, s>>>(x, x_st, M, K, x8, scale);
+    constexpr int MOST = sizeof(T) == 2 ? 16 : 8;  // 64 registers of a row
+    auto kern = K <= 1024        ? quant_rows_kernel<T, 4>
+                : K <= 2048      ? quant_rows_kernel<T, 8>
+                : K <= 256 * MOST ? quant_rows_kernel<T, MOST>
+                                  : quant_rows_kernel<T, 0>;
+    kern<<<blocks, QUANT_NT, 0, s>>>(x, x_st, M, K, x8, scale);
     return cudaGetLastError() == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
 }
 
@@ -538,6 +684,35 @@ static size_t workspace(int M, int K) {
     return use_few(M, K) ? 0 : ((size_t)M * K + 255) / 256 * 256 + (size_t)M * sizeof(float);
 }
 
+// The tile (of <pair, 256>, <pair, 128>, <single, 128>, <single, 64>) whose
+// waves over the GPU are estimated to cost least, in cycles.  A K = 128 slice
+// takes the longer of its MMAs (an MMA of K = 32 reads 128 + BN rows of 32
+// bytes at 128 bytes a cycle and computes 8192 products a cycle: 128, 64, 64,
+// 48 cycles) and its copies (40 bytes a cycle and SM with all SMs copying,
+// measured at 43,968 x 4096 -> 1024; about 80 for a few).  The epilogue of a
+// wave overlaps the next wave's slices.  Measured: 43,968 x 4096 -> 1024 runs
+// 130 us on <pair, 256> and 207 us on <pair, 128>.
+static int pick_tile(const LinArgs &a) {
+    const int cg[4] = {2, 2, 1, 1}, bn[4] = {256, 128, 128, 64}, mma[4] = {128, 64, 64, 48};
+    const double slices = (a.K + 127) / 128;
+    int best = 0;
+    double least = 1e300;
+    for (int i = 0; i < 4; ++i) {
+        const long long tiles = (long long)((a.M + 128 * cg[i] - 1) / (128 * cg[i])) * ((a.N + bn[i] - 1) / bn[i]);
+        const long long slots = 148 / cg[i], waves = (tiles + slots - 1) / slots;
+        const double active = (double)((tiles < slots ? tiles : slots) * cg[i]);
+        const double rate = active > 74 ? 5920.0 / active : 80.0, bytes = 128.0 * (128 + bn[i] / cg[i]);
+        const double slice = bytes / rate > 4 * mma[i] ? bytes / rate : 4 * mma[i];
+        const double epilogue = bn[i] * (a.gelu ? 30.0 : 12.0), main = slices * slice;
+        const double cost = waves * (main > epilogue ? main : epilogue) + epilogue;
+        if (cost < least) {
+            least = cost;
+            best = i;
+        }
+    }
+    return best;
+}
+
 template <typename T, typename O>
 static int linear(const void *x, long long x_st, const LinArgs &a, void *ws, int32_t *status, cudaStream_t s) {
     if (use_few(a.M, a.K)) return launch_few<T, O>(x, x_st, a, s);
@@ -546,11 +721,12 @@ static int linear(const void *x, long long x_st, const LinArgs &a, void *ws, int
     float *sx = reinterpret_cast<float *>(x8 + ((size_t)a.M * a.K + 255) / 256 * 256);
     const int rc = launch_quant((const T *)x, x_st, a.M, a.K, x8, sx, s);
     if (rc != RESS_OK) return rc;
-    const long long pairs = (long long)((a.M + 255) / 256) * ((a.N + 255) / 256);
-    if (pairs >= 74) return launch_gemm<2, 256, O>(x8, sx, a, status, s);
-    const long long ones = (long long)((a.M + 127) / 128) * ((a.N + 127) / 128);
-    if (ones >= 100) return launch_gemm<1, 128, O>(x8, sx, a, status, s);
-    return launch_gemm<1, 64, O>(x8, sx, a, status, s);
+    switch (pick_tile(a)) {
+        case 0: return launch_gemm<2, 256, O>(x8, sx, a, status, s);
+        case 1: return launch_gemm<2, 128, O>(x8, sx, a, status, s);
+        case 2: return launch_gemm<1, 128, O>(x8, sx, a, status, s);
+        default: return launch_gemm<1, 64, O>(x8, sx, a, status, s);
+    }
 }
 
 }  // namespace i8

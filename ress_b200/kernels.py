@@ -562,8 +562,10 @@ def _dev_status(i: int) -> int:
     return p
 
 
-def _raw_stream(i: int) -> int:
-    return torch.cuda.current_stream(i).cuda_stream
+# the current stream's handle; torch's own accessor for generated code, a
+# microsecond cheaper than building a Stream object
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _on_device(i: int, *ts):
@@ -637,7 +639,7 @@ def cache_append(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, *, q=Non
         Hq, qp = qshape[2], q.data_ptr()
         if qshape[0] != B or qshape[1] != T or q.dtype is not dtype or Hq % Hkv:
             raise RessError("q must have k's tokens and type, and a multiple of its heads")
-        q_out = torch.empty((B, T, Hq, HD), dtype=dtype, device=k.device)
+        q_out = q.new_empty((B, T, Hq, HD))
         q_out_p = q_out.data_ptr()
     if n_new is not None and (n_new.dtype is not _I32 or n_new.shape != (B,) or not n_new.is_contiguous()):
         raise RessError("n_new holds one contiguous int32 per stream")
@@ -697,7 +699,7 @@ def cache_attn(q, k_pages, v_pages, k_scale, v_scale, table, lens, *, limits=Non
             raise RessError("limits must be contiguous (B, T) int32 on the call's device")
         lim = limits.data_ptr()
     if out is None:
-        out = torch.empty(shape, dtype=_BF16 if out_bf16 else _F32, device=q.device)
+        out = q.new_empty(shape) if out_bf16 else q.new_empty(shape, dtype=_F32)
         osh, ost, osb = HD, Hq * HD, T * Hq * HD
     else:
         oshape, osb, ost, osh = _head_rows(out, "out")
@@ -710,7 +712,7 @@ def cache_attn(q, k_pages, v_pages, k_scale, v_scale, table, lens, *, limits=Non
     rows = T * (Hq // Hkv)
     if rows > 16:  # one token needs no workspace
         need = lib.ress_cache_attn_workspace(B, Hkv, rows, table.shape[1])
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
     args = _lib.ATTN_ARGS.pack(q.data_ptr(), out.data_ptr(), T, Hq, sb, st, sh, osb, ost, osh, bool(out_bf16), lim,
                                0.125 if sm_scale is None else sm_scale, 0 if ws is None else ws.data_ptr())
     code = lib.ress_cache_attn(cache, args, _dev_status(i), _raw_stream(i))
@@ -765,12 +767,12 @@ def int8_linear(x, w8, w_scale, bias=None, *, act=None, out_dtype=None):
     if len(shape) != 2 or x.stride(1) != 1:
         x = _rows2d(x)
     M = x.shape[0]
-    out = torch.empty(shape[:-1] + (N,), dtype=out_dtype, device=x.device)
+    out = x.new_empty(shape[:-1] + (N,), dtype=out_dtype)
     if M == 0:
         return out
     lib = _lib.load()
     need = lib.ress_int8_linear_workspace(M, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     code = lib.ress_int8_linear(x.data_ptr(), dt, M, N, K, x.stride(0) if M > 1 else K, w8.data_ptr(),
                                 w_scale.data_ptr(), None if bias is None else bias.data_ptr(), act is not None,
                                 out.data_ptr(), odt, N, None if ws is None else ws.data_ptr(), _dev_status(i),
