@@ -24,7 +24,6 @@ struct LinArgs {
     long long out_st;
     int M, N, K;
     int gelu;
-    int vec;              // w_scale and bias can be read four at a time
 };
 
 // The scale of a row from the bits of its largest magnitude; a row that is
@@ -99,9 +98,8 @@ __device__ __forceinline__ float gelu(float y) {
     const float g = fminf(u, 1e30f) * (p * t * e);  // |y| Phi(-|y|); 0 for an infinite y
     return fmaxf(y, 0.0f) - g;
 }
-__device__ __forceinline__ float finish(int acc, float sx, float sw, float bias, int act) {
-    const float y = __fmaf_rn(__fmul_rn((float)acc, sx), sw, bias);
-    return act ? gelu(y) : y;
+__device__ __forceinline__ float scaled(int acc, float sx, float sw, float bias) {
+    return __fmaf_rn(__fmul_rn((float)acc, sx), sw, bias);
 }
 
 // Rows to int8 with one scale each: one warp per row, eight values a lane at
@@ -287,7 +285,8 @@ __global__ void __launch_bounds__(FEW_NT) few_kernel(const T *__restrict__ x, lo
         int acc = 0;
 #pragma unroll
         for (int w = 0; w < FEW_WARPS; ++w) acc += sums[w][r][col];
-        const float y = finish(acc, sx[r], a.w_scale[n], a.bias != nullptr ? a.bias[n] : 0.0f, a.gelu);
+        float y = scaled(acc, sx[r], a.w_scale[n], a.bias != nullptr ? a.bias[n] : 0.0f);
+        if (a.gelu) y = gelu(y);
         DT<O>::store(reinterpret_cast<O *>(a.out), (size_t)(r * a.out_st + n), y);
     }
 }
@@ -322,7 +321,7 @@ template <int CG, int BN, typename O> struct Tile {
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int OUT_COLS = 128 / (int)sizeof(O);  // one 128-byte swizzled row
     static constexpr int OUT_BYTES = 32 * 128;             // of a warp: 32 rows
-    static constexpr int RING = 196608;
+    static constexpr int RING = 180 * 1024;
     static constexpr int NS = RING / STAGE < 8 ? RING / STAGE : 8;
     static constexpr int OFF_OUT = NS * STAGE;
     static constexpr int SMEM = OFF_OUT + 8 * OUT_BYTES + 1024;
@@ -402,6 +401,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
 
 struct GemmBars {
     uint64_t full[8], empty[8], acc_full[2], acc_free[2];
+    float w_scale[256], bias[256];  // of the tile's channels
     uint32_t tmem;
     int abort_flag;
 };
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CU
                                                       const float *__restrict__ sx, int tma_out, int32_t *status) {
     using C = Tile<CG, BN, O>;
     extern __shared__ unsigned char raw[];
-    __shared__ GemmBars B;
+    __shared__ __align__(16) GemmBars B;
     unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     const uint32_t ring = smem_u32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -513,16 +513,34 @@ __global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CU
         unsigned char *out_s = smem + C::OFF_OUT + (warp - 4) * C::OUT_BYTES;
         const uint32_t out_a = smem_u32(out_s);
         int n = 0;
+        // one channel's scale and bias a thread, asked for a tile ahead (behind the
+        // operands' copies they take microseconds)
+        const int ch = threadIdx.x - 128;
+        float next_w = 0.0f, next_b = 0.0f;
+        bool aborted = false;
+        auto ask = [&](int tile) {
+            const int col = (tile % tiles_n) * BN + ch;
+            const bool in = tile < tiles && ch < BN && col < a.N;
+            next_w = in ? __ldg(a.w_scale + col) : 0.0f;
+            next_b = in && a.bias != nullptr ? __ldg(a.bias + col) : 0.0f;
+        };
+        ask(first);
         for (int tile = first; tile < tiles; tile += step, ++n) {
             const int buf = n & 1;
             const int m0 = (tile / tiles_n) * 128 * CG + rank * 128 + quad * 32, n0 = (tile % tiles_n) * BN;
             const int m = m0 + lane;
             const float s_row = m < a.M ? sx[m] : 0.0f;
-            if (!wait_bar_warp(&B.acc_full[buf], (n >> 1) & 1, abort_flag, status)) break;
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // everyone is done with the tile before
+            B.w_scale[ch] = next_w;
+            B.bias[ch] = next_b;
+            ask(tile + step);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const bool ok = wait_bar_warp(&B.acc_full[buf], (n >> 1) & 1, abort_flag, status);
+            if (!ok) aborted = true;  // the barriers above still want every warp
             fence_after();
             const uint32_t tq = tmem + buf * BN + ((uint32_t)(quad * 32) << 16);
 #pragma unroll 1
-            for (int c = half * C::OUT_COLS; c < BN; c += 2 * C::OUT_COLS) {
+            for (int c = half * C::OUT_COLS; c < BN && !aborted; c += 2 * C::OUT_COLS) {
                 if (n0 + c >= a.N) break;
                 // the piece written before has been read by its store
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -533,28 +551,18 @@ __global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CU
                     tmem_ld32(tq + c + part, v);
                     tmem_wait_ld();
                     const int col = n0 + c + part;
-                    const bool full = a.vec && col + 32 <= a.N;
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
-                        float w[4], bb[4] = {0.f, 0.f, 0.f, 0.f};
-                        if (full) {
-                            const float4 w4 = __ldg(reinterpret_cast<const float4 *>(a.w_scale + col + i));
-                            w[0] = w4.x; w[1] = w4.y; w[2] = w4.z; w[3] = w4.w;
-                            if (a.bias != nullptr) {
-                                const float4 b4 = __ldg(reinterpret_cast<const float4 *>(a.bias + col + i));
-                                bb[0] = b4.x; bb[1] = b4.y; bb[2] = b4.z; bb[3] = b4.w;
-                            }
-                        } else {
+                        const float4 w = *reinterpret_cast<const float4 *>(&B.w_scale[c + part + i]);
+                        const float4 bb = *reinterpret_cast<const float4 *>(&B.bias[c + part + i]);
+                        v[i] = __float_as_uint(scaled((int)v[i], s_row, w.x, bb.x));
+                        v[i + 1] = __float_as_uint(scaled((int)v[i + 1], s_row, w.y, bb.y));
+                        v[i + 2] = __float_as_uint(scaled((int)v[i + 2], s_row, w.z, bb.z));
+                        v[i + 3] = __float_as_uint(scaled((int)v[i + 3], s_row, w.w, bb.w));
+                    }
+                    if (a.gelu) {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const bool in = col + i + j < a.N;
-                                w[j] = in ? a.w_scale[col + i + j] : 0.0f;
-                                if (in && a.bias != nullptr) bb[j] = a.bias[col + i + j];
-                            }
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            v[i + j] = __float_as_uint(finish((int)v[i + j], s_row, w[j], bb[j], a.gelu));
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(gelu(__uint_as_float(v[i])));
                     }
                     if (tma_out) {
                         // 16-byte pieces of the lane's row, 128B-swizzled
@@ -761,8 +769,7 @@ extern "C" int ress_int8_linear(const void *x, int dtype, int M, int N, int K, l
     const int size = dtype == RESS_BF16 ? 2 : 4;
     if ((((uintptr_t)x | (uintptr_t)w8) & 15) || ((x_st * size) & 15)) return RESS_E_ARG;
     if (((uintptr_t)workspace & 15) || M > (1 << 26)) return RESS_E_ARG;
-    const int vec = (((uintptr_t)w_scale | (uintptr_t)bias) & 15) == 0;
-    const i8::LinArgs a{w8, w_scale, bias, out, out_st, M, N, K, gelu, vec};
+    const i8::LinArgs a{w8, w_scale, bias, out, out_st, M, N, K, gelu};
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == RESS_BF16)
         return out_dtype == RESS_BF16 ? i8::linear<__nv_bfloat16, __nv_bfloat16>(x, x_st, a, workspace, status, s)
