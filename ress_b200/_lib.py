@@ -8,6 +8,7 @@ wrapper raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import struct
 
@@ -80,7 +81,9 @@ CACHE = struct.Struct("PPPPqqqqqPqqPq")
 APPEND_ARGS = struct.Struct("PPPPqqqqqqqqqqqqPPPPdPPPqP")
 ATTN_ARGS = struct.Struct("PPqqqqqqqqqPdP")
 
+HOST_PATH = os.path.join(HERE, "_host.so")
 _lib = None
+_host = None
 
 
 class RessError(RuntimeError):
@@ -108,3 +111,20 @@ def check(code: int, what: str):
     if code != RESS_OK:
         msg = load().ress_error_string(code).decode()
         raise RessError(f"{what} failed: {msg} (code {code})")
+
+
+def host(status_of):
+    """The compiled host side of the streaming calls (csrc/host.cpp), bound to
+    the library; status_of(device index) gives the address of that device's
+    status word."""
+    global _host
+    if _host is None:
+        lib = load()
+        if not os.path.exists(HOST_PATH):
+            raise RessError(f"{HOST_PATH} is missing: build it with `python -m ress_b200.build`")
+        spec = importlib.util.spec_from_file_location("ress_b200._host", HOST_PATH)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m.bind(RessError, status_of, {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in SIGNATURES})
+        _host = m
+    return _host

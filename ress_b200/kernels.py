@@ -546,202 +546,56 @@ def qkv_prologue(qkv, H, qn_weight=None, qn_bias=None, kn_weight=None, kn_bias=N
 
 
 # ----------------------------------------------------------------- streaming
-# These calls are made per token: their checks read each tensor's attributes
-# once, and structs and raw pointers keep the host's share of a call small.
+# These calls are made per token and take the GPU a few microseconds, so their
+# checks, allocations and launches are compiled (csrc/host.cpp).
 PAGE = 64  # tokens per cache page
-_E4M3, _E8M0, _BF16, _F32, _I32 = (torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.bfloat16, torch.float32,
-                                   torch.int32)
-_status_ptr = {}
+_host = None
 
 
-def _dev_status(i: int) -> int:
-    """Address of device i's status word (it lives as long as the process)."""
-    p = _status_ptr.get(i)
-    if p is None:
-        p = _status_ptr[i] = status_word(torch.device("cuda", i)).data_ptr()
-    return p
-
-
-# the current stream's handle; torch's own accessor for generated code, a
-# microsecond cheaper than building a Stream object
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda i: torch.cuda.current_stream(i).cuda_stream)
-
-
-def _on_device(i: int, *ts):
-    for t in ts:
-        if t is not None and t.get_device() != i:
-            raise RessError("all tensors of a call are on one CUDA device")
-
-
-def _pack_cache(i, B, k_pages, v_pages, k_scale, v_scale, table, lens):
-    """Checks the cache's tensors (device i, B streams); the struct and the heads."""
-    if k_pages.dtype is not _E4M3 or v_pages.dtype is not _E4M3:
-        raise RessError("cache pages are float8_e4m3fn")
-    if k_scale.dtype is not _E8M0 or v_scale.dtype is not _E8M0:
-        raise RessError("cache scales are float8_e8m0fnu")
-    if table.dtype is not _I32 or lens.dtype is not _I32:
-        raise RessError("the page table and the lengths are int32")
-    _on_device(i, k_pages, v_pages, k_scale, v_scale, table, lens)
-    shape, strides = k_pages.shape, k_pages.stride()
-    if len(shape) != 4 or shape[2:] != (PAGE, HD) or v_pages.shape != shape:
-        raise RessError("cache pages are (pages, heads, 64, 64), alike for k and v")
-    if strides[2:] != (HD, 1) or v_pages.stride() != strides:
-        raise RessError("a page's block of one head is contiguous, and k and v pages share strides")
-    n, H = shape[:2]
-    sstr = k_scale.stride()
-    if k_scale.shape != (n, H) or v_scale.shape != (n, H) or v_scale.stride() != sstr or (sstr[1] != 1 and H > 1):
-        raise RessError("cache scales are (pages, heads) with contiguous heads, alike for k and v")
-    tshape, tstr = table.shape, table.stride()
-    if len(tshape) != 2 or tshape[0] != B or (tstr[1] != 1 and tshape[1] > 1):
-        raise RessError("the page table is (streams, pages) with contiguous rows")
-    if lens.shape != (B,) or not lens.is_contiguous():
-        raise RessError("lens holds one contiguous length per stream")
-    ps, hs, ss = strides[0], strides[1], sstr[0]
-    if n == 1 or H == 1:  # the stride of a single page or head is never used
-        hs = hs if H > 1 else PAGE * HD
-        ps, ss = (ps, ss) if n > 1 else (H * hs, H)
-    return _lib.CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, H, ps,
-                           hs, ss, table.data_ptr(), tstr[0], tshape[1], lens.data_ptr(), B), H
-
-
-def _head_rows(x, what):
-    """Shape and strides of (B, T, heads, 64) rows; 0 for a stride that is never used."""
-    shape, s = x.shape, x.stride()
-    if len(shape) != 4 or shape[3] != HD or s[3] != 1:
-        raise RessError(f"{what} must be (B, T, heads, 64) with a contiguous last dim")
-    return shape, s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0
+def _bind():
+    global _host
+    _host = _lib.host(lambda i: status_word(torch.device("cuda", i)).data_ptr())
+    return _host
 
 
 def cache_append(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, *, q=None, n_new=None, qn_weight=None,
                  qn_bias=None, kn_weight=None, kn_bias=None, eps=1e-5, pos=None, rope_cos=None, rope_sin=None):
-    """New tokens into a paged 8-bit cache (ress_cache_append).  k, v (B, T,
-    Hkv, 64) and q (B, T, Hq, 64) bf16 or fp32, any strides with a contiguous
-    last dim (views of a qkv Linear's output); lens (B,) int32 tokens that the
-    streams hold (not changed), n_new (B,) int32 of the T tokens that count.
-    q and k are normalised over the head dims where weight and bias are given
-    and rotated where rope_cos, rope_sin (positions, 32) and pos (B, T, 2) are;
-    k and v are quantised into their pages.  Returns q's rows (B, T, Hq, 64),
-    or None without q."""
-    _dev_ok(k)
-    i, dtype = k.get_device(), k.dtype
-    dt = _dtype_code(dtype)
-    shape, ksb, kst, ksh = _head_rows(k, "k")
-    vshape, vsb, vst, vsh = _head_rows(v, "v")
-    B, T = shape[0], shape[1]
-    cache, Hkv = _pack_cache(i, B, k_pages, v_pages, k_scale, v_scale, table, lens)
-    if vshape != shape or shape[2] != Hkv or v.dtype is not dtype:
-        raise RessError("k and v must be alike, with the cache's heads")
-    _on_device(i, v, q, n_new, pos, rope_cos, rope_sin)
-    Hq, qsb, qst, qsh, qp, q_out, q_out_p = 0, 0, 0, 0, 0, None, 0
-    if q is not None:
-        qshape, qsb, qst, qsh = _head_rows(q, "q")
-        Hq, qp = qshape[2], q.data_ptr()
-        if qshape[0] != B or qshape[1] != T or q.dtype is not dtype or Hq % Hkv:
-            raise RessError("q must have k's tokens and type, and a multiple of its heads")
-        q_out = q.new_empty((B, T, Hq, HD))
-        q_out_p = q_out.data_ptr()
-    if n_new is not None and (n_new.dtype is not _I32 or n_new.shape != (B,) or not n_new.is_contiguous()):
-        raise RessError("n_new holds one contiguous int32 per stream")
-    norms = []
-    for w, b in ((qn_weight, qn_bias), (kn_weight, kn_bias)):
-        if (w is None) != (b is None):
-            raise RessError("a norm has both weight and bias")
-        for x in (w, b):
-            if x is None:
-                norms.append(0)
-                continue
-            if x.dtype is not _F32 or x.shape != (HD,) or x.get_device() != i or x.stride(0) != 1:
-                raise RessError("norm weights and biases are contiguous fp32 (64,) on the call's device")
-            norms.append(x.data_ptr())
-    pos_p = cos_p = sin_p = rope_len = 0
-    if (rope_cos is None) != (rope_sin is None):
-        raise RessError("the rotary embedding has both tables")
-    if rope_cos is not None:
-        if pos is None or pos.dtype is not torch.int64 or pos.shape != (B, T, 2):
-            raise RessError("pos must be (B, T, 2) int64")
-        tshape = rope_cos.shape
-        if rope_cos.dtype is not dtype or rope_sin.dtype is not dtype or len(tshape) != 2 or tshape[1] != 32 or \
-                rope_sin.shape != tshape:
-            raise RessError("rotary tables must be (max_pos, 32) in k's dtype")
-        rope_cos, rope_sin, pos = rope_cos.contiguous(), rope_sin.contiguous(), pos.contiguous()
-        pos_p, cos_p, sin_p, rope_len = pos.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), tshape[0]
-    if T == 0 or B == 0:
-        return q_out
-    args = _lib.APPEND_ARGS.pack(qp, k.data_ptr(), v.data_ptr(), q_out_p, dt, T, Hq, qsb, qst, qsh, ksb, kst, ksh, vsb,
-                                 vst, vsh, *norms, eps, pos_p, cos_p, sin_p, rope_len,
-                                 0 if n_new is None else n_new.data_ptr())
-    code = _lib.load().ress_cache_append(cache, args, _dev_status(i), _raw_stream(i))
-    if code:
-        check(code, "ress_cache_append")
-    return q_out
+    """New tokens into a paged 8-bit cache (ress_cache_append).
+
+    k_pages, v_pages (pages, heads, 64 tokens, 64) float8_e4m3fn and k_scale,
+    v_scale (pages, heads) float8_e8m0fnu are the pool; token i of stream b
+    lies in slot i % 64 of page table[b, i // 64] (table (B, pages) int32).
+    k, v (B, T, heads, 64) and q (B, T, Hq, 64) are bf16 or fp32, any strides
+    with a contiguous last dim (views of a qkv Linear's output).  They come
+    behind the lens[b] tokens that stream b holds (lens (B,) int32, not
+    changed); n_new (B,) int32 of the T count, all by default.  q and k are
+    normalised over the head dims where weight and bias (fp32) are given, and
+    rotated where rope_cos, rope_sin (positions, 32) and pos (B, T, 2) int64
+    are; k and v are quantised into their pages, at the smallest power of two
+    per page and head that they fit.  Returns q's rows (B, T, Hq, 64), or None
+    without q.  Tokens without a page are dropped and reported by
+    check_status."""
+    return (_host or _bind()).cache_append(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, q, n_new, qn_weight,
+                                           qn_bias, kn_weight, kn_bias, eps, pos, rope_cos, rope_sin)
 
 
 def cache_attn(q, k_pages, v_pages, k_scale, v_scale, table, lens, *, limits=None, sm_scale=None, out=None,
                out_bf16=True):
     """Attention of q (B, T, Hq, 64) bf16 over a paged 8-bit cache
-    (ress_cache_attn): query t of stream b sees the tokens below lens[b], or
-    below min(lens[b], limits[b, t]) with limits (B, T) int32 (a causal or
-    frame-wise mask, a prefix).  A query that sees none gives zeros.  out: a
-    (B, T, Hq, 64) tensor, bf16 or fp32; by default a new one."""
-    _dev_ok(q)
-    i = q.get_device()
-    if q.dtype is not _BF16:
-        raise RessError("cache_attn takes bf16 q")
-    shape, sb, st, sh = _head_rows(q, "q")
-    B, T, Hq, _ = shape
-    cache, Hkv = _pack_cache(i, B, k_pages, v_pages, k_scale, v_scale, table, lens)
-    if Hq % Hkv:
-        raise RessError("q's heads must be a multiple of the cache's")
-    lim = 0
-    if limits is not None:
-        if limits.dtype is not _I32 or limits.shape != (B, T) or not limits.is_contiguous() or limits.get_device() != i:
-            raise RessError("limits must be contiguous (B, T) int32 on the call's device")
-        lim = limits.data_ptr()
-    if out is None:
-        out = q.new_empty(shape) if out_bf16 else q.new_empty(shape, dtype=_F32)
-        osh, ost, osb = HD, Hq * HD, T * Hq * HD
-    else:
-        oshape, osb, ost, osh = _head_rows(out, "out")
-        if oshape != shape or out.dtype not in (_BF16, _F32) or out.get_device() != i:
-            raise RessError("cache_attn output must have q's shape, bf16 or fp32, on the call's device")
-        out_bf16 = out.dtype is _BF16
-    if T == 0 or B == 0:
-        return out
-    lib, ws = _lib.load(), None
-    rows = T * (Hq // Hkv)
-    if rows > 16:  # one token needs no workspace
-        need = lib.ress_cache_attn_workspace(B, Hkv, rows, table.shape[1])
-        ws = q.new_empty(need, dtype=torch.uint8) if need else None
-    args = _lib.ATTN_ARGS.pack(q.data_ptr(), out.data_ptr(), T, Hq, sb, st, sh, osb, ost, osh, bool(out_bf16), lim,
-                               0.125 if sm_scale is None else sm_scale, 0 if ws is None else ws.data_ptr())
-    code = lib.ress_cache_attn(cache, args, _dev_status(i), _raw_stream(i))
-    if code:
-        check(code, "ress_cache_attn")
-    return out
-
-
-def _rows2d(x):
-    """x as (M, K) rows with one stride; a copy only where its strides do not allow that."""
-    if x.dim() == 2 and x.stride(1) == 1:
-        return x
-    x = x.reshape(-1, x.shape[-1])
-    return x if x.stride(1) == 1 else x.contiguous()
+    (ress_cache_attn; the cache as in cache_append): query t of stream b sees
+    the tokens below lens[b], or below min(lens[b], limits[b, t]) with limits
+    (B, T) int32 (a causal or frame-wise mask, a prefix).  A query that sees
+    none gives zeros.  Query heads are consecutive groups per cache head.  out:
+    a (B, T, Hq, 64) tensor, bf16 or fp32; by default a new one, bf16 unless
+    out_bf16 is False."""
+    return (_host or _bind()).cache_attn(q, k_pages, v_pages, k_scale, v_scale, table, lens, limits, sm_scale, out,
+                                         out_bf16)
 
 
 def int8_quant_rows(x):
     """(..., K) bf16 or fp32 -> int8 of the same shape and one fp32 scale per
     row (ress_int8_quant_rows): tokens, or the output channels of a weight."""
-    _dev_ok(x)
-    i = x.get_device()
-    x2 = _rows2d(x)
-    M, K = x2.shape
-    x8 = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=_F32, device=x.device)
-    if M:
-        check(_lib.load().ress_int8_quant_rows(x2.data_ptr(), _dtype_code(x.dtype), M, K, x2.stride(0) if M > 1 else K,
-                                               x8.data_ptr(), scale.data_ptr(), _raw_stream(i)), "ress_int8_quant_rows")
-    return x8, scale
+    return (_host or _bind()).int8_quant_rows(x)
 
 
 def int8_linear(x, w8, w_scale, bias=None, *, act=None, out_dtype=None):
@@ -749,34 +603,7 @@ def int8_linear(x, w8, w_scale, bias=None, *, act=None, out_dtype=None):
     fp32 is quantised per token, w8 (N, K) int8 and w_scale (N,) fp32 are the
     weight's (int8_quant_rows lays them out once).  act: None or "gelu".
     Returns (..., N) in x's type, or out_dtype."""
-    _dev_ok(x)
-    i, dtype, shape, wshape = x.get_device(), x.dtype, x.shape, w8.shape
-    if w8.dtype is not torch.int8 or len(wshape) != 2 or not w8.is_contiguous():
-        raise RessError("w8 must be contiguous int8 (N, K)")
-    N, K = wshape
-    if shape[-1] != K:
-        raise RessError(f"x has {shape[-1]} features, the weight {K}")
-    _on_device(i, w8, w_scale, bias)
-    for t in (w_scale, bias):
-        if t is not None and (t.dtype is not _F32 or t.shape != (N,) or not t.is_contiguous()):
-            raise RessError("w_scale and bias are contiguous fp32 (N,)")
     if act is not None and act != "gelu":
         raise RessError(f"unknown activation {act!r}")
-    out_dtype = dtype if out_dtype is None else out_dtype
-    dt, odt = _dtype_code(dtype), _dtype_code(out_dtype)
-    if len(shape) != 2 or x.stride(1) != 1:
-        x = _rows2d(x)
-    M = x.shape[0]
-    out = x.new_empty(shape[:-1] + (N,), dtype=out_dtype)
-    if M == 0:
-        return out
-    lib = _lib.load()
-    need = lib.ress_int8_linear_workspace(M, K)
-    ws = x.new_empty(need, dtype=torch.uint8) if need else None
-    code = lib.ress_int8_linear(x.data_ptr(), dt, M, N, K, x.stride(0) if M > 1 else K, w8.data_ptr(),
-                                w_scale.data_ptr(), None if bias is None else bias.data_ptr(), act is not None,
-                                out.data_ptr(), odt, N, None if ws is None else ws.data_ptr(), _dev_status(i),
-                                _raw_stream(i))
-    if code:
-        check(code, "ress_int8_linear")
-    return out
+    return (_host or _bind()).int8_linear(x, w8, w_scale, bias, act is not None,
+                                          -1 if out_dtype is None else _dtype_code(out_dtype))
