@@ -13,22 +13,28 @@ using namespace tc;
 // Each warp takes pages of its own: K and V blocks (4 KB each, K0 V0 K1 V1
 // ..) arrive by bulk copies in a ring of three, so the warps never wait for
 // one another before the end; sixteen warps an SM keep 64 KB or more in
-// flight.  The codes become fp16 fragments in registers (one conversion per
-// two values; e4m3 is exact in fp16):
-//   S: B operand = K.  A lane's 16-byte piece of a key row serves the four
-//      k-steps; that orders the head dims differently from memory, and the
-//      q fragments are loaded in the same order.
-//   O: B operand = V, A = P straight from S's accumulators.  Keys are
-//      assigned to accumulator columns as n ^ ((n >> 1) & 1) within eight,
+// flight.  Keys (then head dims) are the MMA's 16 rows and the queries its 8
+// columns, so that no half of a product is empty; the codes become fp16
+// fragments in registers, once for all queries of the tile (one conversion
+// per two values; e4m3 is exact in fp16):
+//   S^T = K Q^T: a lane's 16-byte piece of a key row serves the four k-steps;
+//      that orders the head dims differently from memory, and the q fragments
+//      are loaded in the same order.
+//   O^T = V^T P^T: P's 8x8 tiles are transposed in registers (movmatrix), V's
+//      bytes are paired by key.  Key i of sixteen lies in row i ^ ((i >> 1) & 1),
 //      so that both K's and V's shared-memory reads touch even and odd rows
 //      (64-byte rows: two of equal parity meet in a bank).
+// (mma.sync in e4m3 would need no conversions in the source, but measured
+// slower, 142 against 122 us for 16 streams of 11 to 44 thousand tokens and 8
+// heads: its operands take more instructions than these conversions.)
 // The running maximum, sums and O are fp32.  Row scales of q (a power of two
 // that brings its largest element to [1, 2)) keep q exact in fp16; P is
 // rounded to fp16 after scaling by 2^14 and the page's V scale over the
 // largest one seen, so that small probabilities keep their bits.
 // The pages are split over the CTAs of a cluster (and the warps of a CTA).
 // Each CTA sends its rows' partial results to the shared memory of the row's
-// owner, which joins them in CTA order: one launch, no workspace.
+// owner, which joins them in CTA order: one launch, no workspace.  Up to 32
+// streams are started longest first, so that the last CTAs are short.
 constexpr int FEW_ROWS = 16, FEW_WARPS = 8, FEW_RING = 3, FEW_SPLITS = 16;
 constexpr int FEW_NT = FEW_WARPS * 32;
 constexpr int FEW_SMEM = FEW_WARPS * FEW_RING * BLOCK_BYTES;
@@ -47,6 +53,11 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -94,8 +105,20 @@ __device__ __forceinline__ float load_q16(const AttnArgs &a, int b, int h, int r
     return scale_value(e) * a.scale_log2;
 }
 
-// HALF: eight rows at most, the tile's upper half is not computed.
-template <bool HALF>
+// The stream that CTAs of index z work on: the z-th longest of up to 32.
+__device__ __forceinline__ int stream_by_length(const AttnArgs &a, int z, int streams) {
+    if (streams == 1 || streams > 32) return z;
+    const int lane = threadIdx.x & 31, len = lane < streams ? a.lens[lane] : INT_MIN;
+    int rank = 0;
+    for (int j = 0; j < streams; ++j) {
+        const int other = __shfl_sync(0xffffffffu, len, j);
+        rank += other > len || (other == len && j < lane);
+    }
+    return __ffs(__ballot_sync(0xffffffffu, lane < streams && rank == z)) - 1;
+}
+
+// NT: groups of eight rows in the tile.
+template <int NT>
 __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv_heads) {
     extern __shared__ __align__(128) unsigned char dyn[];
     __shared__ uint64_t full[FEW_WARPS][FEW_RING];
@@ -104,7 +127,7 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
     // what the cluster's CTAs send to this one: for its n-th row, one slot per CTA
     __shared__ __align__(16) float inbox[FEW_ROWS * SLOT + FEW_SPLITS * SLOT];
     const int split = blockIdx.x, splits = gridDim.x;
-    const int h = blockIdx.y % kv_heads, tile = blockIdx.y / kv_heads, b = blockIdx.z;
+    const int h = blockIdx.y % kv_heads, tile = blockIdx.y / kv_heads, b = stream_by_length(a, blockIdx.z, gridDim.z);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int r0 = tile * FEW_ROWS, rows = min(FEW_ROWS, a.rows - r0);
@@ -112,60 +135,57 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
     if (threadIdx.x < FEW_WARPS * FEW_RING) mbar_init(&full[0][0] + threadIdx.x, 1);
     if (threadIdx.x == 0) abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncthreads();
-    if (splits > 1) cluster_arrive();  // waited for before the first store into a peer
-
-    // what the rows see
+    // what the rows see; a lane works on rows 2t and 2t + 1 of each group
     const int len = stream_len(a, b);
-    if (threadIdx.x == 0 && split == 0 && bad_len(a, b)) atomicOr(a.status, RESS_STATUS_CACHE_RANGE);
-    int lim[2], lo = INT_MAX, hi = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        lim[i] = row_limit(a, b, len, r0 + g + 8 * i);
-        if (lim[i] >= 0) {
-            lo = min(lo, lim[i]);
-            hi = max(hi, lim[i]);
-        }
-    }
+    int lim[NT][2], lo = len, hi = len;
     if (a.limits != nullptr) {
+        lo = INT_MAX;
+        hi = 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                lim[n][e] = row_limit(a, b, len, r0 + 8 * n + 2 * t + e);
+                if (lim[n][e] >= 0) {
+                    lo = min(lo, lim[n][e]);
+                    hi = max(hi, lim[n][e]);
+                }
+            }
         lo = __reduce_min_sync(0xffffffffu, lo);
         hi = __reduce_max_sync(0xffffffffu, hi);
-    } else {
-        lo = hi = len;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (lim[i] < 0) lim[i] = hi;  // rows past the last: computed, never written
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (a.limits == nullptr || lim[n][e] < 0) lim[n][e] = hi;  // rows past the last: computed, never written
+    __syncthreads();
+    if (splits > 1) cluster_arrive();  // waited for before the first store into a peer
+    if (threadIdx.x == 0 && split == 0 && bad_len(a, b)) atomicOr(a.status, RESS_STATUS_CACHE_RANGE);
 
     // this warp's pages: first, first + FEW_WARPS, ... (count of them)
-    const int n = (hi + PAGE - 1) / PAGE;
-    const int p0 = (int)((long long)n * split / splits), p1 = (int)((long long)n * (split + 1) / splits);
+    const int pages = (hi + PAGE - 1) / PAGE;
+    const int p0 = (int)((long long)pages * split / splits), p1 = (int)((long long)pages * (split + 1) / splits);
     const int first = p0 + warp, count = p1 > first ? (p1 - first + FEW_WARPS - 1) / FEW_WARPS : 0;
     // page ids and scales, 32 pages at a time: lane i holds page base + i
     const int32_t *table = a.table + b * a.table_stride;
-    auto fetch = [&](int base, int &id, int &su) {
-        id = 0;
-        su = 0;
+    auto fetch_id = [&](int base) {
         const int i = base + lane;
-        if (i < count) {
-            id = table[first + i * FEW_WARPS];
-            if (id < 0 || id >= a.n_pages) {  // no such page: its tokens count as NaN
-                atomicOr(a.status, RESS_STATUS_CACHE_RANGE);
-                id = 0;
-                su = 0xFFFF;
-            } else {
-                su = a.K.scale[id * a.K.scale_stride + h] | (a.V.scale[id * a.V.scale_stride + h] << 8);
-            }
+        int id = i < count ? table[first + i * FEW_WARPS] : 0;
+        if (id < 0 || id >= a.n_pages) {  // no such page: its tokens count as NaN
+            atomicOr(a.status, RESS_STATUS_CACHE_RANGE);
+            id = -1;
         }
+        return id;
     };
-    int id_a, su_a, id_b = 0, su_b = 0;  // batches of even and odd number
-    fetch(0, id_a, su_a);
+    auto fetch_scale = [&](const Pages &P, int id) { return id < 0 ? 255 : (int)P.scale[id * P.scale_stride + h]; };
+    int id_a = fetch_id(0), id_b = 0;  // batches of even and odd number
     unsigned char *ring = dyn + warp * FEW_RING * BLOCK_BYTES;
     const uint32_t ring_a = smem_u32(ring);
     const int blocks = 2 * count;
     int fill_slot = 0;  // ring slot of the next block to ask for
     auto issue = [&](int n) {  // block n: K (even) or V of page n / 2; all lanes call it
-        const int i = n >> 1, id = __shfl_sync(0xffffffffu, (i & 32) ? id_b : id_a, i & 31);
+        const int i = n >> 1, id = max(__shfl_sync(0xffffffffu, (i & 32) ? id_b : id_a, i & 31), 0);
         if (lane == 0) {
             const Pages &P = n & 1 ? a.V : a.K;
             mbar_expect_tx(&full[warp][fill_slot], BLOCK_BYTES);
@@ -176,18 +196,31 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
     };
     int issued = 0;
     while (issued < min(blocks, FEW_RING)) issue(issued++);
-    fetch(32, id_b, su_b);
+    // the scales, behind the first copies
+    int uk_a = fetch_scale(a.K, id_a), uv_a = fetch_scale(a.V, id_a), uk_b = 0, uv_b = 0;
+    if (count > 32) {
+        id_b = fetch_id(32);
+        uk_b = fetch_scale(a.K, id_b);
+        uv_b = fetch_scale(a.V, id_b);
+    }
 
-    uint32_t q0[8], q1[8] = {};
-    const float rf0 = load_q16(a, b, h, r0 + g, t, q0);
-    float rf1 = 0.0f;
-    if (!HALF) rf1 = load_q16(a, b, h, r0 + g + 8, t, q1);
+    uint32_t q[NT][8];
+    float rf[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const float f = load_q16(a, b, h, r0 + 8 * n + g, t, q[n]);
+        rf[n][0] = __shfl_sync(0xffffffffu, f, 8 * t);  // of row 2t: its lanes are 4 * 2t ..
+        rf[n][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+    }
 
-    float o[8][4] = {};
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    float o[NT][4][4] = {};
+    float m[NT][2], l[NT][2] = {};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
     int uref = 0;  // O counts in units of 2^(uref - 127 - P_SHIFT)
-    const int kf = 2 * t + (t & 1), kh = 2 * t + 1 - (t & 1);  // keys of a lane's even and odd columns
-    const uint32_t koff = (uint32_t)(g ^ ((g >> 1) & 1)) * HD + t * 16;
+    const int pg = g ^ ((g >> 1) & 1);  // this lane's key of eight in S^T
+    const int kf = 2 * t + (t & 1), kh = 2 * t + 1 - (t & 1);  // and its pair of keys in V^T
+    const uint32_t koff = (uint32_t)pg * HD + t * 16;
     int slot = 0, phase = 0;  // of the block consumed next
     auto take = [&]() -> const unsigned char * {
         if (!wait_bar_warp(&full[warp][slot], phase, abort_flag, a.status)) return nullptr;
@@ -203,139 +236,136 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
     };
     for (int i = 0; i < count; ++i) {
         // the batch two ahead replaces the one just used up
-        if ((i & 31) == 0 && i > 0) {
-            if (i & 32) fetch(i + 32, id_a, su_a);
-            else fetch(i + 32, id_b, su_b);
+        if ((i & 31) == 0 && i > 0 && i + 32 < count) {
+            if (i & 32) {
+                id_a = fetch_id(i + 32);
+                uk_a = fetch_scale(a.K, id_a);
+                uv_a = fetch_scale(a.V, id_a);
+            } else {
+                id_b = fetch_id(i + 32);
+                uk_b = fetch_scale(a.K, id_b);
+                uv_b = fetch_scale(a.V, id_b);
+            }
         }
-        const int su = __shfl_sync(0xffffffffu, (i & 32) ? su_b : su_a, i & 31);
-        const int uk = su & 255, uv = su >> 8;
+        const int uk = __shfl_sync(0xffffffffu, (i & 32) ? uk_b : uk_a, i & 31);
+        const int uv = __shfl_sync(0xffffffffu, (i & 32) ? uv_b : uv_a, i & 31);
         const unsigned char *sk = take();
         if (sk == nullptr) break;
-        uint4 kx[8];
+        float c[4][NT][4] = {};  // sixteen keys each: keys pg (0, 1) and pg + 8 (2, 3) of rows 2t, 2t + 1
+        {
+            uint4 ka[4], kb[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) kx[j] = *reinterpret_cast<const uint4 *>(sk + j * 8 * HD + koff);
-        float c[8][4] = {};
-#pragma unroll
-        for (int st = 0; st < 4; ++st)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t w = st == 0 ? kx[j].x : st == 1 ? kx[j].y : st == 2 ? kx[j].z : kx[j].w;
-                mma_16816(c[j], q0[2 * st], HALF ? 0u : q1[2 * st], q0[2 * st + 1], HALF ? 0u : q1[2 * st + 1],
-                          e4m3_to_half2((uint16_t)w), e4m3_to_half2((uint16_t)(w >> 16)));
+            for (int mt = 0; mt < 4; ++mt) {
+                ka[mt] = *reinterpret_cast<const uint4 *>(sk + mt * 16 * HD + koff);
+                kb[mt] = *reinterpret_cast<const uint4 *>(sk + (mt * 16 + 8) * HD + koff);
             }
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt) {
+                    const uint32_t x = st == 0 ? ka[mt].x : st == 1 ? ka[mt].y : st == 2 ? ka[mt].z : ka[mt].w;
+                    const uint32_t y = st == 0 ? kb[mt].x : st == 1 ? kb[mt].y : st == 2 ? kb[mt].z : kb[mt].w;
+                    const uint32_t a0 = e4m3_to_half2((uint16_t)x), a1 = e4m3_to_half2((uint16_t)y);
+                    const uint32_t a2 = e4m3_to_half2((uint16_t)(x >> 16)), a3 = e4m3_to_half2((uint16_t)(y >> 16));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_16816(c[mt][n], a0, a1, a2, a3, q[n][2 * st], q[n][2 * st + 1]);
+                }
+        }
         done();
-        const float fk = scale_value(uk);
-        const float c0 = rf0 * fk, c1 = rf1 * fk;
         const int base = (first + i * FEW_WARPS) * PAGE;
         const bool whole = base + PAGE <= lo;
-        float x0 = -INFINITY, x1 = -INFINITY;
-        if (!whole) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {  // hidden tokens: -inf, whatever lies there
-                const int ke = base + 8 * j + kf, ko = base + 8 * j + kh;
-                if (ke >= lim[0]) c[j][0] = -INFINITY;
-                if (ko >= lim[0]) c[j][1] = -INFINITY;
-                if (!HALF && ke >= lim[1]) c[j][2] = -INFINITY;
-                if (!HALF && ko >= lim[1]) c[j][3] = -INFINITY;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x0 = fmaxf(x0, fmaxf(c[j][0], c[j][1]));
-            if (!HALF) x1 = fmaxf(x1, fmaxf(c[j][2], c[j][3]));
-        }
-        // the page's largest score; the factors are not negative (a NaN one shows in the exponentials)
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-        const float n0 = fmaxf(m0, x0 == -INFINITY ? x0 : x0 * c0), b0 = n0 == -INFINITY ? 0.0f : n0;
-        float al0 = ex2(m0 - b0), al1 = 1.0f, b1 = 0.0f;
-        m0 = n0;
-        if (!HALF) {
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-            const float n1 = fmaxf(m1, x1 == -INFINITY ? x1 : x1 * c1);
-            b1 = n1 == -INFINITY ? 0.0f : n1;
-            al1 = ex2(m1 - b1);
-            m1 = n1;
-        }
-        l0 *= al0;
-        l1 *= al1;
+        const float fk = scale_value(uk);
         // a page of larger V scale moves O's unit
-        float fv = scale_value(uv);  // NaN stays NaN
+        float fv = scale_value(uv), move = 1.0f;  // NaN stays NaN
         if (uv != 255) {
             if (uv > uref) {
-                const float d = scale_value(max(127 + uref - uv, 0));
-                al0 *= d;
-                al1 *= d;
+                move = scale_value(max(127 + uref - uv, 0));
                 uref = uv;
             }
             fv = scale_value(max(127 + P_SHIFT + uv - uref, 0));
         }
-        if (__any_sync(0xffffffffu, al0 != 1.0f || al1 != 1.0f)) {
+        uint32_t pb[NT][4][2];
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                o[d][0] *= al0;
-                o[d][1] *= al0;
-                o[d][2] *= al1;
-                o[d][3] *= al1;
-            }
-        }
-        // P: probabilities for the sums, and times the V scale as fp16 fragments
-        uint32_t pa[4][4];
+        for (int n = 0; n < NT; ++n) {
+            float bias[2], cs[2], alpha[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float p[4] = {};
-            p[0] = ex2(fmaf(c[j][0], c0, -b0));
-            p[1] = ex2(fmaf(c[j][1], c0, -b0));
-            if (!HALF) {
-                p[2] = ex2(fmaf(c[j][2], c1, -b1));
-                p[3] = ex2(fmaf(c[j][3], c1, -b1));
-            }
-            if (!whole) {  // a hidden token is 0 even where a factor is 0 or NaN
-                const int ke = base + 8 * j + kf, ko = base + 8 * j + kh;
-                if (ke >= lim[0]) p[0] = 0.0f;
-                if (ko >= lim[0]) p[1] = 0.0f;
-                if (ke >= lim[1]) p[2] = 0.0f;
-                if (ko >= lim[1]) p[3] = 0.0f;
-            }
-            l0 += p[0] + p[1];
-            l1 += p[2] + p[3];
+            for (int e = 0; e < 2; ++e) {
+                float top = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] *= fv;
-            if (!whole && uv == 255) {
-                const int ke = base + 8 * j + kf, ko = base + 8 * j + kh;
-                if (ke >= lim[0]) p[0] = 0.0f;
-                if (ko >= lim[0]) p[1] = 0.0f;
-                if (ke >= lim[1]) p[2] = 0.0f;
-                if (ko >= lim[1]) p[3] = 0.0f;
+                for (int mt = 0; mt < 4; ++mt) {
+                    if (!whole) {  // hidden tokens: -inf, whatever lies there
+                        if (base + mt * 16 + pg >= lim[n][e]) c[mt][n][e] = -INFINITY;
+                        if (base + mt * 16 + 8 + pg >= lim[n][e]) c[mt][n][e + 2] = -INFINITY;
+                    }
+                    top = fmaxf(top, fmaxf(c[mt][n][e], c[mt][n][e + 2]));
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                cs[e] = rf[n][e] * fk;  // not negative; a NaN one shows in the exponentials
+                const float mn = fmaxf(m[n][e], top == -INFINITY ? top : top * cs[e]);
+                const float mb = mn == -INFINITY ? 0.0f : mn;
+                alpha[e] = ex2(m[n][e] - mb);
+                l[n][e] *= alpha[e];
+                alpha[e] *= move;
+                m[n][e] = mn;
+                bias[e] = -mb;
             }
-            pa[j >> 1][2 * (j & 1)] = half2_bits(p[0], p[1]);
-            pa[j >> 1][2 * (j & 1) + 1] = HALF ? 0u : half2_bits(p[2], p[3]);
+            if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    o[n][d][0] *= alpha[0];
+                    o[n][d][1] *= alpha[1];
+                    o[n][d][2] *= alpha[0];
+                    o[n][d][3] *= alpha[1];
+                }
+            }
+            // P: probabilities for the sums, and times the V scale as fp16 fragments
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float p[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        p[e] = ex2(fmaf(c[mt][n][2 * k + e], cs[e], bias[e]));
+                        // a hidden token is 0 even where a factor is 0 or NaN
+                        const bool hidden = !whole && base + mt * 16 + 8 * k + pg >= lim[n][e];
+                        if (hidden) p[e] = 0.0f;
+                        l[n][e] += p[e];
+                        p[e] *= fv;
+                        if (hidden) p[e] = 0.0f;
+                    }
+                    pb[n][mt][k] = transpose8x8(half2_bits(p[0], p[1]));
+                }
         }
         const unsigned char *sv = take();
         if (sv == nullptr) break;
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            const unsigned char *va = sv + st * 16 * HD + g * 8;
+        for (int mt = 0; mt < 4; ++mt) {
+            const unsigned char *va = sv + mt * 16 * HD + g * 8;
             uint2 v0 = *reinterpret_cast<const uint2 *>(va + kf * HD), v1 = *reinterpret_cast<const uint2 *>(va + kh * HD);
             uint2 v2 = *reinterpret_cast<const uint2 *>(va + (8 + kf) * HD);
             uint2 v3 = *reinterpret_cast<const uint2 *>(va + (8 + kh) * HD);
             if (base + PAGE > len) {  // slots past the stream's end hold anything, NaN codes too
-                const int e = len - base - 16 * st;
+                const int e = len - base - 16 * mt;
                 if (kf >= e) v0 = make_uint2(0, 0);
                 if (kh >= e) v1 = make_uint2(0, 0);
                 if (8 + kf >= e) v2 = make_uint2(0, 0);
                 if (8 + kh >= e) v3 = make_uint2(0, 0);
             }
 #pragma unroll
-            for (int d = 0; d < 8; d += 2) {
-                const uint32_t sel = (d & 2) ? 0x7362u : 0x5140u;
-                const uint32_t y0 = d < 4 ? __byte_perm(v0.x, v1.x, sel) : __byte_perm(v0.y, v1.y, sel);
-                const uint32_t y1 = d < 4 ? __byte_perm(v2.x, v3.x, sel) : __byte_perm(v2.y, v3.y, sel);
-                mma_16816(o[d], pa[st][0], pa[st][1], pa[st][2], pa[st][3], e4m3_to_half2((uint16_t)y0),
-                          e4m3_to_half2((uint16_t)y1));
-                mma_16816(o[d + 1], pa[st][0], pa[st][1], pa[st][2], pa[st][3], e4m3_to_half2((uint16_t)(y0 >> 16)),
-                          e4m3_to_half2((uint16_t)(y1 >> 16)));
+            for (int d = 0; d < 4; d += 2) {  // dims 8g + d, and + 4 in the lower half of the rows
+                const uint32_t sel = d == 0 ? 0x5140u : 0x7362u;
+                const uint32_t y0 = __byte_perm(v0.x, v1.x, sel), y1 = __byte_perm(v0.y, v1.y, sel);
+                const uint32_t y2 = __byte_perm(v2.x, v3.x, sel), y3 = __byte_perm(v2.y, v3.y, sel);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t a0 = e4m3_to_half2((uint16_t)(y0 >> (16 * k))), a1 = e4m3_to_half2((uint16_t)(y1 >> (16 * k)));
+                    const uint32_t a2 = e4m3_to_half2((uint16_t)(y2 >> (16 * k))), a3 = e4m3_to_half2((uint16_t)(y3 >> (16 * k)));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_16816(o[n][d + k], a0, a1, a2, a3, pb[n][mt][0], pb[n][mt][1]);
+                }
             }
         }
         done();
@@ -347,29 +377,30 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
         while (!mbar_try_wait(smem_u32(&full[warp][s]), (last / FEW_RING) & 1) && globaltimer() - t0 < TIMEOUT_NS) {
         }
     }
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    if (t == 0) {
-        part_m[warp][g] = m0;
-        part_l[warp][g] = l0;
-        part_m[warp][g + 8] = m1;
-        part_l[warp][g + 8] = l1;
-    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+            if (g == 0) {
+                part_m[warp][8 * n + 2 * t + e] = m[n][e];
+                part_l[warp][8 * n + 2 * t + e] = l[n][e];
+            }
+        }
     __syncthreads();
     // the warps' O meet in the ring, 4 KB a warp
     float *po = reinterpret_cast<float *>(dyn) + warp * FEW_ROWS * HD;
     const float unit = scale_value(uref), down = scale_value(127 - P_SHIFT);
 #pragma unroll
-    for (int half = 0; half < (HALF ? 1 : 2); ++half)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int d = 0; d < 8; d += 4)
-                *reinterpret_cast<float4 *>(po + (g + 8 * half) * HD + 16 * t + 8 * e + d) =
-                    make_float4(o[d][2 * half + e] * down * unit, o[d + 1][2 * half + e] * down * unit,
-                                o[d + 2][2 * half + e] * down * unit, o[d + 3][2 * half + e] * down * unit);
+            for (int k = 0; k < 2; ++k)
+                *reinterpret_cast<float4 *>(po + (8 * n + 2 * t + e) * HD + 8 * g + 4 * k) =
+                    make_float4(o[n][0][e + 2 * k] * down * unit, o[n][1][e + 2 * k] * down * unit,
+                                o[n][2][e + 2 * k] * down * unit, o[n][3][e + 2 * k] * down * unit);
     __syncthreads();
     if (splits > 1) cluster_wait();  // the peers have started
     const float *co = reinterpret_cast<const float *>(dyn);
@@ -452,10 +483,19 @@ static bool allow_wide_clusters(const void *kern, int which) {
 static int launch_few(const AttnArgs &a, int B, int Hkv, cudaStream_t stream) {
     const int tiles = (a.rows + FEW_ROWS - 1) / FEW_ROWS;
     const long long groups = (long long)tiles * Hkv * B;
-    // CTAs for about two per SM, as long as there is a page for each warp
+    // CTAs per (rows, head, stream).  While the CTAs fit on an SM each, pages enough
+    // for half a CTA's warps suffice (1 x 16 heads x 1,374 tokens: 9.6 us in one
+    // CTA, 6.5 in four, 6.7 in eight); beyond that two pages a warp, and CTAs
+    // for four per SM, so that the longer streams' can start first (16 x 8 heads
+    // x 11 to 44 thousand: 122 us in two, 113 in four, 118 in eight).  Sixteen
+    // CTAs make a cluster that is hard to place: only where eight leave half of
+    // the GPU idle.
     int splits = 1;
-    while (splits < FEW_SPLITS && groups * splits * 2 <= 148 * 2 && splits * 2 * FEW_WARPS <= a.table_width) splits *= 2;
-    auto kern = a.rows <= 8 ? few_kernel<true> : few_kernel<false>;
+    const long long width = a.table_width;
+    while (splits < 8 && groups * splits * 2 <= 148 && splits * 2 * FEW_WARPS / 2 <= width) splits *= 2;
+    while (splits < 8 && groups * splits * 2 <= 148 * 4 && splits * 2 * FEW_WARPS * 2 <= width) splits *= 2;
+    if (splits == 8 && groups * 16 <= 148 && 16 * FEW_WARPS <= width) splits = 16;
+    auto kern = a.rows <= 8 ? few_kernel<1> : few_kernel<2>;
     set_smem_attr((const void *)kern, FEW_SMEM);
     if (splits > 8 && !allow_wide_clusters((const void *)kern, a.rows <= 8)) return RESS_E_LAUNCH;
     cudaLaunchConfig_t cfg = {};
