@@ -2,26 +2,34 @@
 // the tensor cores (cache_attn.cuh has the definition).
 //
 // One CTA per 256 rows of a (stream, key/value head), as two tiles of 128
-// that share every page of keys and values; 24 warps:
+// that share every page of keys and values; 16 warps:
 //   warp 0       loads pages: K blocks (TMA, 64B-swizzled), V blocks (bulk);
 //   warp 1       issues S = Q K^T, tcgen05.mma kind::f8f6f4.  K's codes are an
 //                operand as they lie in the cache.  q is split into two e4m3
 //                parts, q = hi + lo (4 + 4 significant bits, as many as bf16
 //                has), so S takes four K = 32 steps: hi and lo against the same
 //                K, which is what bf16 would take.  Scales are applied to S.
-//   warp 2       issues O += P V, kind::f16 in bf16.  N = 80: sixteen columns
-//                of ones give the row sums of P.
+//   warp 2       issues O += P V, kind::f16 in bf16, P from tensor memory (an
+//                MMA of 128 x 80 x 16 takes 40 cycles so, 52 with P in shared
+//                memory).  N = 80: sixteen columns of ones give the row sums.
 //   warp 3       allocates tensor memory.
 //   warps 4-7    turn V's codes into bf16 (exact: the scale is a power of two)
 //                in the 128B-swizzled layout that the MMA reads, once for both
 //                tiles.
-//   warps 8-23   softmax, eight warps a tile, two threads per row: thread =
-//                (row, 32 of the page's 64 keys).  The running maximum moves
-//                only when it grows by more than 2^8, so O in tensor memory is
-//                rarely rescaled.
-// Pages that all rows of a tile see take the hot path; the first page and
-// those that a limit cuts run out of line.  P is rounded to bf16 for the MMA,
-// numerator and denominator alike; everything else is fp32.
+//   warps 8-15   softmax, four warps a tile, one thread per row: a page's 64
+//                scores in registers (two loads of the 32x32b shape, which
+//                reads tensor memory twice as fast as the 16-lane shapes), no
+//                exchange between threads, P back to tensor memory.  The
+//                running maximum moves only when it grows by more than 2^8, so
+//                O in tensor memory is rarely rescaled.
+// Scores are double-buffered.  The bound is the exponential unit: 64 of 16 a
+// cycle and SM, 1024 cycles for both tiles of a page, against 708 cycles of
+// MMAs; with two softmax warps a sub-partition one computes exponentials
+// while the other waits for its scores, reads them and finds their maximum.
+// (Sixteen softmax warps with two threads a row and P in shared memory:
+// 1850 cycles a page.)
+// P is rounded to bf16 for the MMA, numerator and denominator alike;
+// everything else is fp32.
 // When the tiles are too few for the GPU the pages are split over several
 // CTAs; the one that finishes last joins the pieces in page order, so the
 // result does not depend on the order of arrival.
@@ -34,21 +42,22 @@ namespace many {
 
 using namespace tc;
 
-constexpr int NT = 768, TILE = 128, TILES = 2, NSOFT = 256;  // softmax threads of a tile
-constexpr int NK = 6, NC = 6, NV = 3, NP = 3;                // rings: K, V codes, V in bf16, P
-constexpr int INFO = 32;  // scales of pages in flight: more than any ring is deep
-constexpr int REGS_CTRL = 32, REGS_SOFT = 104;
-static_assert(256 * REGS_CTRL + 512 * REGS_SOFT <= NT * 80, "register split above the launch's registers");
-constexpr int Q_BYTES = TILE * 128, V_BYTES = PAGE * 128, P_BYTES = TILE * 128, ONES_BYTES = 16 * 128;
+constexpr int NT = 512, TILE = 128, TILES = 2;
+constexpr int NK = 8, NC = 8, NV = 4;  // rings: K, V codes, V in bf16
+constexpr int INFO = 32;               // scales of pages in flight: more than any ring is deep
+constexpr int REGS_CTRL = 64, REGS_SOFT = 192;
+static_assert(256 * REGS_CTRL + 256 * REGS_SOFT <= NT * 128, "register split above the launch's registers");
+constexpr int Q_BYTES = TILE * 128, V_BYTES = PAGE * 128, ONES_BYTES = 16 * 128;
 constexpr int OFF_Q = 0;
 constexpr int OFF_K = OFF_Q + TILES * Q_BYTES;
 constexpr int OFF_C = OFF_K + NK * BLOCK_BYTES;
 constexpr int OFF_V = OFF_C + NC * BLOCK_BYTES;
-constexpr int OFF_P = OFF_V + NV * V_BYTES;
-constexpr int OFF_ONES = OFF_P + TILES * NP * P_BYTES;
+constexpr int OFF_ONES = OFF_V + NV * V_BYTES;
 constexpr int SMEM = OFF_ONES + ONES_BYTES + 1024;
 static_assert(V_BYTES == 4 * 2048, "four K = 16 slices a page");
 static_assert(SMEM + 4096 <= 227 * 1024, "shared memory");
+// Tensor memory columns: S (two buffers of 64 a tile), O (64 and the 16 row-sum columns), P (bf16 pairs)
+constexpr uint32_t COL_S = 0, COL_O = 256, COL_P = 448, O_STRIDE = 96;
 constexpr float RESCALE_THRESH = 8.0f;
 constexpr int SPLIT_MAX = 8, PART_ROW = HD + 4;  // a partial row: O, maximum, sum
 
@@ -59,7 +68,7 @@ constexpr uint32_t IDESC_O =
 
 struct Bars {
     uint64_t k_full[NK], k_empty[NK], c_full[NC], c_empty[NC], v_full[NV], v_empty[NV];
-    uint64_t s_full[TILES][2], s_free[TILES][2], p_full[TILES][NP], o_full[TILES][NP];
+    uint64_t s_full[TILES][2], s_free[TILES][2], p_full[TILES], o_full[TILES];
     uint64_t s_done, pv_done;
     uint32_t tmem;
     int abort_flag, hi, lo[TILES], join[TILES];
@@ -93,6 +102,11 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
     return p != 0;
 }
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return r;
+}
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -116,82 +130,132 @@ __device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t f, uint32_t &
 // 2^e as a bf16 pair
 __device__ __forceinline__ uint32_t pow2_bf16x2(int e) { return (uint32_t)((e + 127) << 7) * 0x00010001u; }
 
-// What an out-of-line softmax step needs of its thread.
+// Tensor memory to registers and back: lane = row, n columns.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+    uint32_t v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr));
+    return v;
+}
+// O += P V with P (A) in tensor memory.
+__device__ __forceinline__ void mma_pv(uint32_t d, uint32_t p, uint64_t b, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(p), "l"(b), "r"(IDESC_O), "r"(acc));
+}
+
+// This thread's row of O, row sum included, times alpha.  Out of line, as
+// everything rare is: the loop over pages has to fit the instruction cache
+// (unrolled by two with the masked path inline it ran at 2330 cycles a page).
+__device__ __noinline__ void rescale_o(uint32_t tO, float alpha) {
+#pragma unroll 1
+    for (int c = 0; c < HD + 16; c += 8) {
+        uint32_t o[8];
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7])
+                     : "r"(tO + c));
+        tmem_wait_ld();
+#pragma unroll
+        for (int t = 0; t < 8; ++t) o[t] = __float_as_uint(__uint_as_float(o[t]) * alpha);
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(tO + c), "r"(o[0]),
+                     "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
+                     : "memory");
+    }
+    tmem_wait_st();
+}
+
+// A wait whose usual case, the phase complete, is one probe.
+__device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int32_t *status) {
+    return wait_bar_warp(bar, parity, abort_flag, status);
+}
+__device__ __forceinline__ bool wait_quick(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int32_t *status) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(smem_u32(bar), parity))) return true;
+    return wait_slow(bar, parity, abort_flag, status);
+}
+
+// What the out-of-line step needs of its thread.
 struct Row {
-    uint32_t tS, tO, lane_addr, sP, prow, rsw, ch0;
-    int col0;
-    uint64_t *o_full, *s_free;
+    uint32_t tS, tO, tP;
+    uint64_t *s_free, *o_full;
     volatile int *abort_flag;
     int32_t *status;
 };
 
-// This thread's half of its row of O (and of the row-sum columns) times alpha.
-__device__ __noinline__ void rescale_o(uint32_t tO, uint32_t lane_addr, float alpha) {
-    uint32_t o[32], s8[8];
-    tmem_ld_half32(tO + lane_addr, o);
-    tmem_ld_half8(tO + HD + lane_addr, s8);
-    tmem_wait_ld();
-#pragma unroll
-    for (int t = 0; t < 32; ++t) o[t] = __float_as_uint(__uint_as_float(o[t]) * alpha);
-#pragma unroll
-    for (int t = 0; t < 8; ++t) s8[t] = __float_as_uint(__uint_as_float(s8[t]) * alpha);
-    tmem_st_half32(tO + lane_addr, o);
-    tmem_st_half8(tO + HD + lane_addr, s8);
-    tmem_wait_st();
-}
-
-// The general step for page j: the row sees the page's first `seen` keys, its
-// maximum may not be set yet.  Returns the new maximum, NaN when a wait failed.
-__device__ __noinline__ float step_general(const Row &rc, int j, int seen, float c, float m) {
-    const int sb = j & 1, pb = j % NP;
-    uint32_t sv[32];
-    tmem_ld_half32(rc.tS + sb * 64 + rc.lane_addr, sv);
-    tmem_wait_ld();
-    fence_before();
-    mbar_arrive(rc.s_free + sb);
+// Page j, of which the row sees the first `seen` keys; c is the factor of its
+// scores.  Takes the running maximum and returns the new one, NaN when a wait
+// failed.  The scores are there; P and its barrier are the caller's.
+__device__ __noinline__ float step_masked(const Row &rc, int j, int seen, float c, float m) {
+    uint32_t p[32];
     float mx = -INFINITY;
+#pragma unroll 1
+    for (int h = 0; h < 64; h += 32) {
+        uint32_t sv[32];
+        tmem_ld32(rc.tS + (j & 1) * 64 + h, sv);
+        tmem_wait_ld();
 #pragma unroll
-    for (int t = 0; t < 32; ++t) {
-        const float x = rc.col0 + t < seen ? __uint_as_float(sv[t]) * c : -INFINITY;
-        sv[t] = __float_as_uint(x);
-        mx = fmaxf(mx, x);
+        for (int t = 0; t < 32; ++t)
+            if (h + t < seen) mx = fmaxf(mx, __uint_as_float(sv[t]));
     }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));  // the row's other half
-    const bool grow = mx > m + RESCALE_THRESH;             // m = -inf: whenever a key is seen
+    mx = mx == -INFINITY ? mx : mx * c;
+    const bool grow = mx > m + RESCALE_THRESH;  // m = -inf: whenever a key is seen
     const float m_new = grow ? mx : m;
-    if (__any_sync(0xffffffffu, grow && j > 0)) {
-        const int pj = j - 1;
-        if (!wait_bar_warp(rc.o_full + pj % NP, (pj / NP) & 1, rc.abort_flag, rc.status))
-            return __int_as_float(0x7fffffff);
-        fence_after();
-        rescale_o(rc.tO, rc.lane_addr, grow ? ex2(m - m_new) : 1.0f);
-    }
-    const float mb = m_new == -INFINITY ? 0.0f : m_new;
+    const float bias = m_new == -INFINITY ? 0.0f : -m_new;
 #pragma unroll
-    for (int ch = 0; ch < 4; ++ch) {
-        uint32_t h[4];
+    for (int h = 0; h < 64; h += 32) {
+        uint32_t sv[32];
+        tmem_ld32(rc.tS + (j & 1) * 64 + h, sv);
+        tmem_wait_ld();
 #pragma unroll
-        for (int t = 0; t < 8; t += 2)
-            h[t >> 1] = pack_bf16(ex2(__uint_as_float(sv[ch * 8 + t]) - mb), ex2(__uint_as_float(sv[ch * 8 + t + 1]) - mb));
-        sts128(rc.sP + pb * P_BYTES + rc.prow + (((rc.ch0 + (uint32_t)ch) ^ rc.rsw) << 4), h[0], h[1], h[2], h[3]);
+        for (int t = 0; t < 32; t += 2) {  // a hidden key is 0 even where the factor is 0 or NaN
+            const float x0 = ex2(fmaf(__uint_as_float(sv[t]), c, bias)), x1 = ex2(fmaf(__uint_as_float(sv[t + 1]), c, bias));
+            p[(h + t) >> 1] = pack_bf16(h + t < seen ? x0 : 0.0f, h + t + 1 < seen ? x1 : 0.0f);
+        }
     }
     fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(rc.s_free + (j & 1));
+    if (j > 0) {
+        if (!wait_bar_warp(rc.o_full, (j - 1) & 1, rc.abort_flag, rc.status)) return __int_as_float(0x7fffffff);
+        fence_after();
+        if (__any_sync(0xffffffffu, grow)) rescale_o(rc.tO, grow ? ex2(m - m_new) : 1.0f);
+    }
+    tmem_st32(rc.tP, p);
     return m_new;
 }
 
-// Half a row (32 dims from col0) to the output, times inv.
-__device__ __forceinline__ void store_row(const AttnArgs &a, long long at, const float (&o)[32], float inv) {
+// A row to the output, times inv.
+__device__ __forceinline__ void store_row(const AttnArgs &a, long long at, const float (&o)[HD], float inv) {
     if (a.out_bf16) {
         uint4 *p = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + at);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
             p[i] = make_uint4(pack_bf16(o[8 * i] * inv, o[8 * i + 1] * inv), pack_bf16(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
                               pack_bf16(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
                               pack_bf16(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
     } else {
         float4 *p = reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + at);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 16; ++i)
             p[i] = make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
     }
 }
@@ -217,21 +281,19 @@ __global__ void __launch_bounds__(NT, 1)
         }
         for (int i = 0; i < NC; ++i) {
             mbar_init(&B.c_full[i], 1);
-            mbar_init(&B.c_empty[i], 128);
+            mbar_init(&B.c_empty[i], 4);
         }
         for (int i = 0; i < NV; ++i) {
-            mbar_init(&B.v_full[i], 128);
+            mbar_init(&B.v_full[i], 4);
             mbar_init(&B.v_empty[i], 1);
         }
         for (int t = 0; t < TILES; ++t) {
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&B.s_full[t][i], 1);
-                mbar_init(&B.s_free[t][i], NSOFT);
+                mbar_init(&B.s_free[t][i], TILE / 32);
             }
-            for (int i = 0; i < NP; ++i) {
-                mbar_init(&B.p_full[t][i], NSOFT);
-                mbar_init(&B.o_full[t][i], 1);
-            }
+            mbar_init(&B.p_full[t], TILE / 32);
+            mbar_init(&B.o_full[t], 1);
             B.lo[t] = INT_MAX;
         }
         mbar_init(&B.s_done, 1);
@@ -256,28 +318,27 @@ __global__ void __launch_bounds__(NT, 1)
             atomicMin(&B.lo[tid / TILE], l);
         }
     } else {
-        // q of one row, 32 dims a thread: scaled by a power of two to [128, 256), split into two e4m3 parts
-        const int i = tid - TILES * TILE, row = i >> 1, half = i & 1;
-        uint4 u[4] = {};
+        // q of one row a thread: scaled by a power of two to [128, 256), split into two e4m3 parts
+        const int row = tid - TILES * TILE;
+        uint4 u[8] = {};
         if (r0 + row < a.rows) {
-            const uint4 *p = reinterpret_cast<const uint4 *>(a.q + row_at(a, b, h, r0 + row, a.q_sb, a.q_st, a.q_sh) + half * 32);
+            const uint4 *p = reinterpret_cast<const uint4 *>(a.q + row_at(a, b, h, r0 + row, a.q_sb, a.q_st, a.q_sh));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) u[k] = __ldg(p + k);
+            for (int k = 0; k < 8; ++k) u[k] = __ldg(p + k);
         }
         uint32_t am = 0;
         const uint32_t *w = reinterpret_cast<const uint32_t *>(u);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) am = max(am, max((w[k] << 16) & 0x7FFFFFFFu, w[k] & 0x7FFF0000u));
-        am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
+        for (int k = 0; k < 32; ++k) am = max(am, max((w[k] << 16) & 0x7FFFFFFFu, w[k] & 0x7FFF0000u));
         const int e = max((int)(am >> 23), 8);  // 2^(134 - e) stays in range, for a zero row as well
         const float f = scale_inverse(e) * 128.0f;
         const uint32_t base = sQ + (row / TILE) * Q_BYTES + (row % TILE) * 128;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {  // 16 dims: one 16-byte piece of each part
+        for (int k = 0; k < 4; ++k) {  // 16 dims: one 16-byte piece of each part
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                float x[4], y[4];
+                float x[4];
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
                     const uint32_t ww = w[k * 8 + n * 2 + v];
@@ -288,17 +349,13 @@ __global__ void __launch_bounds__(NT, 1)
                 const uint32_t h01 = e4m3_to_half2((uint16_t)hi[n]), h23 = e4m3_to_half2((uint16_t)(hi[n] >> 16));
                 const float2 f01 = __half22float2(*reinterpret_cast<const __half2 *>(&h01));
                 const float2 f23 = __half22float2(*reinterpret_cast<const __half2 *>(&h23));
-                y[0] = x[0] - f01.x;
-                y[1] = x[1] - f01.y;
-                y[2] = x[2] - f23.x;
-                y[3] = x[3] - f23.y;
-                lo[n] = e4m3x4(y[0], y[1], y[2], y[3]);
+                lo[n] = e4m3x4(x[0] - f01.x, x[1] - f01.y, x[2] - f23.x, x[3] - f23.y);
             }
             const uint32_t sw = (uint32_t)(row & 7);
-            sts128(base + (((uint32_t)(half * 2 + k) ^ sw) << 4), hi[0], hi[1], hi[2], hi[3]);
-            sts128(base + (((uint32_t)(4 + half * 2 + k) ^ sw) << 4), lo[0], lo[1], lo[2], lo[3]);
+            sts128(base + (((uint32_t)k ^ sw) << 4), hi[0], hi[1], hi[2], hi[3]);
+            sts128(base + (((uint32_t)(4 + k) ^ sw) << 4), lo[0], lo[1], lo[2], lo[3]);
         }
-        if (half == 0) B.unit[row] = scale_value(e) * 0.0078125f * a.scale_log2;
+        B.unit[row] = scale_value(e) * 0.0078125f * a.scale_log2;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     fence_before();
@@ -361,7 +418,7 @@ __global__ void __launch_bounds__(NT, 1)
                 bool ok = true;
                 const bool elected = elect_one();
                 const uint64_t dq = make_desc(sQ, 16, 1024, LAYOUT_SW128), dk = make_desc(sK, 16, 512, LAYOUT_SW64);
-                int ks = 0, kphase = 0, pb = 0;
+                int ks = 0, kphase = 0;
                 for (int j = 0; ok && j < cnt; ++j) {
                     const int sb = j & 1;
                     if (!wait_bar_warp(&B.k_full[ks], kphase, abort_flag, a.status)) break;
@@ -370,16 +427,11 @@ __global__ void __launch_bounds__(NT, 1)
                             ok = false;
                             break;
                         }
-                        // P_j takes the place of P_{j-NP}, whose product must be done
-                        if (j >= NP && !wait_bar_warp(&B.o_full[t][pb], ((j - NP) / NP) & 1, abort_flag, a.status)) {
-                            ok = false;
-                            break;
-                        }
                         fence_after();
                         if (elected) {
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk)  // hi, hi, lo, lo against K's two halves
-                                mma_e4m3(tmem + t * 128 + sb * 64, dq + t * (Q_BYTES >> 4) + kk * 2,
+                                mma_e4m3(tmem + COL_S + t * 128 + sb * 64, dq + t * (Q_BYTES >> 4) + kk * 2,
                                          dk + ks * (BLOCK_BYTES >> 4) + (kk & 1) * 2, kk > 0 ? 1u : 0u);
                             mma_commit(&B.s_full[t][sb]);
                         }
@@ -390,7 +442,6 @@ __global__ void __launch_bounds__(NT, 1)
                         ks = 0;
                         kphase ^= 1;
                     }
-                    if (++pb == NP) pb = 0;
                 }
                 if (elected) {
                     mma_commit(&B.s_done);  // every MMA of this thread completes before tensor memory is freed
@@ -406,14 +457,13 @@ __global__ void __launch_bounds__(NT, 1)
                 const bool elected = elect_one();
                 // B = [V | ones]: the second 128-byte atom along N lies LBO bytes past the
                 // first; a step of 2048 bytes in V moves the start and the distance
-                const uint64_t dp = make_desc(smem_u32(smem + OFF_P), 16, 1024, LAYOUT_SW128);
                 const uint64_t dv = make_desc(sV, sOnes - sV, 1024, LAYOUT_SW128);
                 constexpr uint64_t V_STEP = (2048 >> 4) - ((uint64_t)(2048 >> 4) << 16);
-                int vs = 0, vphase = 0, pb = 0, pphase = 0;
+                int vs = 0, vphase = 0;
                 for (int j = 0; ok && j < cnt; ++j) {
                     if (!wait_bar_warp(&B.v_full[vs], vphase, abort_flag, a.status)) break;
                     for (int t = 0; t < nt; ++t) {
-                        if (!wait_bar_warp(&B.p_full[t][pb], pphase, abort_flag, a.status)) {
+                        if (!wait_bar_warp(&B.p_full[t], j & 1, abort_flag, a.status)) {
                             ok = false;
                             break;
                         }
@@ -421,9 +471,9 @@ __global__ void __launch_bounds__(NT, 1)
                         if (elected) {
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk)
-                                mma_f16(tmem + 256 + t * 128, dp + (t * NP + pb) * (P_BYTES >> 4) + kk * 2,
-                                        dv + (uint64_t)(vs * 4 + kk) * V_STEP, IDESC_O, (j | kk) ? 1u : 0u);
-                            mma_commit(&B.o_full[t][pb]);
+                                mma_pv(tmem + COL_O + t * O_STRIDE, tmem + COL_P + t * 32 + kk * 8,
+                                       dv + (uint64_t)(vs * 4 + kk) * V_STEP, (j | kk) ? 1u : 0u);
+                            mma_commit(&B.o_full[t]);
                         }
                         __syncwarp();
                     }
@@ -431,10 +481,6 @@ __global__ void __launch_bounds__(NT, 1)
                     if (++vs == NV) {
                         vs = 0;
                         vphase ^= 1;
-                    }
-                    if (++pb == NP) {
-                        pb = 0;
-                        pphase ^= 1;
                     }
                 }
                 if (elected) {
@@ -481,117 +527,127 @@ __global__ void __launch_bounds__(NT, 1)
                     sts128(row + (((uint32_t)(2 * qd + 1) ^ sw) << 4), o[4], o[5], o[6], o[7]);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&B.v_full[vs]);
-                mbar_arrive(&B.c_empty[cs]);
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&B.v_full[vs]);
+                    mbar_arrive(&B.c_empty[cs]);
+                }
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
         // ------------------------------------------------------------ softmax
-        const int tile = (warp - 8) >> 3, w = warp & 7;
+        const int tile = (warp - 8) >> 2, quad = warp & 3;
         if (tile < nt) {
-            const int lane0 = (w & 3) * 32 + (w >> 2) * 16;  // first tensor-memory lane of this warp
-            const int r = lane0 + (lane & 15), col0 = (lane >> 4) * 32;
-            Row rc;
-            rc.tS = tmem + tile * 128;
-            rc.tO = tmem + 256 + tile * 128;
-            rc.lane_addr = (uint32_t)lane0 << 16;
-            rc.sP = smem_u32(smem + OFF_P) + tile * NP * P_BYTES;
-            rc.prow = (uint32_t)r * 128u;
-            rc.rsw = (uint32_t)(r & 7);
-            rc.ch0 = (uint32_t)(col0 >> 3);
-            rc.col0 = col0;
-            rc.o_full = B.o_full[tile];
-            rc.s_free = B.s_free[tile];
-            rc.abort_flag = abort_flag;
-            rc.status = a.status;
+            const int r = quad * 32 + lane;
+            const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+            const uint32_t tS = lanes + COL_S + tile * 128, tO = lanes + COL_O + tile * O_STRIDE;
+            const uint32_t tP = lanes + COL_P + tile * 32;
             const float unit = B.unit[tile * TILE + r];
             const int lim = B.lim[tile * TILE + r], lo = B.lo[tile];
-            uint32_t poff[4];  // swizzled places of this thread's four pieces in its row of P
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch) poff[ch] = rc.sP + rc.prow + (((rc.ch0 + (uint32_t)ch) ^ rc.rsw) << 4);
+            const Row rc{tS, tO, tP, B.s_free[tile], &B.o_full[tile], abort_flag, a.status};
+            // K's scales of 32 pages, one a lane (NaN where V's is, or the page number is
+            // bad), times the row's unit: the factor of a page's scores is at hand before
+            // they are
+            const int32_t *table = a.table + b * a.table_stride + p0;
+            auto fetch = [&](int first) {
+                int u = 255;
+                if (first + lane < cnt) {
+                    const int id = table[first + lane];
+                    if (id >= 0 && id < a.n_pages) {
+                        u = a.K.scale[id * a.K.scale_stride + h];
+                        if (a.V.scale[id * a.V.scale_stride + h] == 255) u = 255;
+                    }
+                }
+                return scale_value(u);
+            };
+            float scales = fetch(0), scales_next = fetch(32);
             float m = -INFINITY;
-            bool ok = true, ready = false;
-            int pb = 0;
-            for (int j = 0; j < cnt; ++j) {
-                const int sb = j & 1;
-                if (!__all_sync(0xffffffffu, ready) &&
-                    !wait_bar_warp(&B.s_full[tile][sb], (j >> 1) & 1, abort_flag, a.status)) {
+            bool ok = true;
+            const int hot = max(0, min(cnt, lo / PAGE - p0));  // pages that every row sees whole
+            int j = 0;
+#pragma unroll 1
+            for (; j < hot; ++j) {
+                if ((j & 31) == 0 && j > 0) {
+                    scales = scales_next;
+                    scales_next = fetch(j + 32);
+                }
+                const float c = unit * __shfl_sync(0xffffffffu, scales, j & 31);
+                if (!wait_quick(&B.s_full[tile][j & 1], (j >> 1) & 1, abort_flag, a.status)) {
                     ok = false;
                     break;
                 }
                 fence_after();
-                const int su = B.info[j % INFO], base = (p0 + j) * PAGE;
-                const float c =
-                    unit * ((su & 255) == 255 || su >= 0xFF00 ? __int_as_float(0x7FC00000) : scale_value(su & 255));
-                if (j > 0 && base + PAGE <= lo) {
-                    uint32_t sv[32];
-                    tmem_ld_half32(rc.tS + sb * 64 + rc.lane_addr, sv);
-                    tmem_wait_ld();
-                    fence_before();
-                    mbar_arrive(&B.s_free[tile][sb]);
-                    float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+                uint32_t sv[64], p[32];
+                tmem_ld32(tS + (j & 1) * 64, sv);
+                tmem_ld32(tS + (j & 1) * 64 + 32, sv + 32);
+                tmem_wait_ld();
+                fence_before();
+                if (lane == 0) mbar_arrive(&B.s_free[tile][j & 1]);  // of the whole warp, which waited
+                float top[4];
 #pragma unroll
-                    for (int t = 0; t < 32; t += 8) {
-                        a0 = fmaxf(a0, fmaxf(__uint_as_float(sv[t]), __uint_as_float(sv[t + 1])));
-                        a1 = fmaxf(a1, fmaxf(__uint_as_float(sv[t + 2]), __uint_as_float(sv[t + 3])));
-                        a2 = fmaxf(a2, fmaxf(__uint_as_float(sv[t + 4]), __uint_as_float(sv[t + 5])));
-                        a3 = fmaxf(a3, fmaxf(__uint_as_float(sv[t + 6]), __uint_as_float(sv[t + 7])));
-                    }
-                    float mx = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)) * c;  // with the row's other half
-                    const bool grow = mx > m + RESCALE_THRESH;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float m_new = grow ? mx : m;
-                        const int pj = j - 1;
-                        if (!wait_bar_warp(&B.o_full[tile][pj % NP], (pj / NP) & 1, abort_flag, a.status)) {
-                            ok = false;
-                            break;
-                        }
-                        fence_after();
-                        rescale_o(rc.tO, rc.lane_addr, grow ? ex2(m - m_new) : 1.0f);
-                        m = m_new;
-                    }
-                    const float bias = -m;
-                    // S_{j+1} is looked for now and used after this page's exponentials
-                    ready = mbar_test_wait(smem_u32(&B.s_full[tile][sb ^ 1]), ((j + 1) >> 1) & 1);
+                for (int t = 0; t < 4; ++t) top[t] = max3(sv[3 * t], sv[3 * t + 1], sv[3 * t + 2]);
 #pragma unroll
-                    for (int ch = 0; ch < 4; ++ch) {
-                        uint32_t hh[4];
+                for (int t = 12; t < 60; t += 8)
 #pragma unroll
-                        for (int t = 0; t < 8; t += 2) {
-                            float x0, x1;
-                            fma2(x0, x1, __uint_as_float(sv[ch * 8 + t]), __uint_as_float(sv[ch * 8 + t + 1]), c, bias);
-                            hh[t >> 1] = pack_bf16(ex2(x0), ex2(x1));
-                        }
-                        sts128(poff[ch] + pb * P_BYTES, hh[0], hh[1], hh[2], hh[3]);
-                    }
-                    fence_before();
-                } else {
-                    ready = false;
-                    m = step_general(rc, j, lim - base, c, m);
-                    if (m != m) {
+                    for (int k = 0; k < 4; ++k) top[k] = max3(__float_as_uint(top[k]), sv[t + 2 * k], sv[t + 2 * k + 1]);
+                top[0] = max3(__float_as_uint(top[0]), sv[60], sv[61]);
+                top[1] = max3(__float_as_uint(top[1]), sv[62], sv[63]);
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                const bool grow = mx > m + RESCALE_THRESH;  // m = -inf: at once
+                const float m_new = grow ? mx : m;
+#pragma unroll
+                for (int t = 0; t < 64; t += 2) {
+                    float x0, x1;
+                    fma2(x0, x1, __uint_as_float(sv[t]), __uint_as_float(sv[t + 1]), c, -m_new);
+                    p[t >> 1] = pack_bf16(ex2(x0), ex2(x1));
+                }
+                // P_{j-1} has been read, and O may be rescaled, once its product is done
+                if (j > 0) {
+                    if (!wait_quick(&B.o_full[tile], (j - 1) & 1, abort_flag, a.status)) {
                         ok = false;
                         break;
                     }
+                    fence_after();
+                    if (__any_sync(0xffffffffu, grow)) rescale_o(tO, grow ? ex2(m - m_new) : 1.0f);
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&B.p_full[tile][pb]);
-                pb = pb == NP - 1 ? 0 : pb + 1;
+                m = m_new;
+                tmem_st32(tP, p);
+                tmem_wait_st();
+                fence_before();
+                if (lane == 0) mbar_arrive(&B.p_full[tile]);
+            }
+#pragma unroll 1
+            for (; ok && j < cnt; ++j) {  // a limit cuts these for some row
+                if ((j & 31) == 0 && j > 0) {
+                    scales = scales_next;
+                    scales_next = fetch(j + 32);
+                }
+                const float c = unit * __shfl_sync(0xffffffffu, scales, j & 31);
+                ok = wait_quick(&B.s_full[tile][j & 1], (j >> 1) & 1, abort_flag, a.status);
+                if (!ok) break;
+                fence_after();
+                m = step_masked(rc, j, lim - (p0 + j) * PAGE, c, m);
+                ok = m == m;
+                if (!ok) break;
+                tmem_wait_st();
+                fence_before();
+                if (lane == 0) mbar_arrive(&B.p_full[tile]);
             }
             if (ok && cnt > 0) {
-                ok = wait_bar_warp(&B.o_full[tile][(cnt - 1) % NP], ((cnt - 1) / NP) & 1, abort_flag, a.status);
+                ok = wait_bar_warp(&B.o_full[tile], (cnt - 1) & 1, abort_flag, a.status);
                 fence_after();
             }
-            float l = 0.0f, o[32];
+            float l = 0.0f, o[HD];
             if (ok && cnt > 0) {
-                uint32_t ov[32];
-                const uint32_t lv = tmem_ld_rowsum(rc.tO + HD + rc.lane_addr);
-                tmem_ld_half32(rc.tO + rc.lane_addr, ov);
+                uint32_t ov[HD];
+                const uint32_t lv = tmem_ld1(tO + HD);
+                tmem_ld32(tO, ov);
+                tmem_ld32(tO + 32, ov + 32);
                 tmem_wait_ld();
                 l = __uint_as_float(lv);
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {  // columns of V came in pairs (0, 2), (1, 3)
+                for (int i = 0; i < HD; i += 4) {  // columns of V came in pairs (0, 2), (1, 3)
                     o[i] = __uint_as_float(ov[i]);
                     o[i + 1] = __uint_as_float(ov[i + 2]);
                     o[i + 2] = __uint_as_float(ov[i + 1]);
@@ -599,11 +655,11 @@ __global__ void __launch_bounds__(NT, 1)
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+                for (int i = 0; i < HD; ++i) o[i] = 0.0f;
             }
             const int row = r0 + tile * TILE + r;
             const bool in = row < a.rows;
-            const long long at = in ? row_at(a, b, h, row, a.o_sb, a.o_st, a.o_sh) + col0 : 0;
+            const long long at = in ? row_at(a, b, h, row, a.o_sb, a.o_st, a.o_sh) : 0;
             if (splits == 1) {
                 if (in) store_row(a, at, o, l == 0.0f ? 0.0f : 1.0f / l);
             } else {
@@ -611,16 +667,14 @@ __global__ void __launch_bounds__(NT, 1)
                 float *slot = a.partial + (group * splits * TILE + r) * PART_ROW;  // this row of piece 0
                 float *mine = slot + (long long)split * TILE * PART_ROW;
 #pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                    *reinterpret_cast<float4 *>(mine + col0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                if (col0 == 0) {
-                    mine[HD] = m;
-                    mine[HD + 1] = l;
-                }
+                for (int i = 0; i < HD; i += 4)
+                    *reinterpret_cast<float4 *>(mine + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                mine[HD] = m;
+                mine[HD + 1] = l;
                 __threadfence();
-                asm volatile("bar.sync %0, 256;" ::"r"(1 + tile) : "memory");
-                if (r == 0 && col0 == 0) B.join[tile] = atomicAdd(&a.arrived[group], 1) == splits - 1;
-                asm volatile("bar.sync %0, 256;" ::"r"(1 + tile) : "memory");
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + tile) : "memory");
+                if (r == 0) B.join[tile] = atomicAdd(&a.arrived[group], 1) == splits - 1;
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + tile) : "memory");
                 if (B.join[tile] && in) {
                     __threadfence();
                     float mm = -INFINITY;
@@ -628,14 +682,14 @@ __global__ void __launch_bounds__(NT, 1)
                     const float mb = mm == -INFINITY ? 0.0f : mm;
                     float sum = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+                    for (int i = 0; i < HD; ++i) o[i] = 0.0f;
                     for (int s = 0; s < splits; ++s) {
                         const float *p = slot + (long long)s * TILE * PART_ROW;
                         const float f = ex2(__ldcg(p + HD) - mb);
                         sum = fmaf(__ldcg(p + HD + 1), f, sum);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + col0 + i));
+                        for (int i = 0; i < HD; i += 4) {
+                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + i));
                             o[i] = fmaf(v.x, f, o[i]);
                             o[i + 1] = fmaf(v.y, f, o[i + 1]);
                             o[i + 2] = fmaf(v.z, f, o[i + 2]);
