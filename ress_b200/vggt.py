@@ -118,7 +118,9 @@ class Mlp(nn.Module):
         self.fc2 = nn.Linear(ratio * dim, dim)
 
     def forward(self, x):
-        return self.fc2(F.gelu(self.fc1(x)))
+        h = self.fc1(x)
+        # an 8-bit fc1 (stream.Int8Linear) applies the GELU itself
+        return self.fc2(h if getattr(self.fc1, "act", None) == "gelu" else F.gelu(h))
 
 
 class LayerScale(nn.Module):

@@ -1,0 +1,151 @@
+"""Streaming global attention (ress_b200.stream) on the VGGT-shaped aggregator:
+frames fed one by one against the same model with exact frame-causal attention
+in fp32, and the 8-bit Linears in it.
+
+Tolerances: e4m3 keys and values err by 2^-4 of a value at most, 2 to 3 % of
+its typical size on average, independently from token to token; an attention
+output, an average over tokens, errs by about as much of its own size.  The
+module test allows 5 % in the 2-norm and the model's outputs (the residual
+stream, to which a block adds a hundredth) 2 % of the largest value, as the
+other whole-model tests do.  int8 codes err by 1/254 of a row's largest
+value."""
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from ress_b200 import kernels as K
+from ress_b200 import stream, vggt
+from ress_b200._lib import RessError
+
+pytestmark = pytest.mark.gpu
+
+IMG, FRAME = 112, 64 + 5
+
+
+def _model(dtype=torch.bfloat16):
+    torch.manual_seed(0)
+    m = vggt.VGGTAggregatorModel(dim=256, depth=2, num_heads=4, img=IMG, encoder_depth=1, intermediate=(0, 1))
+    return m.cuda().to(dtype).eval()
+
+
+def _images(streams, frames):
+    return torch.rand(streams, frames, 3, IMG, IMG, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+
+
+def _frame_causal(attn, x, pos):
+    """The attention module in fp32 with an exact frame-causal mask."""
+    B, T, C = x.shape
+    H = attn.num_heads
+    q, k, v = attn.qkv(x).view(B, T, 3, H, C // H).permute(2, 0, 3, 1, 4).unbind(0)
+    q, k = attn.rope(attn.q_norm(q), pos), attn.rope(attn.k_norm(k), pos)
+    f = torch.arange(T, device=x.device) // FRAME
+    o = F.scaled_dot_product_attention(q, k, v, attn_mask=f[:, None] >= f[None])
+    return attn.proj(o.transpose(1, 2).reshape(B, T, C))
+
+
+def _rel(a, b):
+    a, b = a.detach().double(), b.detach().double()
+    return float((a - b).norm() / b.norm())
+
+
+@pytest.mark.parametrize("streams,chunks", [(1, [1] * 5), (2, [1, 3, 1]), (1, [5])])
+def test_stream_matches_frame_causal_attention(streams, chunks):
+    ref_model, m = _model(torch.float32), _model()
+    images = _images(streams, 5)
+    for block in ref_model.aggregator.global_blocks:
+        block.attn.forward = lambda x, pos=None, _a=block.attn: _frame_causal(_a, x, pos)
+    stream.apply_stream(m, streams=streams, max_frames=5, frame_tokens=FRAME)
+    with torch.inference_mode():
+        ref, _ = ref_model(images)
+        got, at = [], 0
+        for n in chunks:
+            got.append(m(images[:, at:at + n], first_frame=at == 0)[0])
+            at += n
+    torch.cuda.synchronize()
+    assert K.check_status() == 0
+    for layer in range(2):
+        out = torch.cat([g[layer] for g in got], 1).float()
+        assert (out - ref[layer]).abs().max() <= 2e-2 * ref[layer].abs().max()
+    assert stream.stream_caches(m)[0].lens.tolist() == [5 * FRAME] * streams
+
+
+def test_stream_attention_module():
+    torch.manual_seed(2)
+    attn = vggt.Attention(256, 4, True, vggt.RotaryPosition2D()).cuda()
+    x = torch.randn(2, 3 * FRAME, 256, device="cuda")
+    pos = torch.randint(0, 9, (2, 3 * FRAME, 2), device="cuda")
+    with torch.inference_mode():
+        ref = _frame_causal(attn, x, pos)
+        for dtype in (torch.float32, torch.bfloat16):
+            a = attn.to(dtype)
+            cache, pro = stream.StreamCache(2, 4, 3 * FRAME), stream._prologue(a)
+            one = [stream.stream_attention_forward(a, x[:, i:i + FRAME].to(dtype), pos[:, i:i + FRAME], cache, FRAME, pro)
+                   for i in range(0, 3 * FRAME, FRAME)]
+            cache.reset()
+            whole = stream.stream_attention_forward(a, x.to(dtype), pos, cache, FRAME, pro)
+            assert whole.dtype == dtype
+            assert _rel(torch.cat(one, 1), ref) < 0.05 and _rel(whole, ref) < 0.05
+    assert K.check_status() == 0
+
+
+def test_int8_linears_in_a_stream():
+    m, q = _model(), _model()
+    n = stream.quantize_linears(q.aggregator.frame_blocks) + stream.quantize_linears(q.aggregator.global_blocks)
+    assert n == 4 * 4  # qkv, proj, fc1, fc2 of four blocks
+    images = _images(1, 3)
+    outs = []
+    for model in (m, q):
+        stream.apply_stream(model, max_frames=3, frame_tokens=FRAME)
+        with torch.inference_mode():
+            outs.append([model(images[:, i:i + 1], first_frame=i == 0)[0] for i in range(3)])
+    torch.cuda.synchronize()
+    assert K.check_status() == 0
+    for a, b in zip(*outs):
+        for x, y in zip(a, b):
+            assert (x.float() - y.float()).abs().max() <= 2e-2 * x.float().abs().max()
+
+
+def test_int8_linear_module():
+    torch.manual_seed(3)
+    lin = torch.nn.Linear(256, 96).cuda()
+    x = torch.randn(4, 50, 256, device="cuda")
+    q = stream.Int8Linear(lin)
+    assert _rel(q(x), lin(x)) < 0.02
+    assert _rel(stream.Int8Linear(lin, "gelu")(x), F.gelu(lin(x))) < 0.02
+    b = stream.Int8Linear(torch.nn.Linear(256, 96, bias=False).cuda()).bfloat16()
+    assert b.scale.dtype == torch.float32 and b.w8.dtype == torch.int8 and b(x.bfloat16()).dtype == torch.bfloat16
+    assert (q.weight - lin.weight).abs().max() <= lin.weight.abs().max() / 254 * 1.01
+    mlp = vggt.Mlp(64).cuda()
+    y = torch.randn(30, 64, device="cuda")
+    ref = mlp(y)
+    assert stream.quantize_linears(mlp) == 2 and mlp.fc1.act == "gelu" and mlp.fc2.act is None
+    assert _rel(mlp(y), ref) < 0.03
+
+
+def test_reset_remove_and_refusals():
+    m = _model()
+    images = _images(1, 2)
+    before = [b.attn.forward for b in m.aggregator.global_blocks]
+    with torch.inference_mode():
+        ref = m(images)[0]
+        stream.apply_stream(m, max_frames=2, frame_tokens=FRAME)
+        first = m(images[:, :1])[0]
+        m(images[:, 1:], first_frame=False)
+        with pytest.raises(RessError, match="do not fit"):
+            m(images[:, :1], first_frame=False)
+        stream.reset_stream(m)
+        again = m(images[:, :1])[0]
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+        with pytest.raises(RessError, match="whole number of frames"):
+            stream.stream_attention_forward(m.aggregator.global_blocks[0].attn,
+                                            torch.zeros(1, FRAME + 1, 256, device="cuda").bfloat16(), None,
+                                            stream.stream_caches(m)[0], FRAME, {})
+        stream.remove_stream(m)
+        assert all(torch.equal(a, b) for a, b in zip(m(images)[0], ref))
+    assert [b.attn.forward for b in m.aggregator.global_blocks] == before
+    with pytest.raises(RessError):
+        stream.StreamCache(1, 0, 10)
+    odd = vggt.Attention(96, 3, True, None)  # 32 head dims
+    with pytest.raises(RessError, match="64 head dims"):
+        stream._prologue(odd)
