@@ -57,6 +57,27 @@ def test_linear(m, k, n, dtype):
         assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("m,k,n", [(12001, 1008, 1024), (9999, 1024, 1000), (8200, 2064, 1024), (5000, 4096, 1016)])
+def test_linear_over_several_waves(m, k, n):
+    """Tiles for several waves of the GPU; rows of a
+    wider tensor, a zero row and one that is not finite among them."""
+    x, w, bias = _inputs(m, k + 16, n, torch.bfloat16, seed=m)
+    x, w = x[:, 8:k + 8], w[:, :k].contiguous()
+    x[m // 2] = 0
+    x[m - 1, 3] = torch.inf
+    w8, sw = K.int8_quant_rows(w)
+    out = K.int8_linear(x, w8, sw, bias, act="gelu")
+    torch.cuda.synchronize()
+    assert K.check_status() == 0
+    x8, sx = quant_rows(x)
+    _check(out[:-1], x8[:-1], sx[:-1], w8, sw, bias, "gelu")
+    assert bool(out[-1].isnan().all())
+    for _ in range(3):
+        assert torch.equal(K.int8_linear(x, w8, sw, bias, act="gelu")[:-1], out[:-1])
+    # the same bits as among few tokens
+    assert torch.equal(K.int8_linear(x[77:177], w8, sw, bias, act="gelu"), out[77:177])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("m,k", [(1, 16), (7, 80), (1000, 1040), (33, 4096)])
 def test_quant_rows(m, k, dtype):
