@@ -145,6 +145,9 @@ template <> struct Piece<float> {
 template <typename T, int CH>
 __global__ void __launch_bounds__(QUANT_NT) quant_rows_kernel(const T *__restrict__ x, long long x_st, int M, int K,
                                                               int8_t *__restrict__ q, float *__restrict__ scale) {
+    // the product's CTAs may start (and set themselves up) once every CTA of this
+    // kernel has; they wait for its end before they read anything of it
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const long long m = ((long long)blockIdx.x * QUANT_NT + threadIdx.x) >> 5;
     if (m >= M) return;
@@ -453,6 +456,7 @@ __global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CU
     pair_sync<CG>();  // the peer's barriers exist before anything arrives on them
     fence_after();
     const uint32_t tmem = B.tmem;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the tokens' codes and scales are there
 
     if (warp == 0) {
         if (lane == 0) {
@@ -664,12 +668,14 @@ static int launch_gemm(const int8_t *x8, const float *sx, const LinArgs &a, int3
     cfg.blockDim = dim3(C::NT);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CG;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = CG;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kern, tx, tw, to, a, sx, tma_out, status) == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
 }
 
@@ -696,10 +702,12 @@ static size_t workspace(int M, int K) {
 // waves over the GPU are estimated to cost least, in cycles.  A K = 128 slice
 // takes the longer of its MMAs (an MMA of K = 32 reads 128 + BN rows of 32
 // bytes at 128 bytes a cycle and computes 8192 products a cycle: 128, 64, 64,
-// 48 cycles) and its copies (40 bytes a cycle and SM with all SMs copying,
-// measured at 43,968 x 4096 -> 1024; about 80 for a few).  The epilogue of a
-// wave overlaps the next wave's slices.  Measured: 43,968 x 4096 -> 1024 runs
-// 130 us on <pair, 256> and 207 us on <pair, 128>.
+// 48 cycles) and its copies (40 bytes a cycle and SM with all SMs copying, as
+// measured; about 80 for a few; a pair's smaller slices are no faster than its
+// larger ones).  The epilogue of a wave overlaps the next wave's slices; pairs
+// start and end 3000 cycles later.  Measured, us on the four tiles: 43,968 x
+// 1024 -> 1024: 74, 90, 85, 135; 1374 x 1024 -> 4096 with GELU: 19.0, 19.4,
+// 17.5, 22.1; 165 x 1536 -> 1000: 12.6, 11.5, 10.3, 10.2.
 static int pick_tile(const LinArgs &a) {
     const int cg[4] = {2, 2, 1, 1}, bn[4] = {256, 128, 128, 64}, mma[4] = {128, 64, 64, 48};
     const double slices = (a.K + 127) / 128;
@@ -709,10 +717,10 @@ static int pick_tile(const LinArgs &a) {
         const long long tiles = (long long)((a.M + 128 * cg[i] - 1) / (128 * cg[i])) * ((a.N + bn[i] - 1) / bn[i]);
         const long long slots = 148 / cg[i], waves = (tiles + slots - 1) / slots;
         const double active = (double)((tiles < slots ? tiles : slots) * cg[i]);
-        const double rate = active > 74 ? 5920.0 / active : 80.0, bytes = 128.0 * (128 + bn[i] / cg[i]);
+        const double rate = active > 74 ? 5920.0 / active : 80.0, bytes = 128.0 * (bn[i] > 64 ? 256 : 192);
         const double slice = bytes / rate > 4 * mma[i] ? bytes / rate : 4 * mma[i];
         const double epilogue = bn[i] * (a.gelu ? 30.0 : 12.0), main = slices * slice;
-        const double cost = waves * (main > epilogue ? main : epilogue) + epilogue;
+        const double cost = waves * (main > epilogue ? main : epilogue) + epilogue + (cg[i] > 1 ? 3000.0 : 0.0);
         if (cost < least) {
             least = cost;
             best = i;
