@@ -82,26 +82,35 @@ __device__ __forceinline__ uint32_t amax8(const float (&x)[8]) {
     return m;
 }
 
-// GELU: y Phi(y) = max(y, 0) - |y| Phi(-|y|).  log2 Phi(-u) is a smooth function,
-// here its polynomial of degree 7 on [0, 6.5] (fitted so that Phi's largest
-// error is least: 1.1e-7; beyond 6.5, Phi(-u) < 5e-11): one exponential and no
-// reciprocal, where the epilogue is bound by the exponential unit.
-__device__ __forceinline__ float gelu(float y) {
-    const float u = fminf(fabsf(y), 6.5f);
-    float p = 8.481062650e-06f, e, top;
-    p = fmaf(p, u, -5.400051305e-05f);
-    p = fmaf(p, u, -4.209168255e-04f);
-    p = fmaf(p, u, 7.388782687e-03f);
-    p = fmaf(p, u, -5.269075559e-02f);
-    p = fmaf(p, u, -4.591532648e-01f);
-    p = fmaf(p, u, -1.151110888f);
-    p = fmaf(p, u, -0.9999998808f);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(p));
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(y), "f"(0.0f));
-    return fmaf(-u, e, top);
+// GELU of two values: y Phi(y) = max(y, 0) - |y| Phi(-|y|).  log2 Phi(v) is a
+// smooth function, here its polynomial of degree 7 on [-6.5, 0] (fitted so that
+// Phi's largest error is least: 1.1e-7; below, Phi < 5e-11): one exponential and
+// no reciprocal, and packed arithmetic, where the instructions issued bound the
+// epilogue (10,992 x 1024 -> 4096: a rational form of erfc 58 us, this polynomial
+// 54, packed 49).
+__device__ __forceinline__ f32x2 twice(float x) { return f2_pack(x, x); }
+__device__ __forceinline__ f32x2 gelu(f32x2 yy) {
+    float y0, y1, p0, p1;
+    f2_unpack(yy, y0, y1);
+    const f32x2 v = f2_pack(fmaxf(-fabsf(y0), -6.5f), fmaxf(-fabsf(y1), -6.5f));
+    f32x2 p = twice(-8.481062650e-06f);
+    p = f2_fma_rn(p, v, twice(-5.400051305e-05f));
+    p = f2_fma_rn(p, v, twice(4.209168255e-04f));
+    p = f2_fma_rn(p, v, twice(7.388782687e-03f));
+    p = f2_fma_rn(p, v, twice(5.269075559e-02f));
+    p = f2_fma_rn(p, v, twice(-4.591532648e-01f));
+    p = f2_fma_rn(p, v, twice(1.151110888f));
+    p = f2_fma_rn(p, v, twice(-0.9999998808f));
+    f2_unpack(p, p0, p1);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(p0));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(p1));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y0) : "f"(0.0f));  // a NaN stays one
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y1) : "f"(0.0f));
+    return f2_fma_rn(v, f2_pack(p0, p1), f2_pack(y0, y1));
 }
-__device__ __forceinline__ float scaled(int acc, float sx, float sw, float bias) {
-    return __fmaf_rn(__fmul_rn((float)acc, sx), sw, bias);
+// an accumulator times its row's and channel's scales, plus the channel's bias
+__device__ __forceinline__ f32x2 scaled(int acc0, int acc1, f32x2 s_row, f32x2 s_w, f32x2 bias) {
+    return f2_fma_rn(f2_mul_rn(f2_pack((float)acc0, (float)acc1), s_row), s_w, bias);
 }
 
 // Rows to int8 with one scale each: one warp per row, eight values a lane at
@@ -290,8 +299,10 @@ __global__ void __launch_bounds__(FEW_NT) few_kernel(const T *__restrict__ x, lo
         int acc = 0;
 #pragma unroll
         for (int w = 0; w < FEW_WARPS; ++w) acc += sums[w][r][col];
-        float y = scaled(acc, sx[r], a.w_scale[n], a.bias != nullptr ? a.bias[n] : 0.0f);
-        if (a.gelu) y = gelu(y);
+        f32x2 yy = scaled(acc, acc, twice(sx[r]), twice(a.w_scale[n]), twice(a.bias != nullptr ? a.bias[n] : 0.0f));
+        if (a.gelu) yy = gelu(yy);
+        float y, same;
+        f2_unpack(yy, y, same);
         DT<O>::store(reinterpret_cast<O *>(a.out), (size_t)(r * a.out_st + n), y);
     }
 }
@@ -393,20 +404,19 @@ template <int CG> __device__ __forceinline__ void pair_sync() {
         __syncthreads();
     }
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+// Sixteen rows of 32 columns: a lane gets two columns of two rows of each eight
+// columns, so that one load of a channel pair's scales serves several rows.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr));
 }
 
 struct GemmBars {
     uint64_t full[8], empty[8], acc_full[2], acc_free[2];
-    float w_scale[256], bias[256];  // of the tile's channels
+    float w_scale[2][256], bias[2][256];  // of this tile's and the next one's channels
     uint32_t tmem;
     int abort_flag;
 };
@@ -519,26 +529,29 @@ __global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CU
         unsigned char *out_s = smem + C::OFF_OUT + (warp - 4) * C::OUT_BYTES;
         const uint32_t out_a = smem_u32(out_s);
         int n = 0;
-        // one channel's scale and bias a thread, asked for a tile ahead (behind the
-        // operands' copies they take microseconds)
+        // one channel's scale and bias a thread and its row's scale, asked for a tile
+        // ahead (behind the operands' copies they take microseconds)
         const int ch = threadIdx.x - 128;
-        float next_w = 0.0f, next_b = 0.0f;
+        float next_w = 0.0f, next_b = 0.0f, next_s = 0.0f;
         bool aborted = false;
         auto ask = [&](int tile) {
             const int col = (tile % tiles_n) * BN + ch;
+            const int m = (tile / tiles_n) * 128 * CG + rank * 128 + quad * 32 + lane;
             const bool in = tile < tiles && ch < BN && col < a.N;
             next_w = in ? __ldg(a.w_scale + col) : 0.0f;
             next_b = in && a.bias != nullptr ? __ldg(a.bias + col) : 0.0f;
+            next_s = tile < tiles && m < a.M ? sx[m] : 0.0f;
         };
         ask(first);
         for (int tile = first; tile < tiles; tile += step, ++n) {
             const int buf = n & 1;
             const int m0 = (tile / tiles_n) * 128 * CG + rank * 128 + quad * 32, n0 = (tile % tiles_n) * BN;
-            const int m = m0 + lane;
-            const float s_row = m < a.M ? sx[m] : 0.0f;
-            asm volatile("bar.sync 1, 256;" ::: "memory");  // everyone is done with the tile before
-            B.w_scale[ch] = next_w;
-            B.bias[ch] = next_b;
+            f32x2 s_row[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_row[i] = twice(__shfl_sync(~0u, next_s, 8 * i + (lane >> 2)));
+            const float *const w_scale = B.w_scale[buf], *const bias = B.bias[buf];
+            B.w_scale[buf][ch] = next_w;  // last read two tiles ago, before everyone's last barrier
+            B.bias[buf][ch] = next_b;
             ask(tile + step);
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const bool ok = wait_bar_warp(&B.acc_full[buf], (n >> 1) & 1, abort_flag, status);
@@ -553,50 +566,63 @@ __global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CU
                 __syncwarp();
 #pragma unroll
                 for (int part = 0; part < C::OUT_COLS; part += 32) {
-                    uint32_t v[32];
-                    tmem_ld32(tq + c + part, v);
+                    uint32_t v[2][16];
+                    tmem_ld16(tq + c + part, v[0]);
+                    tmem_ld16(tq + c + part + (16u << 16), v[1]);
                     tmem_wait_ld();
-                    const int col = n0 + c + part;
+                    const int cp = c + part + 2 * (lane & 3), col = n0 + cp;
+                    f32x2 y[4][4];  // rows 8 r + lane / 4, columns 8 g + 2 (lane % 4) and the next
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 w = *reinterpret_cast<const float4 *>(&B.w_scale[c + part + i]);
-                        const float4 bb = *reinterpret_cast<const float4 *>(&B.bias[c + part + i]);
-                        v[i] = __float_as_uint(scaled((int)v[i], s_row, w.x, bb.x));
-                        v[i + 1] = __float_as_uint(scaled((int)v[i + 1], s_row, w.y, bb.y));
-                        v[i + 2] = __float_as_uint(scaled((int)v[i + 2], s_row, w.z, bb.z));
-                        v[i + 3] = __float_as_uint(scaled((int)v[i + 3], s_row, w.w, bb.w));
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x2 w = *reinterpret_cast<const f32x2 *>(&w_scale[cp + 8 * g]);
+                        const f32x2 b = *reinterpret_cast<const f32x2 *>(&bias[cp + 8 * g]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t *const acc = &v[r >> 1][4 * g + 2 * (r & 1)];
+                            y[g][r] = scaled((int)acc[0], (int)acc[1], s_row[r], w, b);
+                        }
                     }
                     if (a.gelu) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(gelu(__uint_as_float(v[i])));
+                        for (int i = 0; i < 16; ++i) y[i >> 2][i & 3] = gelu(y[i >> 2][i & 3]);
                     }
                     if (tma_out) {
-                        // 16-byte pieces of the lane's row, 128B-swizzled
-                        constexpr int PER = 16 / (int)sizeof(O);
+                        // 16-byte pieces of 32 rows, 128B-swizzled
 #pragma unroll
-                        for (int i = 0; i < 32; i += PER) {
-                            uint4 w;
+                        for (int g = 0; g < 4; ++g) {
                             if constexpr (sizeof(O) == 2) {
                                 uint32_t x[4];
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const __nv_bfloat162 h =
-                                        __floats2bfloat162_rn(__uint_as_float(v[i + 2 * j]), __uint_as_float(v[i + 2 * j + 1]));
-                                    x[j] = *reinterpret_cast<const uint32_t *>(&h);
+                                for (int r = 0; r < 4; ++r) {
+                                    float y0, y1;
+                                    f2_unpack(y[g][r], y0, y1);
+                                    const __nv_bfloat162 h = __floats2bfloat162_rn(y0, y1);
+                                    x[r] = *reinterpret_cast<const uint32_t *>(&h);
                                 }
-                                w = make_uint4(x[0], x[1], x[2], x[3]);
+                                const uint32_t at = out_a + lane * 128 + (((part / 8 + g) ^ (lane & 7)) << 4);
+                                asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at),
+                                             "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
+                                             : "memory");
                             } else {
-                                w = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                            }
-                            const int piece = (part + i) / PER;
-                            *reinterpret_cast<uint4 *>(out_s + lane * 128 + ((piece ^ (lane & 7)) << 4)) = w;
-                        }
-                    } else if (m < a.M) {
+                                const int piece = 2 * g + ((lane & 3) >> 1);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (col + i < a.N)
-                                DT<O>::store(reinterpret_cast<O *>(a.out), (size_t)(m * a.out_st + col + i),
-                                             __uint_as_float(v[i]));
+                                for (int r = 0; r < 4; ++r) {
+                                    const int row = 8 * r + (lane >> 2);
+                                    *reinterpret_cast<f32x2 *>(out_s + row * 128 + ((piece ^ (row & 7)) << 4) + (lane & 1) * 8) =
+                                        y[g][r];
+                                }
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int row = m0 + 8 * (i & 3) + (lane >> 2), to = col + 8 * (i >> 2);
+                            O *const out = reinterpret_cast<O *>(a.out);
+                            float y0, y1;
+                            f2_unpack(y[i >> 2][i & 3], y0, y1);
+                            if (row < a.M && to < a.N) DT<O>::store(out, (size_t)(row * a.out_st + to), y0);
+                            if (row < a.M && to + 1 < a.N) DT<O>::store(out, (size_t)(row * a.out_st + to + 1), y1);
+                        }
                     }
                 }
                 if (tma_out) {
@@ -612,8 +638,10 @@ __global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CU
             fence_before();
             __syncwarp();
             if (lane == 0) {
+                // only tensor memory changes hands: a releasing arrive would wait for the
+                // loads asked ahead (2,000 to 2,900 cycles of a tile's 10,000)
                 if constexpr (CG == 2)
-                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
                                      leader_addr(smem_u32(&B.acc_free[buf])))
                                  : "memory");
                 else
