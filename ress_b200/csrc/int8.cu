@@ -728,22 +728,23 @@ static size_t workspace(int M, int K) {
     return use_few(M, K) ? 0 : ((size_t)M * K + 255) / 256 * 256 + (size_t)M * sizeof(float);
 }
 
-// The tile (of <pair, 256>, <pair, 128>, <single, 128>, <single, 64>) whose
-// waves over the GPU are estimated to cost least, in cycles.  A K = 128 slice
-// takes the longer of its MMAs (an MMA of K = 32 reads 128 + BN rows of 32
-// bytes at 128 bytes a cycle and computes 8192 products a cycle: 128, 64, 64,
-// 48 cycles) and its copies (40 bytes a cycle and SM with all SMs copying, as
-// measured; about 80 for a few; a pair's smaller slices are no faster than its
-// larger ones).  The epilogue of a wave overlaps the next wave's slices; pairs
-// start and end 3000 cycles later.  Measured, us on the four tiles: 43,968 x
-// 1024 -> 1024: 74, 90, 85, 135; 1374 x 1024 -> 4096 with GELU: 19.0, 19.4,
-// 17.5, 22.1; 165 x 1536 -> 1000: 12.6, 11.5, 10.3, 10.2.
+// The tile (of <pair, 256>, <single, 128>, <single, 64>) whose waves over the
+// GPU are estimated to cost least, in cycles.  A K = 128 slice takes the longer
+// of its MMAs (an MMA of K = 32 reads 128 + BN rows of 32 bytes at 128 bytes a
+// cycle and computes 8192 products a cycle: 128, 64, 48 cycles) and its copies
+// (40 bytes a cycle and SM with all SMs copying, as measured; about 80 for a
+// few; a tile of 64 channels' smaller slices are no faster than in proportion).
+// The epilogue of a wave overlaps the next wave's slices; pairs start and end
+// 3000 cycles later.  Measured, us on the three tiles, quantiser included:
+// 43,968 x 1024 -> 1024: 64, 83, 132; 1374 x 1024 -> 4096 with GELU: 15.0,
+// 15.6, 20.0; 1374 x 4096 -> 1024: 19.5, 18.3, 27.8; 165 x 1536 -> 1000: 10.6,
+// 9.3, 8.9 (a pair's tiles of 128 channels: 85, 16.2, 18.8, 9.6).
 static int pick_tile(const LinArgs &a) {
-    const int cg[4] = {2, 2, 1, 1}, bn[4] = {256, 128, 128, 64}, mma[4] = {128, 64, 64, 48};
+    const int cg[3] = {2, 1, 1}, bn[3] = {256, 128, 64}, mma[3] = {128, 64, 48};
     const double slices = (a.K + 127) / 128;
     int best = 0;
     double least = 1e300;
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 3; ++i) {
         const long long tiles = (long long)((a.M + 128 * cg[i] - 1) / (128 * cg[i])) * ((a.N + bn[i] - 1) / bn[i]);
         const long long slots = 148 / cg[i], waves = (tiles + slots - 1) / slots;
         const double active = (double)((tiles < slots ? tiles : slots) * cg[i]);
@@ -769,8 +770,7 @@ static int linear(const void *x, long long x_st, const LinArgs &a, void *ws, int
     if (rc != RESS_OK) return rc;
     switch (pick_tile(a)) {
         case 0: return launch_gemm<2, 256, O>(x8, sx, a, status, s);
-        case 1: return launch_gemm<2, 128, O>(x8, sx, a, status, s);
-        case 2: return launch_gemm<1, 128, O>(x8, sx, a, status, s);
+        case 1: return launch_gemm<1, 128, O>(x8, sx, a, status, s);
         default: return launch_gemm<1, 64, O>(x8, sx, a, status, s);
     }
 }
