@@ -1,15 +1,15 @@
 // cache.cu -- new tokens into the paged 8-bit cache: q/k LayerNorm, the 2-D
 // rotary embedding and the quantisation in one pass over the projection.
 //
-// A CTA takes one page of a stream and a few of its heads in turn: 512
-// threads, eight per token slot.  Thread i of the eight holds dims d..d+3 and
-// d+16..d+19, d = 32*(i/4) + 4*(i%4): the two halves of a rotated pair meet
-// in one thread, the eight's loads still cover the row, and cos and sin are
-// read once for all heads.  With the page in registers its largest magnitude
-// is one reduction away, and codes are written once.  A head's rows are asked
-// for while the head before is worked on.  All math is fp32, two lanes an
-// instruction: LayerNorm (mean, then mean of squared deviations), the
-// rotation x*cos + rotate_half(x)*sin, then
+// A CTA takes one page of a stream and a few of its heads in turn: 256
+// threads, eight per token, two tokens a thread.  Thread i of the eight holds
+// dims d..d+3 and d+16..d+19, d = 32*(i/4) + 4*(i%4): the two halves of a
+// rotated pair meet in one thread, the eight's loads still cover the row, and
+// cos and sin are read once for all heads.  With the page in registers its
+// largest magnitude is one reduction away, and codes are written once.  A
+// head's rows are asked for while the head before is worked on.  All math is
+// fp32, two lanes an instruction: LayerNorm (mean, then mean of squared
+// deviations), the rotation x*cos + rotate_half(x)*sin, then
 //     e = the least integer with max|y| <= 448 * 2^e,  code = e4m3(y / 2^e)
 // over the page's new tokens of that head; a page that holds tokens already
 // keeps the larger of its scale and the new one, and its old codes move by
@@ -17,12 +17,20 @@
 // page's scale NaN, so that attention over it shows it.
 // Heads vary fastest in the grid: CTAs that run together read whole rows of
 // the projection.  q rows of a shared key/value head are taken in turn.
+//
+// 43,968 tokens of 16 heads, bf16, with norms and rotation: 450 MB, 115 us, 3.9
+// TB/s of the 6.45 that a copy reaches; what bounds it is the L1's loads and the
+// instructions issued.  The norms' weights are a third of the loads, which two
+// tokens a thread share: with one token a thread 156 us (at twice the warps),
+// with four 151 (spilling).  A single token 3.5 us, 24 streams of five 4.9, a
+// frame of 1374 tokens 7.9, each close to a launch and two memory latencies.
 #include "cache.cuh"
 
 namespace ress {
 namespace cache {
 
-constexpr int APP_NT = PAGE * 8;
+constexpr int ROWS = 2;  // of a thread, PAGE / ROWS slots apart
+constexpr int APP_NT = PAGE / ROWS * 8;
 
 struct AppendArgs {
     const void *q, *k, *v;
@@ -110,34 +118,49 @@ __device__ __forceinline__ float row_sum(f32x2 x) {
 }
 __device__ __forceinline__ f32x2 twice(float x) { return f2_pack(x, x); }
 
-// LayerNorm (where w is given) and rotation of a row, unrounded.  All lanes of
-// the warp take part.  sn holds sin of dims 16..19 on, and -sin of dims 0..3.
-__device__ __forceinline__ void norm_rotate(f32x2 (&x)[4], int d, float eps, const float *w, const float *b, bool rope,
-                                            const f32x2 (&cs)[4], const f32x2 (&sn)[4]) {
+// LayerNorm (where w is given) and rotation of a thread's rows, unrounded.  All
+// lanes of the warp take part.  sn holds sin of dims 16..19 on, and -sin of
+// dims 0..3.
+__device__ __forceinline__ void norm_rotate(f32x2 (&x)[ROWS][4], int d, float eps, const float *w, const float *b,
+                                            bool rope, const f32x2 (&cs)[ROWS][4], const f32x2 (&sn)[ROWS][4]) {
     if (w != nullptr) {
-        const f32x2 mean = twice(-row_sum(f2_add_rn(f2_add_rn(x[0], x[1]), f2_add_rn(x[2], x[3]))) * (1.0f / HD));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = f2_add_rn(x[i], mean);
-        f32x2 sq = f2_mul_rn(x[0], x[0]);
+        for (int r = 0; r < ROWS; ++r) {
+            const f32x2 mean =
+                twice(-row_sum(f2_add_rn(f2_add_rn(x[r][0], x[r][1]), f2_add_rn(x[r][2], x[r][3]))) * (1.0f / HD));
 #pragma unroll
-        for (int i = 1; i < 4; ++i) sq = f2_fma_rn(x[i], x[i], sq);
-        const f32x2 rstd = twice(rsqrtf(fmaf(row_sum(sq), 1.0f / HD, eps)));
+            for (int i = 0; i < 4; ++i) x[r][i] = f2_add_rn(x[r][i], mean);
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            f32x2 sq = f2_mul_rn(x[r][0], x[r][0]);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) sq = f2_fma_rn(x[r][i], x[r][i], sq);
+            const f32x2 rstd = twice(rsqrtf(fmaf(row_sum(sq), 1.0f / HD, eps)));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[r][i] = f2_mul_rn(x[r][i], rstd);
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             f32x2 w0, w1, b0, b1;
             affine4(w + d + 16 * i, w0, w1);
             affine4(b + d + 16 * i, b0, b1);
-            x[2 * i] = f2_fma_rn(f2_mul_rn(x[2 * i], rstd), w0, b0);
-            x[2 * i + 1] = f2_fma_rn(f2_mul_rn(x[2 * i + 1], rstd), w1, b1);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                x[r][2 * i] = f2_fma_rn(x[r][2 * i], w0, b0);
+                x[r][2 * i + 1] = f2_fma_rn(x[r][2 * i + 1], w1, b1);
+            }
         }
     }
     if (rope) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const f32x2 lo = x[i], hi = x[2 + i];
-            x[i] = f2_fma_rn(lo, cs[i], f2_mul_rn(hi, sn[i]));
-            x[2 + i] = f2_fma_rn(hi, cs[2 + i], f2_mul_rn(lo, sn[2 + i]));
-        }
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const f32x2 lo = x[r][i], hi = x[r][2 + i];
+                x[r][i] = f2_fma_rn(lo, cs[r][i], f2_mul_rn(hi, sn[r][i]));
+                x[r][2 + i] = f2_fma_rn(hi, cs[r][2 + i], f2_mul_rn(lo, sn[r][2 + i]));
+            }
     }
 }
 
@@ -181,52 +204,74 @@ __device__ __noinline__ void move_codes(uint8_t *p, float f) {
 
 // heads: of the cache; the CTA takes [blockIdx.x * per, .. + per) of them.
 template <typename T>
-__global__ void __launch_bounds__(APP_NT, sizeof(T) == 2 ? 2 : 1) append_kernel(const AppendArgs a, int heads, int per) {
-    __shared__ uint32_t red[2][2][APP_NT / 32];
+__global__ void __launch_bounds__(APP_NT, 2) append_kernel(const AppendArgs a, int heads, int per) {
+    constexpr int WARPS = APP_NT / 32;
+    __shared__ uint32_t red[2][2][WARPS];
     const int b = blockIdx.z;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int slot = threadIdx.x >> 3, i8 = threadIdx.x & 7, d = (i8 >> 2) * 32 + (i8 & 3) * 4;
     const int len_raw = a.lens[b];
     const int len = max(len_raw, 0);
     const int fill = len % PAGE;
-    const int t = (int)blockIdx.y * PAGE + slot - fill;  // the new token that falls into this slot
     const int n_new = a.n_new != nullptr ? min(max(a.n_new[b], 0), a.T) : a.T;
-    const bool row = t >= 0 && t < a.T;  // there is a q row (written for padding tokens as well)
-    const bool fresh = t >= 0 && t < n_new;
     if (blockIdx.y > 0 && (int)blockIdx.y * PAGE - fill >= a.T) return;
     const int h0 = blockIdx.x * per, h1 = min(h0 + per, heads);
-
-    const T *kp = reinterpret_cast<const T *>(a.k) + b * a.k_sb + t * a.k_st + d;
-    const T *vp = reinterpret_cast<const T *>(a.v) + b * a.v_sb + t * a.v_st + d;
-    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.q_sb + t * a.q_st + d;
-    const bool has_q = a.q != nullptr, rope = a.cos != nullptr;
-    Raw<T> rk, rv, rq;
-    rk.clear();
-    rv.clear();
-    rq.clear();
-    auto ask_kv = [&](int h) {
-        if (fresh) {
-            rk.load(kp + h * a.k_sh);
-            rv.load(vp + h * a.v_sh);
-        }
-    };
-    auto ask_q = [&](int h) {
-        if (has_q && row) rq.load(qp + (long long)h * a.group * a.q_sh);
-    };
-    ask_kv(h0);
-    ask_q(h0);
-    f32x2 cs[4] = {}, sn[4] = {};
-    if (rope && row) {
-        const long long pa = a.pos[((long long)b * a.T + t) * 2 + (d >> 5)];
-        const int p = (int)(pa < 0 ? 0 : (pa >= a.rope_len ? a.rope_len - 1 : pa));
-        Raw<T> rc, rs;
-        rc.load(reinterpret_cast<const T *>(a.cos) + (size_t)p * 32 + (d & 31));
-        rs.load(reinterpret_cast<const T *>(a.sin) + (size_t)p * 32 + (d & 31));
-        rc.get(cs);
-        rs.get(sn);
+    // the new token that falls into the thread's first slot; the others follow
+    // PAGE / ROWS tokens apart
+    const int t0 = (int)blockIdx.y * PAGE + slot - fill;
+    bool row[ROWS], fresh[ROWS];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) sn[i] ^= 0x8000000080000000ull;
+    for (int r = 0; r < ROWS; ++r) {
+        const int t = t0 + r * (PAGE / ROWS);
+        row[r] = t >= 0 && t < a.T;  // there is a q row (written for padding tokens as well)
+        fresh[r] = t >= 0 && t < n_new;
     }
+
+    const T *kp = reinterpret_cast<const T *>(a.k) + b * a.k_sb + t0 * a.k_st + d;
+    const T *vp = reinterpret_cast<const T *>(a.v) + b * a.v_sb + t0 * a.v_st + d;
+    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.q_sb + t0 * a.q_st + d;
+    const bool has_q = a.q != nullptr, rope = a.cos != nullptr;
+    Raw<T> rk[ROWS], rv[ROWS], rq[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        rk[r].clear();
+        rv[r].clear();
+        rq[r].clear();
+    }
+    auto ask_k = [&](int h) {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            if (fresh[r]) rk[r].load(kp + r * (PAGE / ROWS) * a.k_st + h * a.k_sh);
+    };
+    auto ask_v = [&](int h) {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            if (fresh[r]) rv[r].load(vp + r * (PAGE / ROWS) * a.v_st + h * a.v_sh);
+    };
+    auto ask_q = [&](long long h) {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            if (has_q && row[r]) rq[r].load(qp + r * (PAGE / ROWS) * a.q_st + h * a.q_sh);
+    };
+    // fp32 rows leave no registers to ask for a head's v and q a head ahead
+    constexpr bool AHEAD = sizeof(T) == 2;
+    ask_k(h0);
+    ask_v(h0);
+    if (AHEAD) ask_q((long long)h0 * a.group);
+    f32x2 cs[ROWS][4] = {}, sn[ROWS][4] = {};
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+        if (rope && row[r]) {
+            const long long pa = a.pos[((long long)b * a.T + t0 + r * (PAGE / ROWS)) * 2 + (d >> 5)];
+            const int p = (int)(pa < 0 ? 0 : (pa >= a.rope_len ? a.rope_len - 1 : pa));
+            Raw<T> rc, rs;
+            rc.load(reinterpret_cast<const T *>(a.cos) + (size_t)p * 32 + (d & 31));
+            rs.load(reinterpret_cast<const T *>(a.sin) + (size_t)p * 32 + (d & 31));
+            rc.get(cs[r]);
+            rs.get(sn[r]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) sn[r][i] ^= 0x8000000080000000ull;
+        }
     // the page this CTA writes, if any token falls into it
     const long long at = (long long)(len / PAGE) + blockIdx.y;
     const bool any = (int)blockIdx.y * PAGE < fill + n_new && n_new > 0;
@@ -237,18 +282,32 @@ __global__ void __launch_bounds__(APP_NT, sizeof(T) == 2 ? 2 : 1) append_kernel(
     const bool held = blockIdx.y == 0 && fill > 0;
 
     for (int h = h0; h < h1; ++h) {
-        f32x2 xk[4], xv[4];
-        rk.get(xk);
-        const Raw<T> v_now = rv;  // as loaded: half the registers
-        if (h + 1 < h1) ask_kv(h + 1);
-        norm_rotate(xk, d, a.eps, a.kw, a.kb, rope, cs, sn);
-        uint32_t (*r)[APP_NT / 32] = red[h & 1];  // the other one may still be read
-        const uint32_t mk = __reduce_max_sync(0xffffffffu, fresh ? amax_bits(xk) : 0u);
-        v_now.get(xv);
-        const uint32_t mv = __reduce_max_sync(0xffffffffu, fresh ? amax_bits(xv) : 0u);
+        f32x2 x[ROWS][4];
+        Raw<T> v_now[ROWS];  // as loaded: half the registers
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            rk[r].get(x[r]);
+            v_now[r] = rv[r];
+        }
+        if (h + 1 < h1) {
+            ask_k(h + 1);
+            if (AHEAD) ask_v(h + 1);
+        }
+        norm_rotate(x, d, a.eps, a.kw, a.kb, rope, cs, sn);
+        uint32_t (*red_h)[WARPS] = red[h & 1];  // the other one may still be read
+        uint32_t mk = 0, mv = 0;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            f32x2 xv[4];
+            v_now[r].get(xv);
+            mk = max(mk, fresh[r] ? amax_bits(x[r]) : 0u);
+            mv = max(mv, fresh[r] ? amax_bits(xv) : 0u);
+        }
+        mk = __reduce_max_sync(0xffffffffu, mk);
+        mv = __reduce_max_sync(0xffffffffu, mv);
         if (lane == 0) {
-            r[0][warp] = mk;
-            r[1][warp] = mv;
+            red_h[0][warp] = mk;
+            red_h[1][warp] = mv;
         }
         // the scales of a page that holds tokens already, read before anyone writes them
         int old_k = 0, old_v = 0;
@@ -258,32 +317,40 @@ __global__ void __launch_bounds__(APP_NT, sizeof(T) == 2 ? 2 : 1) append_kernel(
         }
         __syncthreads();
         if (ok) {
-            const int uk = max(scale_code(__reduce_max_sync(0xffffffffu, r[0][lane & 15])), old_k);
-            const int uv = max(scale_code(__reduce_max_sync(0xffffffffu, r[1][lane & 15])), old_v);
+            const int uk = max(scale_code(__reduce_max_sync(0xffffffffu, red_h[0][lane % WARPS])), old_k);
+            const int uv = max(scale_code(__reduce_max_sync(0xffffffffu, red_h[1][lane % WARPS])), old_v);
             uint8_t *pk = a.K.codes + page * a.K.page_stride + h * a.K.head_stride + slot * HD + d;
             uint8_t *pv = a.V.codes + page * a.V.page_stride + h * a.V.head_stride + slot * HD + d;
-            if (fresh) {
-                store_codes(pk, xk, scale_inverse(uk));
-                v_now.get(xv);
-                store_codes(pv, xv, scale_inverse(uv));
-            } else if (held && slot < fill) {
-                if (uk != old_k) move_codes(pk, scale_value(old_k) * scale_inverse(uk));
-                if (uv != old_v) move_codes(pv, scale_value(old_v) * scale_inverse(uv));
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r, pk += PAGE / ROWS * HD, pv += PAGE / ROWS * HD) {
+                if (fresh[r]) {
+                    f32x2 xv[4];
+                    store_codes(pk, x[r], scale_inverse(uk));
+                    v_now[r].get(xv);
+                    store_codes(pv, xv, scale_inverse(uv));
+                } else if (held && slot + r * (PAGE / ROWS) < fill) {
+                    if (uk != old_k) move_codes(pk, scale_value(old_k) * scale_inverse(uk));
+                    if (uv != old_v) move_codes(pv, scale_value(old_v) * scale_inverse(uv));
+                }
             }
             if (threadIdx.x == 0) {
                 a.K.scale[page * a.K.scale_stride + h] = (uint8_t)uk;
                 a.V.scale[page * a.V.scale_stride + h] = (uint8_t)uv;
             }
         }
+        if (!AHEAD && h + 1 < h1) ask_v(h + 1);
         if (!has_q) continue;
-        T *qo = reinterpret_cast<T *>(a.q_out) + (((long long)b * a.T + t) * heads + h) * a.group * HD + d;
-        for (int g = 0; g < a.group; ++g) {
-            f32x2 xq[4];
-            if (g > 0 && row) rq.load(qp + ((long long)h * a.group + g) * a.q_sh);
-            rq.get(xq);
-            if (g + 1 == a.group && h + 1 < h1) ask_q(h + 1);
-            norm_rotate(xq, d, a.eps, a.qw, a.qb, rope, cs, sn);
-            if (row) put(qo + (long long)g * HD, xq);
+        const long long q_row = (long long)heads * a.group * HD;
+        T *qo = reinterpret_cast<T *>(a.q_out) + ((long long)b * a.T + t0) * q_row + (long long)h * a.group * HD + d;
+        for (int g = 0; g < a.group; ++g, qo += HD) {
+            if (!AHEAD || g > 0) ask_q((long long)h * a.group + g);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) rq[r].get(x[r]);
+            if (AHEAD && g + 1 == a.group && h + 1 < h1) ask_q((long long)(h + 1) * a.group);
+            norm_rotate(x, d, a.eps, a.qw, a.qb, rope, cs, sn);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+                if (row[r]) put(qo + r * (PAGE / ROWS) * q_row, x[r]);
         }
     }
 }
@@ -333,11 +400,23 @@ extern "C" int ress_cache_append(const ress_cache *cache, const ress_append_args
     a.K = {cache->k_pages, cache->k_scale, cache->page_stride, cache->head_stride, cache->scale_stride};
     a.V = {cache->v_pages, cache->v_scale, cache->page_stride, cache->head_stride, cache->scale_stride};
     a.status = status;
-    // heads a CTA takes in turn: one while the CTAs fit on the GPU at once
-    // (two per SM), up to four beyond that, where it hides a head's loads
-    const int64_t ctas = cache->heads * pages * cache->streams;
+    // Heads a CTA takes in turn (a head's loads are hidden behind the head
+    // before): the count whose waves of two CTAs per SM take least, where a q row
+    // costs about a third of a head's k and v and a CTA's start nearly as much as
+    // they do.  Measured, us at 1, 2, 4, 8 heads: 43,968 tokens of 16 heads 146,
+    // 119, 110, 107; 10,992 44, 38, 37, 41; 64 streams of one token 13.4, 11.9,
+    // 11.9, 11.9; 8 streams of 1374, 16 q heads on 4 20.4, 22.6, 23.6.
+    const int64_t ctas = cache->heads * ((g.tokens + cache::PAGE - 1) / cache::PAGE) * cache->streams;
+    const int64_t head = 20 + 10 * (int64_t)a.group, start = 27;
     int per = 1;
-    while (per < 4 && ctas / (2 * per) >= 2 * 148) per *= 2;
+    int64_t least = INT64_MAX;
+    for (int p = 1; p <= 8 && p < 2 * cache->heads; p *= 2) {
+        const int64_t cost = ((ctas + p - 1) / p + 2 * 148 - 1) / (2 * 148) * (head * p + start);
+        if (cost < least) {
+            least = cost;
+            per = p;
+        }
+    }
     const int heads = (int)cache->heads;
     const dim3 grid((unsigned)((heads + per - 1) / per), (unsigned)pages, (unsigned)cache->streams);
     if (g.dtype == RESS_BF16)
