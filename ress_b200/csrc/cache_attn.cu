@@ -74,6 +74,7 @@ __device__ __forceinline__ void send4(uint32_t a, const float4 &v) {
                  : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // One query row of the tile in registers: 16 head dims of lane t's, as fp16
@@ -160,7 +161,8 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
         for (int e = 0; e < 2; ++e)
             if (a.limits == nullptr || lim[n][e] < 0) lim[n][e] = hi;  // rows past the last: computed, never written
     __syncthreads();
-    if (splits > 1) cluster_arrive();  // waited for before the first store into a peer
+    // they have started; waited for before the first store into a peer
+    if (splits > 1) cluster_arrive_relaxed();
     if (threadIdx.x == 0 && split == 0 && bad_len(a, b)) atomicOr(a.status, RESS_STATUS_CACHE_RANGE);
 
     // this warp's pages: first, first + FEW_WARPS, ... (count of them)
