@@ -376,7 +376,7 @@ typedef struct {
  *   b*sb + t*st + head*sh (elements; rows 16-byte aligned), RESS_F32 or
  *   RESS_BF16; k and v have the cache's heads, q a multiple of them.
  *   q and k: LayerNorm over the head dims where weight and bias are given
- *   (fp32; NULL: none), then the 2-D rotary embedding as in
+ *   (fp32, 64 values, 16-byte aligned; NULL: none), then the 2-D rotary embedding as in
  *   ress_qkv_prologue when rope_cos is given (tables (rope_len, 32) in the
  *   input's type, pos (streams, tokens, 2) int64), all in fp32 without
  *   intermediate rounding.  q_out (streams, tokens, q_heads, 64) contiguous in

@@ -27,11 +27,14 @@
 // takes about 1700.  The rest are the waits, loads and stores of one tile,
 // which queue behind the other's exponentials, and the supply of instructions:
 // what is rare is out of line, and the loop over pages is kept short.
-// (Measured for 5,496 queries x 43,968 tokens x 16 heads: 1684 us so; 1782
-// with the masked path in the loop; 1860 with the scores read again in pieces
-// of 16; 1835 with steps of 128 keys; 2070 with the next page's scores loaded
-// ahead; 1655 with sixteen softmax warps, two threads a row, and P in shared
-// memory, at 1850 cycles a page but fewer pages per CTA.)
+// 5,496 queries x 43,968 tokens x 16 heads, each frame seeing those up to its
+// own: 1645 us, 570 TFLOP/s of the products that no mask hides; 1374 x 10,992:
+// 155 us, 400 (a CTA's start and join weigh more).
+// (Measured on the first at one and the same split: 1684 us so; 1782 with the
+// masked path in the loop; 1860 with the scores read again in pieces of 16;
+// 1835 with steps of 128 keys; 2070 with the next page's scores loaded ahead;
+// 1845 with the two tiles' exponentials taking turns; a polynomial for a part
+// of the exponentials gained nothing.)
 // P is rounded to bf16 for the MMA, numerator and denominator alike;
 // everything else is fp32.
 // When the tiles are too few for the GPU the pages are split over several

@@ -86,8 +86,8 @@ __device__ __forceinline__ uint32_t amax8(const float (&x)[8]) {
 // smooth function, here its polynomial of degree 7 on [-6.5, 0] (fitted so that
 // Phi's largest error is least: 1.1e-7; below, Phi < 5e-11): one exponential and
 // no reciprocal, and packed arithmetic, where the instructions issued bound the
-// epilogue (10,992 x 1024 -> 4096: a rational form of erfc 58 us, this polynomial
-// 54, packed 49).
+// epilogue (43,968 x 1024 -> 4096 with the quantiser: 196 us; 215 without the
+// packing, and 11 more with a rational form of erfc).
 __device__ __forceinline__ f32x2 twice(float x) { return f2_pack(x, x); }
 __device__ __forceinline__ f32x2 gelu(f32x2 yy) {
     float y0, y1, p0, p1;
@@ -115,7 +115,11 @@ __device__ __forceinline__ f32x2 scaled(int acc0, int acc1, f32x2 s_row, f32x2 s
 
 // Rows to int8 with one scale each: one warp per row, eight values a lane at
 // a time.  CH > 0: the row (at most 256 * CH values) stays in registers
-// between its maximum and its codes; CH = 0: it is read again.
+// between its maximum and its codes; CH = 0: it is read again.  Bound by HBM
+// where the rows are many: 43,968 x 4096 in bf16, 540 MB, 84 us, as fast as a
+// copy.  (Quantising inside the product, by four more warps that feed its
+// operand, was 371 us against 212 for both kernels: every tile of channels
+// quantises its rows again.)
 constexpr int QUANT_NT = 256;
 template <typename T> struct Piece;  // eight values as loaded
 template <> struct Piece<__nv_bfloat16> {
@@ -209,7 +213,9 @@ __global__ void __launch_bounds__(QUANT_NT) quant_rows_kernel(const T *__restric
 // row serves two k-steps.  The first weights are asked for before anything
 // else; meanwhile every CTA quantises the tokens into shared memory (they
 // are few, and no second launch is needed).  The warps' int32 sums are
-// exact, so their order does not matter.
+// exact, so their order does not matter.  1 x 1024 -> 4096: 5.2 us from launch
+// to launch, of which its 4 MB of weights take 0.65; the rest are the launch
+// and two memory latencies.
 constexpr int FEW_NT = 256, FEW_WARPS = 8, FEW_M = 16, FEW_N = 16, FEW_AHEAD = 4;
 template <typename T, typename O>
 __global__ void __launch_bounds__(FEW_NT) few_kernel(const T *__restrict__ x, long long x_st, const LinArgs a) {
@@ -329,6 +335,11 @@ static int launch_few(const void *x, long long x_st, const LinArgs &a, cudaStrea
 //              scales, bias, GELU, one rounding, shared memory, TMA store,
 //              while the next tile is accumulated into the other buffer; two
 //              warps share a quarter of the rows and take its columns in turn.
+// With long K the tensor cores are the bound: 43,968 x 4096 -> 1024 takes 125
+// us after the quantiser, 2.95 POP/s.  With K = 1024 a tile's operands from L2
+// (256 KB at the 40 to 45 bytes a cycle and SM that all SMs reach together) take
+// 6,000 cycles and its MMAs 4,100: 1024 -> 1024 41 us, 2.25 POP/s; with GELU the
+// epilogue's 7,000 instructions' cycles are near: 1024 -> 4096 173 us, 2.1 POP/s.
 using namespace tc;
 
 template <int CG, int BN, typename O> struct Tile {
