@@ -117,9 +117,11 @@ __device__ __forceinline__ f32x2 scaled(int acc0, int acc1, f32x2 s_row, f32x2 s
 // a time.  CH > 0: the row (at most 256 * CH values) stays in registers
 // between its maximum and its codes; CH = 0: it is read again.  Bound by HBM
 // where the rows are many: 43,968 x 4096 in bf16, 540 MB, 84 us, as fast as a
-// copy.  (Quantising inside the product, by four more warps that feed its
-// operand, was 371 us against 212 for both kernels: every tile of channels
-// quantises its rows again.)
+// copy.  (Quantising inside the product's kernel is slower than both kernels,
+// 208 us: by four more warps that feed its operand 371, since every tile of
+// channels quantises its rows again; by four more warps that take each row once
+// and count it for the tiles that wait 308, since four warps an SM keep too few
+// loads in flight.)
 constexpr int QUANT_NT = 256;
 template <typename T> struct Piece;  // eight values as loaded
 template <> struct Piece<__nv_bfloat16> {
