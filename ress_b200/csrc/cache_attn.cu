@@ -1,5 +1,7 @@
 // cache_attn.cu -- attention of a few queries over the paged 8-bit cache, and
 // the C entry for any number (cache_attn.cuh has the definition).
+#include <type_traits>
+
 #include "cache_attn.cuh"
 
 namespace ress {
@@ -35,10 +37,10 @@ using namespace tc;
 // Each CTA sends its rows' partial results to the shared memory of the row's
 // owner, which joins them in CTA order: one launch, no workspace.  Up to 32
 // streams are started longest first, so that the last CTAs are short.
-// 16 streams of 11 to 44 thousand tokens, 24 heads on 8: 86 to 90 us, 5.2 TB/s
-// of the 6.45 that a copy reaches.  One token, 16 heads, 10,992 tokens: 12.3 us
-// for 22.5 MB: a launch, and three pages in turn on each warp, which is bound by
-// the latency of its about 940 instructions a page.
+// 16 streams of 11 to 44 thousand tokens, 24 heads on 8: 86 us, 5.2 TB/s of the
+// 6.45 that a copy reaches.  One token, 16 heads, 10,992 tokens: 11.2 us for 22.5
+// MB: a launch, and three pages in turn on each warp, which is bound by the
+// latency of its about 850 instructions a page.
 constexpr int FEW_ROWS = 16, FEW_WARPS = 8, FEW_RING = 3, FEW_SPLITS = 16;
 constexpr int FEW_NT = FEW_WARPS * 32;
 constexpr int FEW_SMEM = FEW_WARPS * FEW_RING * BLOCK_BYTES;
@@ -279,7 +281,6 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
         }
         done();
         const int base = (first + i * FEW_WARPS) * PAGE;
-        const bool whole = base + PAGE <= lo;
         const float fk = scale_value(uk);
         // a page of larger V scale moves O's unit
         float fv = scale_value(uv), move = 1.0f;  // NaN stays NaN
@@ -290,90 +291,96 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
             }
             fv = scale_value(max(127 + P_SHIFT + uv - uref, 0));
         }
-        uint32_t pb[NT][4][2];
+        // where every row sees the whole page there are no masks (a tenth of the instructions)
+        auto page = [&](auto page_whole) {
+            constexpr bool whole = decltype(page_whole)::value;
+            uint32_t pb[NT][4][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float bias[2], cs[2], alpha[2];
+            for (int n = 0; n < NT; ++n) {
+                float bias[2], cs[2], alpha[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float top = -INFINITY;
+                for (int e = 0; e < 2; ++e) {
+                    float top = -INFINITY;
 #pragma unroll
-                for (int mt = 0; mt < 4; ++mt) {
-                    if (!whole) {  // hidden tokens: -inf, whatever lies there
-                        if (base + mt * 16 + pg >= lim[n][e]) c[mt][n][e] = -INFINITY;
-                        if (base + mt * 16 + 8 + pg >= lim[n][e]) c[mt][n][e + 2] = -INFINITY;
+                    for (int mt = 0; mt < 4; ++mt) {
+                        if (!whole) {  // hidden tokens: -inf, whatever lies there
+                            if (base + mt * 16 + pg >= lim[n][e]) c[mt][n][e] = -INFINITY;
+                            if (base + mt * 16 + 8 + pg >= lim[n][e]) c[mt][n][e + 2] = -INFINITY;
+                        }
+                        top = fmaxf(top, fmaxf(c[mt][n][e], c[mt][n][e + 2]));
                     }
-                    top = fmaxf(top, fmaxf(c[mt][n][e], c[mt][n][e + 2]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    cs[e] = rf[n][e] * fk;  // not negative; a NaN one shows in the exponentials
+                    const float mn = fmaxf(m[n][e], top == -INFINITY ? top : top * cs[e]);
+                    const float mb = mn == -INFINITY ? 0.0f : mn;
+                    alpha[e] = ex2(m[n][e] - mb);
+                    l[n][e] *= alpha[e];
+                    alpha[e] *= move;
+                    m[n][e] = mn;
+                    bias[e] = -mb;
                 }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                cs[e] = rf[n][e] * fk;  // not negative; a NaN one shows in the exponentials
-                const float mn = fmaxf(m[n][e], top == -INFINITY ? top : top * cs[e]);
-                const float mb = mn == -INFINITY ? 0.0f : mn;
-                alpha[e] = ex2(m[n][e] - mb);
-                l[n][e] *= alpha[e];
-                alpha[e] *= move;
-                m[n][e] = mn;
-                bias[e] = -mb;
-            }
-            if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+                if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    o[n][d][0] *= alpha[0];
-                    o[n][d][1] *= alpha[1];
-                    o[n][d][2] *= alpha[0];
-                    o[n][d][3] *= alpha[1];
-                }
-            }
-            // P: probabilities for the sums, and times the V scale as fp16 fragments
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float p[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        p[e] = ex2(fmaf(c[mt][n][2 * k + e], cs[e], bias[e]));
-                        // a hidden token is 0 even where a factor is 0 or NaN
-                        const bool hidden = !whole && base + mt * 16 + 8 * k + pg >= lim[n][e];
-                        if (hidden) p[e] = 0.0f;
-                        l[n][e] += p[e];
-                        p[e] *= fv;
-                        if (hidden) p[e] = 0.0f;
+                    for (int d = 0; d < 4; ++d) {
+                        o[n][d][0] *= alpha[0];
+                        o[n][d][1] *= alpha[1];
+                        o[n][d][2] *= alpha[0];
+                        o[n][d][3] *= alpha[1];
                     }
-                    pb[n][mt][k] = transpose8x8(half2_bits(p[0], p[1]));
                 }
-        }
-        const unsigned char *sv = take();
-        if (sv == nullptr) break;
+                // P: probabilities for the sums, and times the V scale as fp16 fragments
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-            const unsigned char *va = sv + mt * 16 * HD + g * 8;
-            uint2 v0 = *reinterpret_cast<const uint2 *>(va + kf * HD), v1 = *reinterpret_cast<const uint2 *>(va + kh * HD);
-            uint2 v2 = *reinterpret_cast<const uint2 *>(va + (8 + kf) * HD);
-            uint2 v3 = *reinterpret_cast<const uint2 *>(va + (8 + kh) * HD);
-            if (base + PAGE > len) {  // slots past the stream's end hold anything, NaN codes too
-                const int e = len - base - 16 * mt;
-                if (kf >= e) v0 = make_uint2(0, 0);
-                if (kh >= e) v1 = make_uint2(0, 0);
-                if (8 + kf >= e) v2 = make_uint2(0, 0);
-                if (8 + kh >= e) v3 = make_uint2(0, 0);
+                for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float p[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            p[e] = ex2(fmaf(c[mt][n][2 * k + e], cs[e], bias[e]));
+                            // a hidden token is 0 even where a factor is 0 or NaN
+                            const bool hidden = !whole && base + mt * 16 + 8 * k + pg >= lim[n][e];
+                            if (hidden) p[e] = 0.0f;
+                            l[n][e] += p[e];
+                            p[e] *= fv;
+                            if (hidden) p[e] = 0.0f;
+                        }
+                        pb[n][mt][k] = transpose8x8(half2_bits(p[0], p[1]));
+                    }
             }
+            const unsigned char *sv = take();
+            if (sv == nullptr) return false;
 #pragma unroll
-            for (int d = 0; d < 4; d += 2) {  // dims 8g + d, and + 4 in the lower half of the rows
-                const uint32_t sel = d == 0 ? 0x5140u : 0x7362u;
-                const uint32_t y0 = __byte_perm(v0.x, v1.x, sel), y1 = __byte_perm(v0.y, v1.y, sel);
-                const uint32_t y2 = __byte_perm(v2.x, v3.x, sel), y3 = __byte_perm(v2.y, v3.y, sel);
+            for (int mt = 0; mt < 4; ++mt) {
+                const unsigned char *va = sv + mt * 16 * HD + g * 8;
+                uint2 v0 = *reinterpret_cast<const uint2 *>(va + kf * HD), v1 = *reinterpret_cast<const uint2 *>(va + kh * HD);
+                uint2 v2 = *reinterpret_cast<const uint2 *>(va + (8 + kf) * HD);
+                uint2 v3 = *reinterpret_cast<const uint2 *>(va + (8 + kh) * HD);
+                if (!whole && base + PAGE > len) {  // slots past the stream's end hold anything, NaN codes too
+                    const int e = len - base - 16 * mt;
+                    if (kf >= e) v0 = make_uint2(0, 0);
+                    if (kh >= e) v1 = make_uint2(0, 0);
+                    if (8 + kf >= e) v2 = make_uint2(0, 0);
+                    if (8 + kh >= e) v3 = make_uint2(0, 0);
+                }
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t a0 = e4m3_to_half2((uint16_t)(y0 >> (16 * k))), a1 = e4m3_to_half2((uint16_t)(y1 >> (16 * k)));
-                    const uint32_t a2 = e4m3_to_half2((uint16_t)(y2 >> (16 * k))), a3 = e4m3_to_half2((uint16_t)(y3 >> (16 * k)));
+                for (int d = 0; d < 4; d += 2) {  // dims 8g + d, and + 4 in the lower half of the rows
+                    const uint32_t sel = d == 0 ? 0x5140u : 0x7362u;
+                    const uint32_t y0 = __byte_perm(v0.x, v1.x, sel), y1 = __byte_perm(v0.y, v1.y, sel);
+                    const uint32_t y2 = __byte_perm(v2.x, v3.x, sel), y3 = __byte_perm(v2.y, v3.y, sel);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_16816(o[n][d + k], a0, a1, a2, a3, pb[n][mt][0], pb[n][mt][1]);
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t a0 = e4m3_to_half2((uint16_t)(y0 >> (16 * k))), a1 = e4m3_to_half2((uint16_t)(y1 >> (16 * k)));
+                        const uint32_t a2 = e4m3_to_half2((uint16_t)(y2 >> (16 * k))), a3 = e4m3_to_half2((uint16_t)(y3 >> (16 * k)));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16816(o[n][d + k], a0, a1, a2, a3, pb[n][mt][0], pb[n][mt][1]);
+                    }
                 }
             }
-        }
+            return true;
+        };
+        if (!(base + PAGE <= lo ? page(std::true_type{}) : page(std::false_type{}))) break;
         done();
     }
     // copies in flight land before their ring is used again (all have, unless a wait ran out)
