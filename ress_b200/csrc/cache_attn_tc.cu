@@ -320,9 +320,10 @@ __global__ void __launch_bounds__(NT, 1)
     if (tid < TILES * TILE) {
         const int l = row_limit(a, b, len, r0 + tid);
         B.lim[tid] = l;
-        if (l >= 0) {
-            atomicMax(&B.hi, l);
-            atomicMin(&B.lo[tid / TILE], l);
+        const int most = __reduce_max_sync(0xffffffffu, l), least = __reduce_min_sync(0xffffffffu, l >= 0 ? l : INT_MAX);
+        if (tid % 32 == 0) {
+            atomicMax(&B.hi, most);
+            atomicMin(&B.lo[tid / TILE], least);
         }
     } else {
         // q of one row a thread: scaled by a power of two to [128, 256), split into two e4m3 parts
@@ -671,13 +672,14 @@ __global__ void __launch_bounds__(NT, 1)
                 if (in) store_row(a, at, o, l == 0.0f ? 0.0f : 1.0f / l);
             } else {
                 const long long group = ((long long)b * gridDim.y + h) * row_ctas * TILES + cta * TILES + tile;
-                float *slot = a.partial + (group * splits * TILE + r) * PART_ROW;  // this row of piece 0
-                float *mine = slot + (long long)split * TILE * PART_ROW;
+                // a piece: 17 times 128 rows' four floats (O, then maximum and sum), so that
+                // a warp's accesses are contiguous
+                constexpr int PIECE = TILE * PART_ROW / 4;
+                float4 *slot = reinterpret_cast<float4 *>(a.partial) + group * splits * PIECE + r;  // of piece 0
+                float4 *mine = slot + split * PIECE;
 #pragma unroll
-                for (int i = 0; i < HD; i += 4)
-                    *reinterpret_cast<float4 *>(mine + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                mine[HD] = m;
-                mine[HD + 1] = l;
+                for (int i = 0; i < HD; i += 4) mine[i / 4 * TILE] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                mine[HD / 4 * TILE] = make_float4(m, l, 0.0f, 0.0f);
                 __threadfence();
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + tile) : "memory");
                 if (r == 0) B.join[tile] = atomicAdd(&a.arrived[group], 1) == splits - 1;
@@ -685,18 +687,18 @@ __global__ void __launch_bounds__(NT, 1)
                 if (B.join[tile] && in) {
                     __threadfence();
                     float mm = -INFINITY;
-                    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, __ldcg(slot + (long long)s * TILE * PART_ROW + HD));
+                    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, __ldcg(slot + s * PIECE + HD / 4 * TILE).x);
                     const float mb = mm == -INFINITY ? 0.0f : mm;
                     float sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < HD; ++i) o[i] = 0.0f;
                     for (int s = 0; s < splits; ++s) {
-                        const float *p = slot + (long long)s * TILE * PART_ROW;
-                        const float f = ex2(__ldcg(p + HD) - mb);
-                        sum = fmaf(__ldcg(p + HD + 1), f, sum);
+                        const float4 *p = slot + s * PIECE, ml = __ldcg(p + HD / 4 * TILE);
+                        const float f = ex2(ml.x - mb);
+                        sum = fmaf(ml.y, f, sum);
 #pragma unroll
                         for (int i = 0; i < HD; i += 4) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + i));
+                            const float4 v = __ldcg(p + i / 4 * TILE);
                             o[i] = fmaf(v.x, f, o[i]);
                             o[i + 1] = fmaf(v.y, f, o[i + 1]);
                             o[i + 2] = fmaf(v.z, f, o[i + 2]);
