@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(QUANT_NT) quant_rows_kernel(const T *__restric
 // row serves two k-steps.  The first weights are asked for before anything
 // else; meanwhile every CTA quantises the tokens into shared memory (they
 // are few, and no second launch is needed).  The warps' int32 sums are
-// exact, so their order does not matter.  1 x 1024 -> 4096: 5.2 us from launch
+// exact, so their order does not matter.  1 x 1024 -> 4096: 3.4 us from launch
 // to launch, of which its 4 MB of weights take 0.65; the rest are the launch
 // and two memory latencies.
 constexpr int FEW_NT = 256, FEW_WARPS = 8, FEW_M = 16, FEW_N = 16, FEW_AHEAD = 4;
@@ -242,15 +242,11 @@ __global__ void __launch_bounds__(FEW_NT) few_kernel(const T *__restrict__ x, lo
         b0[i] = weight(w0, s0 + i);
         b1[i] = weight(w1, s0 + i);
     }
-    // `per` warps share a token
+    // `per` warps share a token; rows without one hold anything: their products
+    // stay in their own rows, which are not written
     const int per = a.M >= 8 ? 1 : a.M >= 4 ? 2 : a.M >= 2 ? 4 : 8, sub = warp % per;
-    for (int r0 = 0; r0 < FEW_M; r0 += FEW_WARPS / per) {
+    for (int r0 = 0; r0 < a.M; r0 += FEW_WARPS / per) {
         const int r = r0 + warp / per;
-        if (r0 >= a.M) {  // rows without a token
-            for (int k = sub * 256 + lane * 8; k < Kp; k += 256 * per)
-                *reinterpret_cast<uint2 *>(xs + r * pitch + k) = make_uint2(0, 0);
-            continue;
-        }
         const T *row = x + (long long)min(r, a.M - 1) * x_st;
         uint32_t am = 0;
         Piece<T> p;
@@ -424,6 +420,17 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
         "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
           "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr));
 }
 
@@ -676,6 +683,170 @@ __global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CU
     }
 }
 
+// Few tiles: a cluster of S CTAs takes one tile of 128 tokens x 64 channels, each
+// a part of K (one SM's copies, at 40 bytes a cycle, bound a tile otherwise).
+// Every CTA owns 64 / S of the channels: the others send it their int32 sums of
+// those, which are exact, so their order does not matter.
+constexpr int SPLIT_NT = 256;
+template <int S> struct SplitTile {
+    static constexpr int BN = 64, OWN = BN / S, STAGE = (128 + BN) * 128, NS = 6;
+    static constexpr int OFF_IN = NS * STAGE;  // sums from every CTA: S x OWN / 4 x 128 rows of four
+    static constexpr int SMEM = OFF_IN + 128 * BN * 4 + 1024;
+    static constexpr uint32_t IDESC =
+        (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((128u >> 4) << 24);
+};
+template <int S, typename O>
+__global__ void __launch_bounds__(SPLIT_NT, 1) split_kernel(const __grid_constant__ CUtensorMap tm_x,
+                                                            const __grid_constant__ CUtensorMap tm_w, const LinArgs a,
+                                                            const float *__restrict__ sx, int wide_out, int32_t *status) {
+    using C = SplitTile<S>;
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full[C::NS], empty[C::NS], acc_full;
+    __shared__ uint32_t tmem_s;
+    __shared__ int abort_s;
+    unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t ring = smem_u32(smem), inbox = ring + C::OFF_IN;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
+    volatile int *abort_flag = &abort_s;
+    const int m0 = blockIdx.z * 128, n0 = blockIdx.y * C::BN;
+    const int nk = (a.K + 127) / 128, k0 = nk * rank / S, k1 = nk * (rank + 1) / S;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::NS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(&acc_full, 1);
+        abort_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(64)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // started: waited for before the sums are sent
+    const uint32_t tmem = tmem_s;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the tokens' codes and scales are there
+    if (warp == 0 && lane == 0) {
+        for (int k = k0, it = 0; k < k1; ++k, ++it) {
+            const int st = it % C::NS;
+            if (it >= C::NS && !wait_bar(&empty[st], (it / C::NS - 1) & 1, abort_flag, status)) break;
+            mbar_expect_tx(&full[st], C::STAGE);
+            tma_load_2d<1>(ring + st * C::STAGE, &tm_x, smem_u32(&full[st]), k * 128, m0);
+            tma_load_2d<1>(ring + st * C::STAGE + 128 * 128, &tm_w, smem_u32(&full[st]), k * 128, n0);
+        }
+    } else if (warp == 1 && lane == 0) {
+        bool ok = true;
+        for (int k = k0, it = 0; k < k1; ++k, ++it) {
+            const int st = it % C::NS;
+            ok = wait_bar(&full[st], (it / C::NS) & 1, abort_flag, status);
+            if (!ok) break;
+            fence_after();
+            const uint32_t sa = ring + st * C::STAGE, sb = sa + 128 * 128;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+                mma_int8<1>(tmem, make_desc(sa + kk * 32, 16, 1024, LAYOUT_SW128), make_desc(sb + kk * 32, 16, 1024, LAYOUT_SW128),
+                            C::IDESC, (it | kk) ? 1u : 0u);
+            commit<1>(&empty[st]);
+        }
+        if (ok) commit<1>(&acc_full);
+    }
+    __syncwarp();
+    // a warp's 32 rows, and of the 64 channels the first or last 32
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const bool ok = wait_bar_warp(&acc_full, 0, abort_flag, status);
+    fence_after();
+    uint32_t v[32];
+    if (ok) {
+        tmem_ld32(tmem + half * 32 + ((uint32_t)((warp & 3) * 32) << 16), v);
+        tmem_wait_ld();
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (ok && m0 + row < a.M) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            const int col = half * 32 + i, own = col / C::OWN;
+            const uint32_t to = inbox + ((rank * C::OWN + col % C::OWN) / 4 * 128 + row) * 16;
+            uint32_t at;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(to), "r"(own));
+            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]),
+                         "r"(v[i + 3])
+                         : "memory");
+        }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    // meanwhile: the scales of this thread's row and channels
+    constexpr int PER = C::OWN / 2;  // channels of a thread, two threads a row
+    const int r = threadIdx.x & 127, c0 = (threadIdx.x >> 7) * PER, n = n0 + rank * C::OWN + c0;
+    const bool in = m0 + r < a.M;
+    const float s_row = in ? sx[m0 + r] : 0.0f;
+    float w[PER], b[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        w[i] = n + i < a.N ? __ldg(a.w_scale + n + i) : 0.0f;
+        b[i] = n + i < a.N && a.bias != nullptr ? __ldg(a.bias + n + i) : 0.0f;
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (in) {
+        int acc[PER] = {};
+        const int4 *sums = reinterpret_cast<const int4 *>(smem + C::OFF_IN) + c0 / 4 * 128 + r;
+#pragma unroll
+        for (int p = 0; p < S; ++p)
+#pragma unroll
+            for (int i = 0; i < PER; i += 4) {
+                const int4 u = sums[(p * C::OWN + i) / 4 * 128];
+                acc[i] += u.x;
+                acc[i + 1] += u.y;
+                acc[i + 2] += u.z;
+                acc[i + 3] += u.w;
+            }
+        O *const out = reinterpret_cast<O *>(a.out) + (size_t)(m0 + r) * a.out_st + n;
+        float y[PER];
+#pragma unroll
+        for (int i = 0; i < PER; i += 2) {
+            f32x2 yy = scaled(acc[i], acc[i + 1], twice(s_row), f2_pack(w[i], w[i + 1]), f2_pack(b[i], b[i + 1]));
+            if (a.gelu) yy = gelu(yy);
+            f2_unpack(yy, y[i], y[i + 1]);
+        }
+        if (wide_out && n + PER <= a.N) {
+#pragma unroll
+            for (int i = 0; i < PER; i += 16 / (int)sizeof(O)) {
+                if constexpr (sizeof(O) == 2) {
+                    uint32_t u[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(y[i + 2 * k], y[i + 2 * k + 1]);
+                        u[k] = *reinterpret_cast<const uint32_t *>(&h);
+                    }
+                    *reinterpret_cast<uint4 *>(out + i) = make_uint4(u[0], u[1], u[2], u[3]);
+                } else {
+                    *reinterpret_cast<float4 *>(out + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (n + i < a.N) DT<O>::store(out, (size_t)i, y[i]);
+        }
+    }
+    // copies in flight have landed (all have been consumed, unless a wait ran out)
+    if (warp == 0 && lane == 0 && !ok)
+        for (int st = 0; st < min(k1 - k0, C::NS); ++st) {
+            const uint64_t t0 = globaltimer();
+            while (!mbar_try_wait_sleep(smem_u32(&full[st]), ((k1 - k0 - 1 - st) / C::NS) & 1) && globaltimer() - t0 < TIMEOUT_NS) {
+            }
+        }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(64) : "memory");
+}
+
 // Rows of `cols` elements, `stride` bytes apart, in boxes of 128 bytes x box_rows.
 static bool map_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem, long long cols, long long rows,
                    long long stride, int box_rows) {
@@ -722,6 +893,32 @@ static int launch_gemm(const int8_t *x8, const float *sx, const LinArgs &a, int3
     return cudaLaunchKernelEx(&cfg, kern, tx, tw, to, a, sx, tma_out, status) == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
 }
 
+template <int S, typename O>
+static int launch_split(const int8_t *x8, const float *sx, const LinArgs &a, int32_t *status, cudaStream_t s) {
+    using C = SplitTile<S>;
+    CUtensorMap tx, tw;
+    if (!map_2d(&tx, x8, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, a.K, 128) ||
+        !map_2d(&tw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.N, a.K, C::BN))
+        return RESS_E_NO_DEVICE;
+    auto kern = split_kernel<S, O>;
+    set_smem_attr((const void *)kern, C::SMEM);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S, (unsigned)((a.N + C::BN - 1) / C::BN), (unsigned)((a.M + 127) / 128));
+    cfg.blockDim = dim3(SPLIT_NT);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = S;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    const int wide_out = !((uintptr_t)a.out & 15) && !((a.out_st * (int)sizeof(O)) & 15);
+    return cudaLaunchKernelEx(&cfg, kern, tx, tw, a, sx, wide_out, status) == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
+}
+
 template <typename T>
 static int launch_quant(const T *x, long long x_st, int M, int K, int8_t *x8, float *scale, cudaStream_t s) {
     const unsigned blocks = (unsigned)(((long long)M * 32 + QUANT_NT - 1) / QUANT_NT);
@@ -734,11 +931,25 @@ static int launch_quant(const T *x, long long x_st, int M, int K, int8_t *x8, fl
     return cudaGetLastError() == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
 }
 
-// Rows up to which the weights' bytes bound the call and sixteen-row tiles do.
-constexpr int FEW_MAX_M = 16, FEW_MAX_K = 8192;
-static bool use_few(int M, int K) { return M <= FEW_MAX_M && K <= FEW_MAX_K; }
+// Tokens up to which every CTA quantises them all sooner than a second kernel
+// starts.  Measured, us against the tiles below, 1024 channels: 16 x 1024 4.9
+// against 5.5, 16 x 2048 6.4 against 6.7, 16 x 4096 15.5 against 9.2; 8 x 4096 9.5
+// against 9.2; 4 x 8192 11.2 against 14.6.
+static bool use_few(int M, int K) { return K <= 8192 && (M <= 4 || (M <= FEW_M && M * K <= 32 * 1024)); }
 static size_t workspace(int M, int K) {
     return use_few(M, K) ? 0 : ((size_t)M * K + 255) / 256 * 256 + (size_t)M * sizeof(float);
+}
+
+// CTAs that share a tile of 128 x 64: as many as leave every CTA an SM (a GPC's
+// SMs are not all multiples of four) and a slice of K.  Measured, us with one, two
+// and four (quantiser included): 64 x 1024 -> 1024: 7.6, 6.9, 5.9; 165 x 1536 ->
+// 1000: 9.7, 8.7, 7.3; 64 x 4096 -> 1024: 16.4, 12.2, 9.5; beyond an SM each: 100 x
+// 1024 -> 4096 in four 10.3 (two 7.3, one 7.8), 165 x 1024 -> 3000 in two 11.2
+// (one 8.1).
+static int pick_split(const LinArgs &a) {
+    const long long tiles = (long long)((a.M + 127) / 128) * ((a.N + 63) / 64);
+    const int nk = (a.K + 127) / 128;
+    return tiles * 4 <= 128 && nk >= 4 ? 4 : tiles * 2 <= 148 && nk >= 2 ? 2 : 1;
 }
 
 // The tile (of <pair, 256>, <single, 128>, <single, 64>) whose waves over the
@@ -781,6 +992,9 @@ static int linear(const void *x, long long x_st, const LinArgs &a, void *ws, int
     float *sx = reinterpret_cast<float *>(x8 + ((size_t)a.M * a.K + 255) / 256 * 256);
     const int rc = launch_quant((const T *)x, x_st, a.M, a.K, x8, sx, s);
     if (rc != RESS_OK) return rc;
+    const int split = pick_split(a);
+    if (split == 4) return launch_split<4, O>(x8, sx, a, status, s);
+    if (split == 2) return launch_split<2, O>(x8, sx, a, status, s);
     switch (pick_tile(a)) {
         case 0: return launch_gemm<2, 256, O>(x8, sx, a, status, s);
         case 1: return launch_gemm<1, 128, O>(x8, sx, a, status, s);
