@@ -137,6 +137,33 @@ def test_append_in_one_go_or_token_by_token():
         assert torch.equal(_u8(a[n]), _u8(b[n])), n
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,T,Hq,Hkv", [(40, 70, 16, 16), (64, 130, 12, 6), (3, 3000, 5, 5)])
+def test_append_many_pages_equals_stream_by_stream(B, T, Hq, Hkv, dtype):
+    """Calls large enough for a CTA to take several heads in turn store the same
+    bytes as one call per stream, whose CTAs take fewer."""
+    g = _gen(B + T)
+    lens = torch.randint(0, 90, (B,), device="cuda", dtype=torch.int32, generator=g)
+    width = -(-(90 + T) // PAGE)
+    table = shuffled_table(B, width, B * width, seed=T)
+    kw = dict(zip(("qn_weight", "qn_bias", "kn_weight", "kn_bias"), _affine(g) + _affine(g)))
+    cos, sin = _tables(40, dtype)
+    pos = torch.randint(0, 40, (B, T, 2), device="cuda", generator=g)
+    q, k, v = torch.randn(B, T, Hq + 2 * Hkv, HD, device="cuda", generator=g).to(dtype).split([Hq, Hkv, Hkv], 2)
+    one, each = make_cache(B * width, Hkv), make_cache(B * width, Hkv)
+    for n in one:
+        each[n].view(torch.uint8).copy_(one[n].view(torch.uint8))
+    rows = K.cache_append(k, v, **one, table=table, lens=lens, q=q, pos=pos, rope_cos=cos, rope_sin=sin, **kw)
+    for b in range(B):
+        s = slice(b, b + 1)
+        r = K.cache_append(k[s], v[s], **each, table=table[s], lens=lens[s], q=q[s], pos=pos[s], rope_cos=cos, rope_sin=sin,
+                           **kw)
+        assert torch.equal(r, rows[s])
+    assert K.check_status() == 0
+    for n in one:
+        assert torch.equal(_u8(one[n]), _u8(each[n])), n
+
+
 def test_append_ragged_and_idempotent():
     """Streams of unlike length and count (none among them); a repeated call changes nothing."""
     g = _gen(5)

@@ -57,6 +57,26 @@ def test_linear(m, k, n, dtype):
         assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k,n", [(20, 400, 2048), (20, 528, 2049), (256, 2064, 1000), (257, 1024, 1001), (128, 144, 4000),
+                                   (30, 4112, 64), (4, 8192, 40), (5, 6560, 24)])
+def test_linear_few_tiles(m, k, n, dtype):
+    """Tiles few enough for their K to be shared by several CTAs, at the sizes
+    where their number changes; rows and channels past the tiles' last."""
+    x, w, bias = _inputs(m, k, n, dtype, seed=m + k + n)
+    x[m // 2] = 0
+    w8, sw = K.int8_quant_rows(w)
+    x8, sx = quant_rows(x)
+    for act in (None, "gelu"):
+        out = K.int8_linear(x, w8, sw, bias, act=act)
+        torch.cuda.synchronize()
+        assert K.check_status() == 0
+        _check(out, x8, sx, w8, sw, bias, act)
+        # the same bits on the paths of a single token and of the others
+        assert torch.equal(K.int8_linear(x[1:2], w8, sw, bias, act=act), out[1:2])
+        assert torch.equal(K.int8_linear(x[2:], w8, sw, bias, act=act), out[2:])
+
+
 @pytest.mark.parametrize("m,k,n", [(12001, 1008, 1024), (9999, 1024, 1000), (8200, 2064, 1024), (5000, 4096, 1016)])
 def test_linear_over_several_waves(m, k, n):
     """Tiles for several waves of the GPU; rows of a
