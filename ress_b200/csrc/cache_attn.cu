@@ -29,14 +29,18 @@ using namespace tc;
 // (mma.sync in e4m3 would need no conversions in the source, but measured
 // slower, 142 against 122 us for 16 streams of 11 to 44 thousand tokens and 8
 // heads: its operands take more instructions than these conversions.)
-// The running maximum, sums and O are fp32.  Row scales of q (a power of two
-// that brings its largest element to [1, 2)) keep q exact in fp16; P is
-// rounded to fp16 after scaling by 2^14 and the page's V scale over the
-// largest one seen, so that small probabilities keep their bits.
+// The running maximum, sums and O are fp32.  q is scaled by a power of two that
+// brings the row's largest element to [1, 2).  P is rounded to fp16: a page's
+// probabilities count against the page's own maximum, times 2^14, so that small
+// ones keep their bits; the page's weight among the others and its V scale are
+// an fp32 factor of its product, so that neither costs bits.
 // The pages are split over the CTAs of a cluster (and the warps of a CTA).
 // Each CTA sends its rows' partial results to the shared memory of the row's
 // owner, which joins them in CTA order: one launch, no workspace.  Up to 32
 // streams are started longest first, so that the last CTAs are short.
+// More than eight rows are two groups of the tile; what does not change from page
+// to page then lies in shared memory (in registers, with the page's product
+// beside O, it spilled: 16 heads x 32 queries x 43,968 tokens 52 us, 44 so).
 // 16 streams of 11 to 44 thousand tokens, 24 heads on 8: 86 us, 5.2 TB/s of the
 // 6.45 that a copy reaches.  One token, 16 heads, 10,992 tokens: 11.2 us for 22.5
 // MB: a launch, and three pages in turn on each warp, which is bound by the
@@ -68,6 +72,17 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
+}
+// loads that stay where they are written
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
 }
 // shared memory of another CTA of the cluster
 __device__ __forceinline__ uint32_t peer_addr(uint32_t a, int rank) {
@@ -220,12 +235,33 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
         rf[n][0] = __shfl_sync(0xffffffffu, f, 8 * t);  // of row 2t: its lanes are 4 * 2t ..
         rf[n][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
     }
+    // Two groups leave no registers for what does not change: it is read again for every page.
+    __shared__ __align__(16) uint32_t q_s[4][32][4];
+    __shared__ __align__(8) int lim_s[FEW_ROWS];
+    __shared__ __align__(8) float rf_s[FEW_ROWS];
+    if constexpr (NT == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t *w = &q[i >> 1][4 * (i & 1)];
+            if (warp == i) *reinterpret_cast<uint4 *>(q_s[i][lane]) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (warp == 0 && g == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    lim_s[8 * n + 2 * t + e] = lim[n][e];
+                    rf_s[8 * n + 2 * t + e] = rf[n][e];
+                }
+        }
+        __syncthreads();
+    }
 
     float o[NT][4][4] = {};
-    float m[NT][2], l[NT][2] = {};
+    float m[NT][2], l[NT][2] = {};  // sums count in 2^-P_SHIFT
+    const float down = scale_value(127 - P_SHIFT);
 #pragma unroll
     for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
-    int uref = 0;  // O counts in units of 2^(uref - 127 - P_SHIFT)
     const int pg = g ^ ((g >> 1) & 1);  // this lane's key of eight in S^T
     const int kf = 2 * t + (t & 1), kh = 2 * t + 1 - (t & 1);  // and its pair of keys in V^T
     const uint32_t koff = (uint32_t)pg * HD + t * 16;
@@ -259,45 +295,52 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
         const int uv = __shfl_sync(0xffffffffu, (i & 32) ? uv_b : uv_a, i & 31);
         const unsigned char *sk = take();
         if (sk == nullptr) break;
-        float c[4][NT][4] = {};  // sixteen keys each: keys pg (0, 1) and pg + 8 (2, 3) of rows 2t, 2t + 1
-        {
-            uint4 ka[4], kb[4];
+        if constexpr (NT == 2) {
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-                ka[mt] = *reinterpret_cast<const uint4 *>(sk + mt * 16 * HD + koff);
-                kb[mt] = *reinterpret_cast<const uint4 *>(sk + (mt * 16 + 8) * HD + koff);
+            for (int j = 0; j < 4; ++j) {
+                const uint4 u = lds128(smem_u32(q_s[j][lane]));
+                uint32_t *w = &q[j >> 1][4 * (j & 1)];
+                w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
             }
+        }
+        float c[4][NT][4] = {};  // sixteen keys each: keys pg (0, 1) and pg + 8 (2, 3) of rows 2t, 2t + 1
 #pragma unroll
-            for (int st = 0; st < 4; ++st)
+        for (int mt = 0; mt < 4; ++mt) {
+            const uint4 ka = lds128(smem_u32(sk) + mt * 16 * HD + koff), kb = lds128(smem_u32(sk) + (mt * 16 + 8) * HD + koff);
 #pragma unroll
-                for (int mt = 0; mt < 4; ++mt) {
-                    const uint32_t x = st == 0 ? ka[mt].x : st == 1 ? ka[mt].y : st == 2 ? ka[mt].z : ka[mt].w;
-                    const uint32_t y = st == 0 ? kb[mt].x : st == 1 ? kb[mt].y : st == 2 ? kb[mt].z : kb[mt].w;
-                    const uint32_t a0 = e4m3_to_half2((uint16_t)x), a1 = e4m3_to_half2((uint16_t)y);
-                    const uint32_t a2 = e4m3_to_half2((uint16_t)(x >> 16)), a3 = e4m3_to_half2((uint16_t)(y >> 16));
+            for (int st = 0; st < 4; ++st) {
+                const uint32_t x = st == 0 ? ka.x : st == 1 ? ka.y : st == 2 ? ka.z : ka.w;
+                const uint32_t y = st == 0 ? kb.x : st == 1 ? kb.y : st == 2 ? kb.z : kb.w;
+                const uint32_t a0 = e4m3_to_half2((uint16_t)x), a1 = e4m3_to_half2((uint16_t)y);
+                const uint32_t a2 = e4m3_to_half2((uint16_t)(x >> 16)), a3 = e4m3_to_half2((uint16_t)(y >> 16));
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_16816(c[mt][n], a0, a1, a2, a3, q[n][2 * st], q[n][2 * st + 1]);
-                }
+                for (int n = 0; n < NT; ++n) mma_16816(c[mt][n], a0, a1, a2, a3, q[n][2 * st], q[n][2 * st + 1]);
+            }
         }
         done();
         const int base = (first + i * FEW_WARPS) * PAGE;
-        const float fk = scale_value(uk);
-        // a page of larger V scale moves O's unit
-        float fv = scale_value(uv), move = 1.0f;  // NaN stays NaN
-        if (uv != 255) {
-            if (uv > uref) {
-                move = scale_value(max(127 + uref - uv, 0));
-                uref = uv;
-            }
-            fv = scale_value(max(127 + P_SHIFT + uv - uref, 0));
-        }
+        const float fk = scale_value(uk), fv = scale_value(uv) * down;
         // where every row sees the whole page there are no masks (a tenth of the instructions)
         auto page = [&](auto page_whole) {
             constexpr bool whole = decltype(page_whole)::value;
+            if constexpr (NT == 2) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint2 u = lds64(smem_u32(&rf_s[8 * n + 2 * t]));
+                    rf[n][0] = __uint_as_float(u.x);
+                    rf[n][1] = __uint_as_float(u.y);
+                    if (!whole) {
+                        const uint2 w = lds64(smem_u32(&lim_s[8 * n + 2 * t]));
+                        lim[n][0] = (int)w.x;
+                        lim[n][1] = (int)w.y;
+                    }
+                }
+            }
             uint32_t pb[NT][4][2];
+            float f[NT][2];  // of the page's product
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float bias[2], cs[2], alpha[2];
+                float bias[2], cs[2], alpha[2], sum[2] = {};
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float top = -INFINITY;
@@ -313,13 +356,13 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                     cs[e] = rf[n][e] * fk;  // not negative; a NaN one shows in the exponentials
-                    const float mn = fmaxf(m[n][e], top == -INFINITY ? top : top * cs[e]);
+                    top = top == -INFINITY ? top : top * cs[e];
+                    bias[e] = P_SHIFT - (top == -INFINITY ? 0.0f : top);
+                    const float mn = fmaxf(m[n][e], top);
                     const float mb = mn == -INFINITY ? 0.0f : mn;
                     alpha[e] = ex2(m[n][e] - mb);
-                    l[n][e] *= alpha[e];
-                    alpha[e] *= move;
+                    f[n][e] = ex2(top - mb);
                     m[n][e] = mn;
-                    bias[e] = -mb;
                 }
                 if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
 #pragma unroll
@@ -340,23 +383,26 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
                         for (int e = 0; e < 2; ++e) {
                             p[e] = ex2(fmaf(c[mt][n][2 * k + e], cs[e], bias[e]));
                             // a hidden token is 0 even where a factor is 0 or NaN
-                            const bool hidden = !whole && base + mt * 16 + 8 * k + pg >= lim[n][e];
-                            if (hidden) p[e] = 0.0f;
-                            l[n][e] += p[e];
-                            p[e] *= fv;
-                            if (hidden) p[e] = 0.0f;
+                            if (!whole && base + mt * 16 + 8 * k + pg >= lim[n][e]) p[e] = 0.0f;
+                            sum[e] += p[e];
                         }
                         pb[n][mt][k] = transpose8x8(half2_bits(p[0], p[1]));
                     }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    l[n][e] = fmaf(sum[e], f[n][e], l[n][e] * alpha[e]);
+                    // a row that sees none of the page takes nothing from it, a NaN scale neither
+                    f[n][e] = whole || base < lim[n][e] ? f[n][e] * fv : 0.0f;
+                }
             }
             const unsigned char *sv = take();
             if (sv == nullptr) return false;
+            float x[NT][4][4] = {};  // the page's product
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-                const unsigned char *va = sv + mt * 16 * HD + g * 8;
-                uint2 v0 = *reinterpret_cast<const uint2 *>(va + kf * HD), v1 = *reinterpret_cast<const uint2 *>(va + kh * HD);
-                uint2 v2 = *reinterpret_cast<const uint2 *>(va + (8 + kf) * HD);
-                uint2 v3 = *reinterpret_cast<const uint2 *>(va + (8 + kh) * HD);
+                const uint32_t va = smem_u32(sv) + mt * 16 * HD + g * 8;
+                uint2 v0 = lds64(va + kf * HD), v1 = lds64(va + kh * HD);
+                uint2 v2 = lds64(va + (8 + kf) * HD), v3 = lds64(va + (8 + kh) * HD);
                 if (!whole && base + PAGE > len) {  // slots past the stream's end hold anything, NaN codes too
                     const int e = len - base - 16 * mt;
                     if (kf >= e) v0 = make_uint2(0, 0);
@@ -374,10 +420,20 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
                         const uint32_t a0 = e4m3_to_half2((uint16_t)(y0 >> (16 * k))), a1 = e4m3_to_half2((uint16_t)(y1 >> (16 * k)));
                         const uint32_t a2 = e4m3_to_half2((uint16_t)(y2 >> (16 * k))), a3 = e4m3_to_half2((uint16_t)(y3 >> (16 * k)));
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_16816(o[n][d + k], a0, a1, a2, a3, pb[n][mt][0], pb[n][mt][1]);
+                        for (int n = 0; n < NT; ++n) mma_16816(x[n][d + k], a0, a1, a2, a3, pb[n][mt][0], pb[n][mt][1]);
                     }
                 }
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int j = 0; j < 4; j += 2) {
+                        const f32x2 y = f2_fma_rn(f2_pack(x[n][d][j], x[n][d][j + 1]), f2_pack(f[n][0], f[n][1]),
+                                                  f2_pack(o[n][d][j], o[n][d][j + 1]));
+                        f2_unpack(y, o[n][d][j], o[n][d][j + 1]);
+                    }
             return true;
         };
         if (!(base + PAGE <= lo ? page(std::true_type{}) : page(std::false_type{}))) break;
@@ -398,13 +454,12 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
             for (int d = 4; d < 32; d *= 2) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
             if (g == 0) {
                 part_m[warp][8 * n + 2 * t + e] = m[n][e];
-                part_l[warp][8 * n + 2 * t + e] = l[n][e];
+                part_l[warp][8 * n + 2 * t + e] = l[n][e] * down;
             }
         }
     __syncthreads();
     // the warps' O meet in the ring, 4 KB a warp
     float *po = reinterpret_cast<float *>(dyn) + warp * FEW_ROWS * HD;
-    const float unit = scale_value(uref), down = scale_value(127 - P_SHIFT);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -412,8 +467,7 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
 #pragma unroll
             for (int k = 0; k < 2; ++k)
                 *reinterpret_cast<float4 *>(po + (8 * n + 2 * t + e) * HD + 8 * g + 4 * k) =
-                    make_float4(o[n][0][e + 2 * k] * down * unit, o[n][1][e + 2 * k] * down * unit,
-                                o[n][2][e + 2 * k] * down * unit, o[n][3][e + 2 * k] * down * unit);
+                    make_float4(o[n][0][e + 2 * k], o[n][1][e + 2 * k], o[n][2][e + 2 * k], o[n][3][e + 2 * k]);
     __syncthreads();
     if (splits > 1) cluster_wait();  // the peers have started
     const float *co = reinterpret_cast<const float *>(dyn);

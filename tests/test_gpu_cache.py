@@ -453,3 +453,31 @@ def test_refusals():
     K.cache_append(k[:, :0], k[:, :0], **ok)                             # nothing to do
     assert K.cache_attn(q[:, :0], **ok).shape == (1, 0, 4, HD)
     assert K.check_status() == 0
+
+
+@pytest.mark.parametrize("T", [1, 3, 12, 40])
+@pytest.mark.parametrize("gap,weight", [(12, -80), (40, -80), (40, -40), (100, -100), (100, -150)])
+def test_attention_value_scales_far_apart(T, gap, weight):
+    """Pages whose values are 2^gap times the others' and whose weights are
+    2^weight of theirs: what a page adds does not depend on the scales of pages
+    seen before it.  The heads are enough for a warp of the few-query kernel to
+    take pages 8 apart in turn: small values, large ones, small ones again."""
+    H, pages = 300, 24
+    g = _gen(T + gap)
+    cache, table, ln = make_cache(pages, H), shuffled_table(1, pages, pages, seed=gap), _i32(64 * pages)
+    big = table[0, 8:16].long()
+    k = torch.zeros(pages, H, PAGE, HD, device="cuda")
+    k[big, :, :, 0] = -240.0
+    k[..., 1:] = 0.05 * torch.randn(pages, H, PAGE, HD - 1, device="cuda", generator=g)
+    cache["k_pages"].copy_(k)
+    cache["v_pages"].copy_(8 * torch.randn(pages, H, PAGE, HD, device="cuda", generator=g))
+    for n in ("k_scale", "v_scale"):
+        _u8(cache[n]).fill_(127)
+    _u8(cache["v_scale"])[big] = 127 + gap
+    q = torch.randn(1, T, H, HD, device="cuda", generator=g)
+    q[..., 0] = -weight * 0.6931 * 8 / 240
+    q = q.bfloat16()
+    out = K.cache_attn(q, **cache, table=table, lens=ln, out_bf16=False)
+    torch.cuda.synchronize()
+    assert K.check_status() == 0
+    _close(out, *attention(q, cache, table, ln))
