@@ -62,6 +62,8 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
     return (uint32_t)lo | ((uint32_t)hi << 16);
 }
+// The top bits of the bytes of w that are NaN codes (0x7F, 0xFF).
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 // Two codes as halves, exactly (e4m3 lies inside fp16).
 __device__ __forceinline__ uint32_t e4m3_to_half2(uint16_t codes) {
     uint32_t r;

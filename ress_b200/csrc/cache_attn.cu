@@ -41,6 +41,8 @@ using namespace tc;
 // More than eight rows are two groups of the tile; what does not change from page
 // to page then lies in shared memory (in registers, with the page's product
 // beside O, it spilled: 16 heads x 32 queries x 43,968 tokens 52 us, 44 so).
+// A NaN code among V's reaches, in the product, rows that do not see it: where
+// rows see unlike parts of a page it is left out there and looked up at the end.
 // 16 streams of 11 to 44 thousand tokens, 24 heads on 8: 86 us, 5.2 TB/s of the
 // 6.45 that a copy reaches.  One token, 16 heads, 10,992 tokens: 11.2 us for 22.5
 // MB: a launch, and three pages in turn on each warp, which is bound by the
@@ -83,6 +85,28 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
+}
+// Zeros in place of the NaN codes of a block in shared memory; true if there were any.
+__device__ __forceinline__ bool leave_out_nans(uint32_t block, int lane) {
+    bool any = false;
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t at = block + (i * 32 + lane) * 16;
+        uint4 u = lds128(at);
+        if (!(nan_codes(u.x) | nan_codes(u.y) | nan_codes(u.z) | nan_codes(u.w))) continue;
+        any = true;
+        u.x &= ~((nan_codes(u.x) >> 7) * 0xFFu);
+        u.y &= ~((nan_codes(u.y) >> 7) * 0xFFu);
+        u.z &= ~((nan_codes(u.z) >> 7) * 0xFFu);
+        u.w &= ~((nan_codes(u.w) >> 7) * 0xFFu);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+    }
+    any = __any_sync(0xffffffffu, any);
+    if (any) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // a copy takes the block's place
+        __syncwarp();
+    }
+    return any;
 }
 // shared memory of another CTA of the cluster
 __device__ __forceinline__ uint32_t peer_addr(uint32_t a, int rank) {
@@ -257,6 +281,7 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
         __syncthreads();
     }
 
+    bool nan_seen = false;  // a page's NaN codes were left out
     float o[NT][4][4] = {};
     float m[NT][2], l[NT][2] = {};  // sums count in 2^-P_SHIFT
     const float down = scale_value(127 - P_SHIFT);
@@ -397,14 +422,16 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
             }
             const unsigned char *sv = take();
             if (sv == nullptr) return false;
+            // where rows see unlike parts of the page
+            if (!whole && lo != hi && leave_out_nans(smem_u32(sv), lane)) nan_seen = true;
             float x[NT][4][4] = {};  // the page's product
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
                 const uint32_t va = smem_u32(sv) + mt * 16 * HD + g * 8;
                 uint2 v0 = lds64(va + kf * HD), v1 = lds64(va + kh * HD);
                 uint2 v2 = lds64(va + (8 + kf) * HD), v3 = lds64(va + (8 + kh) * HD);
-                if (!whole && base + PAGE > len) {  // slots past the stream's end hold anything, NaN codes too
-                    const int e = len - base - 16 * mt;
+                if (!whole && base + PAGE > hi) {  // slots that no row sees hold anything, NaN codes too
+                    const int e = hi - base - 16 * mt;
                     if (kf >= e) v0 = make_uint2(0, 0);
                     if (kh >= e) v1 = make_uint2(0, 0);
                     if (8 + kf >= e) v2 = make_uint2(0, 0);
@@ -468,6 +495,13 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_kernel(const AttnArgs a, int kv
             for (int k = 0; k < 2; ++k)
                 *reinterpret_cast<float4 *>(po + (8 * n + 2 * t + e) * HD + 8 * g + 4 * k) =
                     make_float4(o[n][0][e + 2 * k], o[n][1][e + 2 * k], o[n][2][e + 2 * k], o[n][3][e + 2 * k]);
+    if (nan_seen) {
+        __syncwarp();
+        const uint64_t dims = nan_dims(a.V.codes + h * a.V.head_stride, a.V.page_stride, table, a.n_pages, first, FEW_WARPS,
+                                       count, lane < 8 * NT ? row_limit(a, b, len, r0 + lane) : 0);
+        for (int d = 0; d < HD; ++d)
+            if (dims >> d & 1) po[lane * HD + d] = NAN;
+    }
     __syncthreads();
     if (splits > 1) cluster_wait();  // the peers have started
     const float *co = reinterpret_cast<const float *>(dyn);

@@ -58,6 +58,29 @@ __device__ __forceinline__ long long row_at(const AttnArgs &a, int b, int h, int
     return b * sb + t * st + (long long)(h * a.group + g) * sh;
 }
 
+// The dims of V in which a row that sees `limit` tokens meets a NaN code, over
+// the stream's pages first, first + step, .. (count of them).  A product with
+// P cannot tell: a NaN would reach the tile's other rows by way of their zeros.
+// So products take such codes as numbers, and where there are any (appends
+// write none) the rows that see them are looked up here.
+static __device__ __noinline__ uint64_t nan_dims(const uint8_t *codes, long long page_stride, const int32_t *table,
+                                                 int n_pages, int first, int step, int count, int limit) {
+    uint64_t dims = 0;
+    for (int i = 0, p = first; i < count && p * PAGE < limit; ++i, p += step) {
+        const int id = table[p];
+        if (id < 0 || id >= n_pages) continue;
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(codes + id * page_stride);
+        const int words = min(PAGE, limit - p * PAGE) * (HD / 4);
+#pragma unroll 1
+        for (int j = 0; j < words; ++j) {
+            const uint32_t nan = nan_codes(__ldg(w + j));
+            if (nan == 0) continue;
+            for (int k = 0; k < 4; ++k) dims |= (uint64_t)(nan >> (8 * k + 7) & 1) << (j % (HD / 4) * 4 + k);
+        }
+    }
+    return dims;
+}
+
 // cache_attn_tc.cu: rows by the hundred.  Workspace bytes (0: none needed) and the launch.
 size_t many_workspace(int B, int Hkv, long long rows, long long table_width);
 int launch_many(const AttnArgs &a, int B, int Hkv, void *workspace, cudaStream_t stream);

@@ -80,6 +80,7 @@ struct Bars {
     uint64_t s_done, pv_done;
     uint32_t tmem;
     int abort_flag, hi, lo[TILES], join[TILES];
+    int nan_seen;  // a NaN code among the values that some row sees
     int info[INFO];
     int lim[TILES * TILE];
     float unit[TILES * TILE];  // of a row's S, in log2 units, K's scale aside
@@ -130,7 +131,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // Four e4m3 codes to bf16 pairs (0, 2) and (1, 3).  A code's exponent and
 // significand bits, moved into a bf16's place, are its value times 2^-120
 // (the biases are 7 and 127; subnormals as well): one multiplication by
-// 2^120 and the page's scale is exact.
+// 2^120 and the page's scale is exact.  NaN codes become 480: what they do to
+// the rows that see them is put in at the end (nan_dims).
 __device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t f, uint32_t &even, uint32_t &odd) {
     even = mul_bf16x2(((w << 8) & 0x80008000u) | ((w & 0x007F007Fu) << 4), f);
     odd = mul_bf16x2((w & 0x80008000u) | ((w & 0x7F007F00u) >> 4), f);
@@ -308,6 +310,7 @@ __global__ void __launch_bounds__(NT, 1)
         mbar_init(&B.pv_done, 1);
         B.abort_flag = 0;
         B.hi = 0;
+        B.nan_seen = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (split == 0 && bad_len(a, b)) atomicOr(a.status, RESS_STATUS_CACHE_RANGE);
     }
@@ -518,9 +521,12 @@ __global__ void __launch_bounds__(NT, 1)
                 const bool nan = uv == 255 || uk == 255;
                 const uint32_t f = nan ? 0u : pow2_bf16x2(min(uv - 7, 120));
                 const bool big = !nan && uv > 127;
+                uint32_t nans = 0;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int key = (c + 128 * i) >> 2, qd = c & 3;
+                    if ((p0 + j) * PAGE + key < B.hi)
+                        nans |= nan_codes(w[i].x) | nan_codes(w[i].y) | nan_codes(w[i].z) | nan_codes(w[i].w);
                     uint32_t o[8];
                     codes_to_bf16(w[i].x, f, o[0], o[1]);
                     codes_to_bf16(w[i].y, f, o[2], o[3]);
@@ -535,6 +541,7 @@ __global__ void __launch_bounds__(NT, 1)
                     sts128(row + (((uint32_t)(2 * qd) ^ sw) << 4), o[0], o[1], o[2], o[3]);
                     sts128(row + (((uint32_t)(2 * qd + 1) ^ sw) << 4), o[4], o[5], o[6], o[7]);
                 }
+                if (nans) B.nan_seen = 1;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
@@ -661,6 +668,12 @@ __global__ void __launch_bounds__(NT, 1)
                     o[i + 1] = __uint_as_float(ov[i + 2]);
                     o[i + 2] = __uint_as_float(ov[i + 1]);
                     o[i + 3] = __uint_as_float(ov[i + 3]);
+                }
+                if (*(volatile int *)&B.nan_seen) {
+                    const uint64_t nan = nan_dims(a.V.codes + h * a.V.head_stride, a.V.page_stride, table - p0, a.n_pages, p0, 1, cnt, lim);
+#pragma unroll
+                    for (int i = 0; i < HD; ++i)
+                        if (nan >> i & 1) o[i] = NAN;
                 }
             } else {
 #pragma unroll

@@ -481,3 +481,30 @@ def test_attention_value_scales_far_apart(T, gap, weight):
     torch.cuda.synchronize()
     assert K.check_status() == 0
     _close(out, *attention(q, cache, table, ln))
+
+
+@pytest.mark.parametrize("T", [1, 12, 140])
+@pytest.mark.parametrize("code", [0x7F, 0xFF])
+def test_attention_nan_codes(T, code):
+    """A NaN among a value's codes shows in its dim of the rows that see it, and
+    nowhere else; one in a key makes those rows NaN."""
+    L, H = 300, 2
+    cache, table, ln = _filled(1, [L], H, seed=13)
+    q = torch.randn(1, T, H, HD, device="cuda", generator=_gen(13)).bfloat16()
+    limits = torch.full((1, T), L, dtype=torch.int32, device="cuda")
+    if T > 1:
+        limits[0, 1::4], limits[0, 2::4], limits[0, 3::4] = 100, 128, 111
+    ref, size = attention(q, cache, table, ln, limits)
+    want = torch.zeros_like(ref, dtype=torch.bool)
+    for token, head, dim, key in ((30, 0, 5, False), (110, 1, 63, False), (110, 1, 8, False), (150, 0, 17, False),
+                                  (299, 1, 40, False), (299, 0, 3, True)):
+        pages = _u8(cache["k_pages" if key else "v_pages"])
+        pages[table[0, token // PAGE].long(), head, token % PAGE, dim] = code
+        sees = limits[0] > token
+        want[0, sees, head] |= True if key else (torch.arange(HD, device="cuda") == dim)
+        out = K.cache_attn(q, **cache, table=table, lens=ln, limits=limits if T > 1 else None, out_bf16=False)
+        torch.cuda.synchronize()
+        assert torch.equal(out.isnan(), want), (token, head, dim)
+        zero = torch.zeros_like(ref)
+        _close(out.masked_fill(want, 0), torch.where(want, zero, ref), size)
+    assert K.check_status() == 0
