@@ -43,7 +43,8 @@ inline int check_cache(const ress_cache *c) {
 __device__ __forceinline__ float scale_value(int u) {
     return __uint_as_float(u == 255 ? 0x7FC00000u : (u == 0 ? 0x00400000u : (uint32_t)u << 23));
 }
-// 2^(127 - u); 0 for the NaN code, so that its page holds zeros
+// 2^(127 - u) of a page's code, which append makes 247 at most; 0 for the NaN
+// code, so that its page holds zeros
 __device__ __forceinline__ float scale_inverse(int u) { return __uint_as_float(u == 255 ? 0u : (uint32_t)(254 - u) << 23); }
 
 // The code of the smallest power of two that brings |x| <= amax to 448 or

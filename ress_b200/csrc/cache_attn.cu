@@ -145,7 +145,7 @@ __device__ __forceinline__ float load_q16(const AttnArgs &a, int b, int h, int r
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
     const int e = (int)(m >> 23);
-    const float inv = scale_inverse(e);
+    const float inv = row_inverse(e);
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = half2_bits(x[2 * j] * inv, x[2 * j + 1] * inv);
     return scale_value(e) * a.scale_log2;

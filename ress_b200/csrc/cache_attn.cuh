@@ -51,6 +51,11 @@ __device__ __forceinline__ int row_limit(const AttnArgs &a, int b, int len, int 
     if (r >= a.rows) return -1;
     return a.limits != nullptr ? max(0, min(len, a.limits[(long long)b * a.Tq + r / a.group])) : len;
 }
+// 2^(127 - e) for the exponent field e of a q row's largest element: finite up
+// to e = 254, 0 for a row that is not (its scale is NaN).
+__device__ __forceinline__ float row_inverse(int e) {
+    return __uint_as_float(e == 255 ? 0u : max((uint32_t)(254 - e) << 23, 0x00400000u));  // 2^-127 is subnormal
+}
 // Element offset of row r of (stream b, key/value head h), for strides (sb, st, sh).
 __device__ __forceinline__ long long row_at(const AttnArgs &a, int b, int h, int r, long long sb, long long st,
                                             long long sh) {

@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(NT, 1)
 #pragma unroll
         for (int k = 0; k < 32; ++k) am = max(am, max((w[k] << 16) & 0x7FFFFFFFu, w[k] & 0x7FFF0000u));
         const int e = max((int)(am >> 23), 8);  // 2^(134 - e) stays in range, for a zero row as well
-        const float f = scale_inverse(e) * 128.0f;
+        const float f = row_inverse(e) * 128.0f;
         const uint32_t base = sQ + (row / TILE) * Q_BYTES + (row % TILE) * 128;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {  // 16 dims: one 16-byte piece of each part

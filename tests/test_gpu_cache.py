@@ -508,3 +508,14 @@ def test_attention_nan_codes(T, code):
         zero = torch.zeros_like(ref)
         _close(out.masked_fill(want, 0), torch.where(want, zero, ref), size)
     assert K.check_status() == 0
+
+
+def test_attention_takes_queries_of_any_size():
+    """bf16 rows up to the largest finite value."""
+    cache, table, ln = _filled(1, [200], 2, seed=15, gain=1e-30)
+    for T in (1, 9, 150):
+        q = torch.randn(1, T, 2, HD, device="cuda", generator=_gen(15))
+        q = (q / q.abs().amax(-1, keepdim=True) * 3.3e38).bfloat16()
+        out = K.cache_attn(q, **cache, table=table, lens=ln, sm_scale=1e-8, out_bf16=False)
+        _close(out, *attention(q, cache, table, ln, sm_scale=1e-8))
+    assert K.check_status() == 0
