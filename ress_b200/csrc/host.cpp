@@ -4,12 +4,14 @@
 //
 // These calls are made per token and take the GPU a few microseconds; the
 // same checks in Python took 6 to 13 microseconds a call, which bounded it.
+// A call runs on its tensors' device, whichever is the current one.
 // The library's entry points and the addresses of the devices' status words
 // are handed over by bind(); nothing here is linked against the library.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include "../../include/ress_sm100.h"
@@ -150,6 +152,7 @@ PyObject *cache_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
         count(n, 18);
         const at::Tensor &k = tensor(o[0], "k"), &v = tensor(o[1], "v");
         const int i = cuda_index(k);
+        const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
         const at::Tensor *q = opt(o[8], "q"), *n_new = opt(o[9], "n_new"), *pos = opt(o[15], "pos"),
                          *cos = opt(o[16], "rope_cos"), *sin = opt(o[17], "rope_sin");
         const at::ScalarType dtype = k.scalar_type();
@@ -219,6 +222,7 @@ PyObject *cache_attn(PyObject *, PyObject *const *o, Py_ssize_t n) {
         count(n, 11);
         const at::Tensor &q = tensor(o[0], "q");
         const int i = cuda_index(q);
+        const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
         require(q.scalar_type() == at::kBFloat16, "cache_attn takes bf16 q");
         const Rows r = head_rows(q, "q");
         const ress_cache c = cache_of(i, r.B, o + 1);
@@ -277,6 +281,7 @@ PyObject *int8_quant_rows(PyObject *, PyObject *const *o, Py_ssize_t n) {
         count(n, 1);
         const at::Tensor &x = tensor(o[0], "x");
         const int i = cuda_index(x), dt = dtype_code(x.scalar_type());
+        const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
         const at::Tensor rows = rows2d(x);
         const int64_t M = rows.size(0), K = rows.size(1);
         require(M <= INT_MAX && K <= INT_MAX, "x is too large");
@@ -301,6 +306,7 @@ PyObject *int8_linear(PyObject *, PyObject *const *o, Py_ssize_t n) {
         const at::Tensor &x = tensor(o[0], "x"), &w = tensor(o[1], "w8"), &ws = tensor(o[2], "w_scale");
         const at::Tensor *bias = opt(o[3], "bias");
         const int i = cuda_index(x), dt = dtype_code(x.scalar_type());
+        const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
         const int gelu = PyObject_IsTrue(o[4]);
         const long want = PyLong_AsLong(o[5]);
         if (PyErr_Occurred()) throw PythonError{};

@@ -4,6 +4,9 @@ they touch a device, their structs have the layout the binding packs, the
 unwired."""
 
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -149,3 +152,70 @@ def test_wiring_without_a_gpu():
     assert "forward" not in m.aggregator.global_blocks[0].attn.__dict__
     with pytest.raises(RessError):
         stream.quantize_linears(m)  # laid out on the GPU
+
+
+# Two devices that do nothing: what the tensor library asks the runtime before a call.
+FAKE_RUNTIME = """
+static int device;
+int cudaGetDeviceCount(int *n) { *n = 2; return 0; }
+int cudaGetDevice(int *d) { *d = device; return 0; }
+int cudaSetDevice(int d) { device = d; return 0; }
+int cudaDeviceGetStreamPriorityRange(int *lo, int *hi) { *lo = 0; *hi = -5; return 0; }
+"""
+ON_ANOTHER_DEVICE = """
+import ctypes, os, sys
+import torch
+from ress_b200 import _lib
+
+class Meta(torch.Tensor):  # a tensor of device 1 without memory
+    @classmethod
+    def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+        raise AssertionError(f)
+
+def t(*shape, dtype=torch.float32):
+    return torch.Tensor._make_wrapper_subclass(Meta, shape, dtype=dtype, device=torch.device("cuda", 1))
+
+runtime = ctypes.CDLL(sys.argv[1])
+def current():
+    d = ctypes.c_int()
+    runtime.cudaGetDevice(ctypes.byref(d))
+    return d.value
+
+# what the tensor library's own start-up would tell its device guard
+has_context = ctypes.CFUNCTYPE(ctypes.c_bool, ctypes.c_byte)(lambda i: True)
+c10 = ctypes.CDLL(os.path.join(os.path.dirname(torch.__file__), "lib", "libc10_cuda.so"))
+c10._ZN3c104cuda9_internal20setHasPrimaryContextEPFbaE(has_context)
+
+# entry points that note the current device
+seen, P = [], ctypes.c_void_p
+call = ctypes.CFUNCTYPE(ctypes.c_int, P, P, P, P)(lambda *a: (seen.append(current()), 0)[1])
+size = ctypes.CFUNCTYPE(ctypes.c_size_t, P, P, P, P)(lambda *a: 0)
+names = dict.fromkeys(_lib.SIGNATURES, ctypes.cast(call, P).value)
+names["ress_cache_attn_workspace"] = ctypes.cast(size, P).value
+import importlib.util
+spec = importlib.util.spec_from_file_location("ress_b200._host", _lib.HOST_PATH)
+host = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(host)
+word = ctypes.c_int()
+host.bind(_lib.RessError, lambda i: ctypes.addressof(word), names)
+
+pages, scales, ints = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.int32
+cache = [t(4, 2, 64, 64, dtype=pages)] * 2 + [t(4, 2, dtype=scales)] * 2 + [t(1, 4, dtype=ints), t(1, dtype=ints)]
+k, q = t(1, 3, 2, 64), t(1, 3, 2, 64, dtype=torch.bfloat16)
+host.cache_append(k, k, *cache, *[None] * 6, 1e-5, None, None, None)
+host.cache_attn(q, *cache, None, None, t(1, 3, 2, 64), True)
+print(*seen, current())
+"""
+
+
+def test_calls_run_on_their_tensors_device(tmp_path):
+    """Tensors of device 1 while device 0 is current: the entry points find device 1 current, and
+    afterwards device 0 is again.  The runtime is a stand-in, nothing is launched."""
+    source, library = tmp_path / "runtime.c", tmp_path / "runtime.so"
+    source.write_text(FAKE_RUNTIME)
+    subprocess.run(["cc", "-shared", "-fPIC", str(source), "-o", str(library)], check=True)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", ON_ANOTHER_DEVICE, str(library)], capture_output=True, text=True, cwd=root,
+                       env={**os.environ, "LD_PRELOAD": str(library), "PYTHONPATH": root})
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert r.stdout.split() == ["1", "1", "0"]
