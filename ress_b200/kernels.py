@@ -10,6 +10,7 @@ into a per-device status word that ``check_status`` reads.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 
@@ -37,6 +38,23 @@ def _ptr(t):
 
 def _stream(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _on_device(f):
+    """Runs a wrapper with its first tensor's device current: the library
+    launches on the current one."""
+
+    @functools.wraps(f)
+    def call(*args, **kw):
+        for x in (*args, *kw.values()):
+            if isinstance(x, torch.Tensor):
+                if x.is_cuda and x.device.index != torch.cuda.current_device():
+                    with torch.cuda.device(x.device):
+                        return f(*args, **kw)
+                break
+        return f(*args, **kw)
+
+    return call
 
 
 def _dtype_code(dt) -> int:
@@ -138,6 +156,7 @@ def _strides(x: torch.Tensor, L: Layout):
 
 
 # ----------------------------------------------------------------- scoring
+@_on_device
 def pool_quant_q(q, L: Layout, pool=True, quant=True):
     _dev_ok(q)
     sb, sh, st = _strides(q, L)
@@ -151,6 +170,7 @@ def pool_quant_q(q, L: Layout, pool=True, quant=True):
     return qbar, q8, qs
 
 
+@_on_device
 def qkv_prologue_scored(qkv, L: Layout, qn_weight=None, qn_bias=None, kn_weight=None, kn_bias=None, eps=1e-5,
                         pos=None, rope_cos=None, rope_sin=None):
     """bf16 (B, T, 3*H*64) qkv Linear output of a global layer (layout L) ->
@@ -188,6 +208,7 @@ def qkv_prologue_scored(qkv, L: Layout, qn_weight=None, qn_bias=None, kn_weight=
     return dict(k=k, v=v, q_special=q_special, qbar=qbar, q8=q8, qs=qs)
 
 
+@_on_device
 def pool_quant_kv(k, v, L: Layout, pool=True, quant=True, ws=None):
     _dev_ok(k, v)
     if k.stride() != v.stride() or k.dtype != v.dtype:
@@ -210,6 +231,7 @@ def pool_quant_kv(k, v, L: Layout, pool=True, quant=True, ws=None):
     return kbar, vbar, k8, ks, v16, km
 
 
+@_on_device
 def predict(qbar, kbar, n_cand, full=True, cond=True):
     """(BH, nq, 64), (BH, nkp, 64) -> attn_full (BH, nq, nkp), attn_cond (BH, nq, n_cand)."""
     _dev_ok(qbar, kbar)
@@ -228,6 +250,7 @@ def cdf_value(cdf_threshold: float, eps: float = 1e-5) -> float:
     return float(torch.as_tensor(cdf_threshold, dtype=torch.float32) + eps)
 
 
+@_on_device
 def baseline(cond, sparse_ratio=None, cdf_threshold=None):
     """compute_baseline_num_to_select on (..., n) -> (...) int32."""
     _dev_ok(cond)
@@ -258,6 +281,7 @@ def scores_norm(head_scores: torch.Tensor) -> torch.Tensor:
     return hs / s
 
 
+@_on_device
 def hess_adjust(base, snorm, max_val, beta=1.0, min_clamp=0, max_iters=1000):
     """base (B, H, nq) int -> (B, H, nq) int32; snorm (H,) fp32 (any device)."""
     _dev_ok(base)
@@ -283,6 +307,7 @@ def round_fracs(n_iters, restore_frac=0.5, decay=0.5):
     return out
 
 
+@_on_device
 def restore_swap(attn_full, vbar, M, nts, n_cand, n_iters=5, track_best=True, restore_frac=0.5, decay=0.5,
                  sink_blocks=0, lead_blocks=0, want_drop=False, want_s=False, want_lists=True, ws=None,
                  list_width=None):
@@ -320,6 +345,7 @@ def restore_swap(attn_full, vbar, M, nts, n_cand, n_iters=5, track_best=True, re
     return dict(drop=drop, s=s, lists=lists, counts=counts)
 
 
+@_on_device
 def select_prob(cond, nts, sink_blocks=0, lead_blocks=0, want_keep=False, want_lists=True, list_width=None):
     _dev_ok(cond, nts)
     c = cond.contiguous()
@@ -336,6 +362,7 @@ def select_prob(cond, nts, sink_blocks=0, lead_blocks=0, want_keep=False, want_l
     return dict(keep=keep, lists=lists, counts=counts)
 
 
+@_on_device
 def top_m_mask(q, counts, largest=True):
     _dev_ok(q)
     qc = q.contiguous()
@@ -352,6 +379,7 @@ def top_m_mask(q, counts, largest=True):
     return out.view(torch.bool)
 
 
+@_on_device
 def round_step(P, term_k, s_sq, term_q, drop, per_iter, raw_bf16, q_bf16, g_norm_sq=None, kept_mass=None,
                k_eps=1e-6):
     _dev_ok(P, term_k, s_sq, term_q, drop, per_iter)
@@ -375,6 +403,7 @@ def round_step(P, term_k, s_sq, term_q, drop, per_iter, raw_bf16, q_bf16, g_norm
     return new.view(torch.bool), cnt
 
 
+@_on_device
 def map_to_lists(block_map):
     _dev_ok(block_map)
     m = block_map.contiguous().view(torch.uint8) if block_map.dtype == torch.bool else block_map.to(torch.uint8).contiguous()
@@ -428,6 +457,7 @@ def split_piece(rows: int, list_width: int, sm_count: int, schedule: bool = True
     return False
 
 
+@_on_device
 def sparse_attn(q8, qscale, k8, kscale, v16, lists, counts, out=None, out_layout=None, sm_scale=None,
                 schedule=True, split=False):
     """Block-sparse attention.  q8 (BH, Tq, 64); k8/v16 (BH, Tk, 64).
@@ -484,6 +514,7 @@ def sparse_attn(q8, qscale, k8, kscale, v16, lists, counts, out=None, out_layout
     return out
 
 
+@_on_device
 def dense_attn(q, k, v, out=None, out_bf16=None, sm_scale=None, out_rows=None):
     """Dense non-causal attention, bf16 on the tensor cores (ress_dense_attn).
     q (S, Tq, 64), k/v (S, Tk, 64) bf16 with a contiguous last dim and one
@@ -520,6 +551,7 @@ def dense_attn(q, k, v, out=None, out_bf16=None, sm_scale=None, out_rows=None):
     return out
 
 
+@_on_device
 def qkv_prologue(qkv, H, qn_weight=None, qn_bias=None, kn_weight=None, kn_bias=None, eps=1e-5, pos=None,
                  rope_cos=None, rope_sin=None):
     """(B, T, 3*H*64) qkv Linear output -> q, k, v (B, H, T, 64): q/k LayerNorm

@@ -71,3 +71,36 @@ def test_dtype_and_shape_codes():
     fake = ctypes.c_void_p(16)  # never dereferenced: rejected before any launch
     assert lib.ress_baseline(7, fake, 1, 10, 0, 0.0, 3, fake, None) == -2  # RESS_E_DTYPE
     assert lib.ress_baseline(0, fake, 1, 20000, 1, 0.97, 3, fake, None) == -3  # RESS_E_SHAPE
+
+
+def test_wrappers_run_on_their_tensors_device(monkeypatch):
+    """Every wrapper that launches makes its tensors' device current (the library launches on the current one)."""
+    import contextlib
+    import inspect
+
+    import torch
+
+    from ress_b200 import kernels as K
+
+    launching = [f for n, f in vars(K).items() if inspect.isfunction(f) and n != "_stream" and "_stream(" in
+                 inspect.getsource(f)]
+    assert len(launching) >= 14 and all(hasattr(f, "__wrapped__") for f in launching)
+
+    class Meta(torch.Tensor):  # a tensor of device 1 without memory
+        @classmethod
+        def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+            raise AssertionError(f)
+
+    now = [0]
+
+    @contextlib.contextmanager
+    def device(d):
+        before, now[0] = now[0], d.index
+        yield
+        now[0] = before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    x = torch.Tensor._make_wrapper_subclass(Meta, (4,), device=torch.device("cuda", 1))
+    f = K._on_device(lambda *a, **kw: now[0])
+    assert f(None, x) == 1 and f(q=x) == 1 and f(torch.zeros(1)) == 0 and now == [0]
