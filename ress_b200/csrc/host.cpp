@@ -202,7 +202,7 @@ PyObject *cache_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
         at::Tensor out;
         if (q != nullptr) {
             const Rows rq = head_rows(*q, "q");
-            require(rq.B == rk.B && rq.T == rk.T && q->scalar_type() == dtype && rq.H > 0 && rq.H % c.heads == 0,
+            require(rq.B == rk.B && rq.T == rk.T && q->scalar_type() == dtype && c.heads > 0 && rq.H > 0 && rq.H % c.heads == 0,
                     "q must have k's tokens and type, and a multiple of its heads");
             out = at::empty({rk.B, rk.T, rq.H, HD}, q->options());
             a.q = data<void>(q);

@@ -519,3 +519,11 @@ def test_attention_takes_queries_of_any_size():
         out = K.cache_attn(q, **cache, table=table, lens=ln, sm_scale=1e-8, out_bf16=False)
         _close(out, *attention(q, cache, table, ln, sm_scale=1e-8))
     assert K.check_status() == 0
+
+
+def test_append_refuses_a_pool_without_heads():
+    cache, table, ln = _filled(1, [10], 2, seed=14)
+    none = {n: t[:, :0] for n, t in cache.items()}
+    k = torch.zeros(1, 3, 0, HD, device="cuda")
+    with pytest.raises(RessError):
+        K.cache_append(k, k, **none, table=table, lens=ln, q=torch.zeros(1, 3, 4, HD, device="cuda"))
