@@ -583,6 +583,7 @@ static bool allow_wide_clusters(const void *kern, int which) {
 
 static int launch_few(const AttnArgs &a, int B, int Hkv, cudaStream_t stream) {
     const int tiles = (a.rows + FEW_ROWS - 1) / FEW_ROWS;
+    if ((long long)tiles * Hkv > 65535) return RESS_E_SHAPE;  // the grid's second dimension
     const long long groups = (long long)tiles * Hkv * B;
     // CTAs per (rows, head, stream).  While the CTAs fit on an SM each, pages enough
     // for half a CTA's warps suffice (1 x 16 heads x 1,374 tokens: 9.6 us in one

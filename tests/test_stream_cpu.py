@@ -219,3 +219,10 @@ def test_calls_run_on_their_tensors_device(tmp_path):
                        env={**os.environ, "LD_PRELOAD": str(library), "PYTHONPATH": root})
     assert r.returncode == 0, r.stderr[-2000:]
     assert r.stdout.split() == ["1", "1", "0"]
+
+
+@pytest.mark.parametrize("heads", [32768, 65535])
+def test_heads_beyond_a_grid_are_refused(heads):
+    """Two tiles of rows a head make more blocks than a grid's second dimension takes."""
+    wide = _cache(heads=heads, ps=heads * 4096, ss=heads)
+    assert _lib.load().ress_cache_attn(wide, _attn(tokens=20, q_heads=heads), FAKE, None) == -3
