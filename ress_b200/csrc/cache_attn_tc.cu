@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(NT, 1)
             const int c = tid - 128;
             for (int j = 0; j < cnt; ++j) {
                 const int cs = j % NC, vs = j % NV;
-                if (!wait_bar(&B.c_full[cs], (j / NC) & 1, abort_flag, a.status)) break;
+                if (!wait_bar_warp(&B.c_full[cs], (j / NC) & 1, abort_flag, a.status)) break;
                 const int uv = (B.info[j % INFO] >> 8) & 255, uk = B.info[j % INFO] & 255;
                 uint4 w[2];
 #pragma unroll
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(NT, 1)
                     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                                  : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
                                  : "r"(sC + cs * BLOCK_BYTES + (c + 128 * i) * 16));
-                if (j >= NV && !wait_bar(&B.v_empty[vs], (j / NV - 1) & 1, abort_flag, a.status)) break;
+                if (j >= NV && !wait_bar_warp(&B.v_empty[vs], (j / NV - 1) & 1, abort_flag, a.status)) break;
                 // 2^(uv - 127 + 120), in two steps where that is beyond bf16; a page of NaN
                 // scale becomes zeros here and NaN in P, where it meets only rows that see it
                 const bool nan = uv == 255 || uk == 255;
