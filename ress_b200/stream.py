@@ -62,7 +62,7 @@ class StreamCache:
             raise RessError(f"the cache holds {self.max_tokens} tokens a stream: {self._most} may be used, {T} more do "
                             "not fit")
         rows = K.cache_append(k, v, **self.tensors, q=q, n_new=n_new, **prologue)
-        self.lens += T if n_new is None else n_new
+        self.lens += T if n_new is None else n_new.clamp(0, T)  # as the call takes it
         self._most += T
         return rows
 

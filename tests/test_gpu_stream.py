@@ -149,3 +149,24 @@ def test_reset_remove_and_refusals():
     odd = vggt.Attention(96, 3, True, None)  # 32 head dims
     with pytest.raises(RessError, match="64 head dims"):
         stream._prologue(odd)
+
+
+def _cache_of(streams, tokens, heads=2):
+    """A cache whose unused slots hold bytes that are no values."""
+    c = stream.StreamCache(streams, heads, tokens)
+    for t in (c.k_pages, c.v_pages, c.k_scale, c.v_scale):
+        t.view(torch.uint8).fill_(0xFF)
+    return c
+
+
+@pytest.mark.parametrize("asked", [9, -3])
+def test_cache_counts_what_was_stored(asked):
+    """n_new beyond the tokens given, or below none: the lengths follow what the pages got."""
+    g = torch.Generator("cuda").manual_seed(5)
+    k, v = torch.randn(2, 2, 5, 2, 64, device="cuda", generator=g)
+    c = _cache_of(2, 200)
+    c.append(k, v)
+    c.append(k, v, n_new=torch.tensor([asked, 2], dtype=torch.int32, device="cuda"))
+    assert c.lens.tolist() == [5 + min(max(asked, 0), 5), 7]
+    out = c.attend(torch.randn(2, 1, 2, 64, device="cuda", generator=g).bfloat16())
+    assert bool(out.isfinite().all()) and K.check_status() == 0
