@@ -42,7 +42,7 @@ class StreamCache:
         self.k_scale, self.v_scale = (torch.empty(n, heads, dtype=torch.float8_e8m0fnu, device=device) for _ in range(2))
         self.table = torch.arange(n, dtype=torch.int32, device=device).view(streams, self.pages_per_stream)
         self.lens = torch.zeros(streams, dtype=torch.int32, device=device)
-        self._most = 0  # tokens that the longest stream can hold by now, known without a look at the device
+        self._most = 0  # tokens that the longest stream can hold by now
 
     @property
     def tensors(self) -> dict:
@@ -55,15 +55,24 @@ class StreamCache:
         return sum(t.numel() * t.element_size() for t in self.tensors.values())
 
     def append(self, k, v, q=None, n_new=None, **prologue):
-        """Adds k, v (streams, T, heads, 64) behind what the streams hold; returns
-        q's rows, normalised and rotated as k's (kernels.cache_append)."""
+        """Adds k, v (streams, T, heads, 64) behind what the streams hold, the
+        first n_new (streams,) of them where given; returns q's rows, normalised
+        and rotated as k's (kernels.cache_append).  Whether they fit is known
+        without a look at the device until the longest stream may be full,
+        padding counted; from then on a call waits for the lengths."""
         T = k.shape[1]
-        if self._most + T > self.max_tokens:
-            raise RessError(f"the cache holds {self.max_tokens} tokens a stream: {self._most} may be used, {T} more do "
+        if n_new is not None and (not isinstance(n_new, torch.Tensor) or n_new.device != self.lens.device):
+            raise RessError("n_new must be a tensor on the cache's device")
+        new = T if n_new is None else n_new.clamp(0, T)  # as the call takes it
+        most = self._most + T
+        if most > self.max_tokens and not torch.cuda.is_current_stream_capturing():
+            most = int((self.lens + new).max())
+        if most > self.max_tokens:
+            raise RessError(f"the cache holds {self.max_tokens} tokens a stream: with {T} more there may be {most}, which do "
                             "not fit")
         rows = K.cache_append(k, v, **self.tensors, q=q, n_new=n_new, **prologue)
-        self.lens += T if n_new is None else n_new.clamp(0, T)  # as the call takes it
-        self._most += T
+        self.lens += new
+        self._most = most
         return rows
 
     def attend(self, q, limits=None, **kw):

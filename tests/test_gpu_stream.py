@@ -170,3 +170,24 @@ def test_cache_counts_what_was_stored(asked):
     assert c.lens.tolist() == [5 + min(max(asked, 0), 5), 7]
     out = c.attend(torch.randn(2, 1, 2, 64, device="cuda", generator=g).bfloat16())
     assert bool(out.isfinite().all()) and K.check_status() == 0
+
+
+def test_cache_counts_tokens_not_padding():
+    """Padded appends whose tokens fit are taken; one that does not fit is not, and changes nothing."""
+    g = torch.Generator("cuda").manual_seed(6)
+    k, v = torch.randn(2, 3, 8, 2, 64, device="cuda", generator=g)
+    c = _cache_of(3, 70)
+    n_new = torch.tensor([1, 5, 0], dtype=torch.int32, device="cuda")
+    for _ in range(14):  # 14 x 8 padded tokens, 70 in the longest stream
+        c.append(k, v, n_new=n_new)
+    assert c.lens.tolist() == [14, 70, 0]
+    with pytest.raises(RessError, match="do not fit"):
+        c.append(k, v, n_new=n_new)
+    assert c.lens.tolist() == [14, 70, 0]
+    c.append(k, v, n_new=torch.tensor([8, 0, 8], dtype=torch.int32, device="cuda"))
+    assert c.lens.tolist() == [22, 70, 8]
+    out = c.attend(torch.randn(3, 1, 2, 64, device="cuda", generator=g).bfloat16())
+    assert bool(out.isfinite().all()) and K.check_status() == 0
+    c.reset()
+    c.append(k, v)
+    assert c.lens.tolist() == [8, 8, 8]
