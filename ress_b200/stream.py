@@ -186,13 +186,14 @@ def apply_stream(model, streams: int = 1, max_frames: int = 64, frame_tokens: in
         p = next(attn.parameters(), None)
         device = p.device if p is not None else next(attn.buffers()).device
         cache = StreamCache(streams, attn.num_heads, max_frames * frame_tokens, device)
-        prologue = _prologue(attn)
+        _prologue(attn)  # refused here, not at the first frame
 
-        def _fwd(self, x, pos=None, xpos=None, attn_bias=None, attn_mask=None, _cache=cache, _prologue=prologue):
+        def _fwd(self, x, pos=None, xpos=None, attn_bias=None, attn_mask=None, _cache=cache):
             if attn_bias is not None or attn_mask is not None:
                 raise AssertionError("streaming attention decides what each frame sees; a caller-side attn_bias or "
                                      "attn_mask has no place in it")
-            return stream_attention_forward(self, x, pos if pos is not None else xpos, _cache, frame_tokens, _prologue)
+            # the norms as they are now: weights may have been loaded or moved since
+            return stream_attention_forward(self, x, pos if pos is not None else xpos, _cache, frame_tokens, _prologue(self))
 
         attn.ress_stream = (cache, attn.__dict__.get("forward"))
         attn.forward = MethodType(_fwd, attn)

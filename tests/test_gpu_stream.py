@@ -191,3 +191,25 @@ def test_cache_counts_tokens_not_padding():
     c.reset()
     c.append(k, v)
     assert c.lens.tolist() == [8, 8, 8]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_loaded_after_apply_stream(dtype):
+    """The norms in use are the model's present ones, whatever its type."""
+    m, fresh = _model(dtype), _model(dtype)
+    state = {n: (t * (1 + 0.5 * torch.sin(torch.arange(t.numel(), device="cuda")).view_as(t))).to(t.dtype)
+             if "_norm" in n else t for n, t in m.state_dict().items()}
+    images = _images(1, 2)
+    stream.apply_stream(m, max_frames=2, frame_tokens=FRAME)
+    m.load_state_dict(state)
+    fresh.load_state_dict(state)
+    stream.apply_stream(fresh, max_frames=2, frame_tokens=FRAME)
+    with torch.inference_mode():
+        for i in range(2):
+            a, b = (x(images[:, i:i + 1], first_frame=i == 0)[0] for x in (m, fresh))
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+    # and they matter
+    stream.reset_stream(m)
+    other = stream.apply_stream(_model(dtype), max_frames=2, frame_tokens=FRAME)
+    with torch.inference_mode():
+        assert not torch.equal(m(images[:, :1])[0][0], other(images[:, :1])[0][0])
