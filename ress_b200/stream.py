@@ -143,7 +143,8 @@ def _prologue(attn) -> dict:
                 norm.bias is None:
             raise RessError("streaming takes q/k LayerNorms over 64 head dims, with weight and bias, or none")
         args[name + "_weight"], args[name + "_bias"] = norm.weight.detach().float(), norm.bias.detach().float()
-        args["eps"] = norm.eps
+        if args.setdefault("eps", norm.eps) != norm.eps:
+            raise RessError("streaming takes q/k LayerNorms of one eps")
     rope = getattr(attn, "rope", None)
     if rope is not None:
         from .vggt import RotaryPosition2D

@@ -226,3 +226,15 @@ def test_heads_beyond_a_grid_are_refused(heads):
     """Two tiles of rows a head make more blocks than a grid's second dimension takes."""
     wide = _cache(heads=heads, ps=heads * 4096, ss=heads)
     assert _lib.load().ress_cache_attn(wide, _attn(tokens=20, q_heads=heads), FAKE, None) == -3
+
+
+def test_norms_of_unlike_eps_are_refused():
+    attn = vggt.Attention(128, 2, True, vggt.RotaryPosition2D())
+    attn.k_norm.eps = 1e-3
+    with pytest.raises(RessError, match="eps"):
+        stream._prologue(attn)
+    attn.q_norm.eps = 1e-3
+    assert stream._prologue(attn)["eps"] == 1e-3
+    attn.q_norm = torch.nn.Identity()
+    attn.k_norm.eps = 1e-4
+    assert stream._prologue(attn)["eps"] == 1e-4
