@@ -26,6 +26,13 @@ def layer_shape(x, pos, num_special_tokens=5, num_heads=16, shape=None):
     return {"B": B, "N": N, "P": P, "head_dim": C // num_heads, "num_heads": num_heads, "H": H, "W": W, "S": S}
 
 
+def _linear_dtype(m):
+    """The type of a Linear's weights.  An 8-bit one (stream.Int8Linear) says so
+    itself: its ``weight`` would be laid out anew for the question."""
+    dtype = getattr(m, "dtype", None)
+    return dtype if isinstance(dtype, torch.dtype) else m.weight.dtype
+
+
 def _fusable_norm(m, hd):
     return (isinstance(m, torch.nn.LayerNorm) and tuple(m.normalized_shape) == (hd,) and m.elementwise_affine
             and m.bias is not None)
@@ -71,7 +78,7 @@ def compute_qkv_scored(self, x, pos, num_special_tokens=5, num_heads=16, shape=N
     None."""
     shp = layer_shape(x, pos, num_special_tokens, num_heads, shape)
     nh, hd = num_heads, x.shape[-1] // num_heads
-    if x.dtype != torch.bfloat16 or self.qkv.weight.dtype != torch.bfloat16:
+    if x.dtype != torch.bfloat16 or _linear_dtype(self.qkv) != torch.bfloat16:
         return None
     args = _prologue_args(self, x, pos, hd)  # x: the Linear's output has its device and dtype
     if args is None:
@@ -125,9 +132,9 @@ def combine_special_and_patch(x_special, x_patch, shape):
 
 def project_out(self, x, B, N, P, nh, hd):
     x = x.transpose(1, 2).reshape(B, N * P, nh * hd)
-    w = self.proj.weight
-    if x.dtype != w.dtype and not torch.is_autocast_enabled():
+    dtype = _linear_dtype(self.proj)
+    if x.dtype != dtype and not torch.is_autocast_enabled():
         # the sparse kernel writes fp32 (attention.py:243); a model held in
         # bf16 without autocast projects in its own dtype
-        x = x.to(w.dtype)
+        x = x.to(dtype)
     return self.proj_drop(self.proj(x))

@@ -213,3 +213,22 @@ def test_weights_loaded_after_apply_stream(dtype):
     other = stream.apply_stream(_model(dtype), max_frames=2, frame_tokens=FRAME)
     with torch.inference_mode():
         assert not torch.equal(m(images[:, :1])[0][0], other(images[:, :1])[0][0])
+
+
+def test_int8_linears_on_the_sparse_path(monkeypatch):
+    """The sparse path asks a quantised block for its type, not for its weights laid out again."""
+    from ress_b200 import qkv
+
+    torch.manual_seed(9)
+    attn = vggt.Attention(256, 4, True, vggt.RotaryPosition2D()).cuda().bfloat16()
+    stream.quantize_linears(attn)
+
+    def unwanted(self):
+        raise AssertionError("the weights were laid out")
+
+    monkeypatch.setattr(stream.Int8Linear, "weight", property(unwanted))
+    x = torch.randn(1, 2 * FRAME, 256, device="cuda").bfloat16()
+    pos = torch.zeros(1, 2 * FRAME, 2, dtype=torch.long, device="cuda")
+    with torch.inference_mode():
+        assert qkv.compute_qkv_scored(attn, x, pos, 5, 4, shape=dict(H=8, W=8, N=2)) is not None
+        qkv.project_out(attn, torch.randn(1, 4, 2 * FRAME, 64, device="cuda"), 1, 2, FRAME, 4, 64)
