@@ -107,8 +107,10 @@ class Int8Linear(nn.Module):
         return K.int8_linear(x, self.w8, self.scale, self.bias, act=self.act)
 
     def _apply(self, fn, recurse=True):
-        # .to(dtype), .half() and the like move the module but keep its scales and bias in fp32
+        # .to(dtype), .half() and the like move the module and change the type it
+        # stands for, but keep its scales and bias in fp32
         kept = {n: b for n, b in self._buffers.items() if b is not None and b.dtype == torch.float32}
+        self.dtype = fn(torch.empty(0, dtype=self.dtype, device=self.w8.device)).dtype
         super()._apply(fn, recurse)
         for n, b in kept.items():
             self._buffers[n] = b.to(self._buffers[n].device)

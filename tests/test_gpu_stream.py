@@ -232,3 +232,22 @@ def test_int8_linears_on_the_sparse_path(monkeypatch):
     with torch.inference_mode():
         assert qkv.compute_qkv_scored(attn, x, pos, 5, 4, shape=dict(H=8, W=8, N=2)) is not None
         qkv.project_out(attn, torch.randn(1, 4, 2 * FRAME, 64, device="cuda"), 1, 2, FRAME, 4, 64)
+
+
+def test_int8_linear_type_follows_the_model():
+    """Quantised in fp32 and then moved to bf16, a block is as one quantised from bf16 weights: type, and the sparse path's route."""
+    from ress_b200 import qkv
+
+    torch.manual_seed(8)
+    attn = vggt.Attention(256, 4, True, vggt.RotaryPosition2D()).cuda()
+    assert stream.quantize_linears(attn) == 2
+    attn = attn.bfloat16()
+    assert attn.qkv.dtype == torch.bfloat16 and attn.qkv.weight.dtype == torch.bfloat16
+    assert attn.qkv.scale.dtype == torch.float32 and attn.qkv.bias.dtype == torch.float32
+    x = torch.randn(1, 2 * FRAME, 256, device="cuda").bfloat16()
+    pos = torch.zeros(1, 2 * FRAME, 2, dtype=torch.long, device="cuda")
+    with torch.inference_mode():
+        got = qkv.compute_qkv_scored(attn, x, pos, 5, 4, shape=dict(H=8, W=8, N=2))
+        assert got is not None
+        out = qkv.project_out(attn, torch.randn(1, 4, 2 * FRAME, 64, device="cuda"), 1, 2, FRAME, 4, 64)
+    assert out.dtype == torch.bfloat16
