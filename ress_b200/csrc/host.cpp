@@ -267,11 +267,16 @@ PyObject *cache_attn(PyObject *, PyObject *const *o, Py_ssize_t n) {
     });
 }
 
-// x as (M, K) rows with one stride; a copy only where its strides do not allow that
+// whether the kernels can read x: (M, K) rows that do not overlap, 16-byte aligned
+bool readable(const at::Tensor &x) {
+    if (x.dim() != 2 || x.stride(1) != 1 || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15)) return false;
+    return x.size(0) <= 1 || (x.stride(0) >= x.size(1) && x.stride(0) * x.element_size() % 16 == 0);
+}
+// x as (M, K) rows; a copy only where they are not readable as they lie
 at::Tensor rows2d(const at::Tensor &x) {
     require(x.dim() >= 1 && x.size(-1) > 0, "x has no features");
     at::Tensor y = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
-    return y.stride(1) == 1 ? y : y.contiguous();
+    return readable(y) ? y : y.clone(at::MemoryFormat::Contiguous);
 }
 int64_t row_stride(const at::Tensor &x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
 
@@ -320,7 +325,7 @@ PyObject *int8_linear(PyObject *, PyObject *const *o, Py_ssize_t n) {
                     "w_scale and bias are contiguous fp32 (N,)");
         at::Tensor copy;
         const at::Tensor *rows = &x;
-        if (x.dim() != 2 || x.stride(1) != 1) {
+        if (!readable(x)) {
             copy = rows2d(x);
             rows = &copy;
         }

@@ -626,14 +626,17 @@ def cache_attn(q, k_pages, v_pages, k_scale, v_scale, table, lens, *, limits=Non
 
 def int8_quant_rows(x):
     """(..., K) bf16 or fp32 -> int8 of the same shape and one fp32 scale per
-    row (ress_int8_quant_rows): tokens, or the output channels of a weight."""
+    row (ress_int8_quant_rows): tokens, or the output channels of a weight.
+    Rows that are not 16-byte aligned, or lie over one another, are copied."""
     return (_host or _bind()).int8_quant_rows(x)
 
 
 def int8_linear(x, w8, w_scale, bias=None, *, act=None, out_dtype=None):
     """A Linear layer in 8-bit integers (ress_int8_linear): x (..., K) bf16 or
     fp32 is quantised per token, w8 (N, K) int8 and w_scale (N,) fp32 are the
-    weight's (int8_quant_rows lays them out once).  act: None or "gelu".
+    weight's (int8_quant_rows lays them out once).  x may have any strides; it is
+    copied where its rows are not 16-byte aligned or lie over one another.  K is
+    a multiple of 16.  act: None or "gelu".
     Returns (..., N) in x's type, or out_dtype."""
     if act is not None and act != "gelu":
         raise RessError(f"unknown activation {act!r}")

@@ -163,3 +163,16 @@ def test_refusals():
             K.int8_linear(*args, **kw)
     with pytest.raises(RessError):
         K.int8_quant_rows(x[:, :24])
+
+
+def test_rows_that_no_copy_engine_takes():
+    """Rows off a 16-byte boundary, at an odd distance, or all the same one (expanded)."""
+    x, w, bias = _inputs(130, 270, 96, torch.bfloat16, seed=4)
+    w8, sw = K.int8_quant_rows(w[:, :256].contiguous())
+    flat = x.reshape(-1)
+    for rows in (x[:, 3:259], x[:, 8:264], flat[1:1 + 100 * 256].view(100, 256), x[:1, :256].expand(70, 256),
+                 x[None, :1, :256].expand(3, 50, 256), x.t()[:256].t(), x.float()[:, 1:257], x.float()[:5, 1:257]):
+        plain = rows.clone(memory_format=torch.contiguous_format)
+        assert torch.equal(K.int8_linear(rows, w8, sw, bias), K.int8_linear(plain, w8, sw, bias))
+        for a, b in zip(K.int8_quant_rows(rows), K.int8_quant_rows(plain)):
+            assert a.shape == b.shape and torch.equal(a, b)
