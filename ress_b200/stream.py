@@ -104,7 +104,13 @@ class Int8Linear(nn.Module):
         return (self.w8.float() * self.scale[:, None]).to(self.dtype)
 
     def forward(self, x):
-        return K.int8_linear(x, self.w8, self.scale, self.bias, act=self.act)
+        if not torch.is_autocast_enabled("cuda"):
+            return K.int8_linear(x, self.w8, self.scale, self.bias, act=self.act)
+        # as a Linear's, the output has autocast's type; fp16, which the kernel has not, goes by fp32
+        dtype = torch.get_autocast_dtype("cuda")
+        x = x.float() if x.dtype == torch.float16 else x
+        out = torch.bfloat16 if dtype == torch.bfloat16 else torch.float32
+        return K.int8_linear(x, self.w8, self.scale, self.bias, act=self.act, out_dtype=out).to(dtype)
 
     def _apply(self, fn, recurse=True):
         # .to(dtype), .half() and the like move the module and change the type it

@@ -251,3 +251,17 @@ def test_int8_linear_type_follows_the_model():
         assert got is not None
         out = qkv.project_out(attn, torch.randn(1, 4, 2 * FRAME, 64, device="cuda"), 1, 2, FRAME, 4, 64)
     assert out.dtype == torch.bfloat16
+
+
+def test_int8_linear_under_autocast():
+    """As a Linear's, the output has autocast's type."""
+    torch.manual_seed(10)
+    lin = torch.nn.Linear(64, 32).cuda()
+    q, x = stream.Int8Linear(lin), torch.randn(5, 64, device="cuda")
+    with torch.inference_mode():
+        assert q(x).dtype == torch.float32
+        for dtype in (torch.bfloat16, torch.float16):
+            with torch.autocast("cuda", dtype=dtype):
+                assert q(x).dtype == lin(x).dtype == dtype
+                assert _rel(q(x), lin(x)) < 0.02
+                assert q(x.bfloat16()).dtype == q(x.to(dtype)).dtype == dtype
