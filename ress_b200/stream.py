@@ -204,8 +204,9 @@ def apply_stream(model, streams: int = 1, max_frames: int = 64, frame_tokens: in
             # the norms as they are now: weights may have been loaded or moved since
             return stream_attention_forward(self, x, pos if pos is not None else xpos, _cache, frame_tokens, _prologue(self))
 
-        attn.ress_stream = (cache, attn.__dict__.get("forward"))
-        attn.forward = MethodType(_fwd, attn)
+        forward = MethodType(_fwd, attn)
+        attn.ress_stream = (cache, attn.__dict__.get("forward"), forward)
+        attn.forward = forward
     return model
 
 
@@ -221,10 +222,11 @@ def reset_stream(model):
 
 
 def remove_stream(model):
-    """Puts the global blocks' attention back to what it was before apply_stream."""
+    """Puts the global blocks' attention back to what it was before apply_stream;
+    a forward that was installed over it since stays."""
     for block in global_blocks(model):
         state = block.attn.__dict__.pop("ress_stream", None)
-        if state is not None:
+        if state is not None and block.attn.__dict__.get("forward") is state[2]:
             del block.attn.forward
             if state[1] is not None:
                 block.attn.forward = state[1]

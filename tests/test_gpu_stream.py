@@ -265,3 +265,20 @@ def test_int8_linear_under_autocast():
                 assert q(x).dtype == lin(x).dtype == dtype
                 assert _rel(q(x), lin(x)) < 0.02
                 assert q(x.bfloat16()).dtype == q(x.to(dtype)).dtype == dtype
+
+
+def test_remove_stream_leaves_what_came_later():
+    m = _model()
+    blocks = m.aggregator.global_blocks
+    stream.apply_stream(m, max_frames=2, frame_tokens=FRAME)
+    later = lambda x, pos=None: x  # noqa: E731
+    blocks[0].attn.forward = later
+    stream.remove_stream(m)
+    assert blocks[0].attn.forward is later and "forward" not in blocks[1].attn.__dict__
+    # taken out from between: what lies below is put back once
+    blocks[0].attn.__dict__.pop("forward")
+    blocks[1].attn.forward = later
+    stream.apply_stream(m, max_frames=2, frame_tokens=FRAME)
+    stream.apply_stream(m, max_frames=1, frame_tokens=FRAME)
+    stream.remove_stream(m)
+    assert "forward" not in blocks[0].attn.__dict__ and blocks[1].attn.forward is later
