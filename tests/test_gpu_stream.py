@@ -282,3 +282,16 @@ def test_remove_stream_leaves_what_came_later():
     stream.apply_stream(m, max_frames=1, frame_tokens=FRAME)
     stream.remove_stream(m)
     assert "forward" not in blocks[0].attn.__dict__ and blocks[1].attn.forward is later
+
+
+def test_fp32_streams_are_not_rounded_to_bf16():
+    """The attention of an fp32 block comes out in fp32."""
+    torch.manual_seed(7)
+    attn = vggt.Attention(256, 4, True, vggt.RotaryPosition2D()).cuda()
+    attn.proj = torch.nn.Identity()
+    x, pos = torch.randn(1, FRAME, 256, device="cuda"), torch.randint(0, 9, (1, FRAME, 2), device="cuda")
+    with torch.inference_mode():
+        cache = stream.StreamCache(1, 4, FRAME)
+        out = stream.stream_attention_forward(attn, x, pos, cache, FRAME, stream._prologue(attn))
+    assert out.dtype == torch.float32
+    assert (out != out.bfloat16().float()).float().mean() > 0.9
