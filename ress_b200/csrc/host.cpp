@@ -63,6 +63,13 @@ inline void on_device(int i, std::initializer_list<const at::Tensor *> ts) {
     for (const at::Tensor *t : ts)
         require(t == nullptr || (t->is_cuda() && t->get_device() == i), "all tensors of a call are on one CUDA device");
 }
+// The operators have no backward: a result without history would cut gradients silently.
+inline void no_gradients(std::initializer_list<const at::Tensor *> ts) {
+    if (!c10::GradMode::is_enabled()) return;
+    for (const at::Tensor *t : ts)
+        require(t == nullptr || !t->requires_grad(),
+                "the streaming operators are for inference: call them under torch.no_grad() or torch.inference_mode()");
+}
 inline int dtype_code(at::ScalarType t) {
     if (t == at::kFloat) return RESS_F32;
     if (t == at::kBFloat16) return RESS_BF16;
@@ -163,6 +170,7 @@ PyObject *cache_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
         require(v.sizes() == k.sizes() && rk.H == c.heads && v.scalar_type() == dtype,
                 "k and v must be alike, with the cache's heads");
         on_device(i, {&v, q, n_new, pos, cos, sin});
+        no_gradients({&k, &v, q});
         a.k = data<void>(&k);
         a.v = data<void>(&v);
         a.tokens = rk.T;
@@ -178,6 +186,7 @@ PyObject *cache_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
             require(w == nullptr || (w->is_cuda() && w->get_device() == i && w->scalar_type() == at::kFloat && w->dim() == 1 &&
                                      w->size(0) == HD && w->is_contiguous()),
                     "norm weights and biases are contiguous fp32 (64,) on the call's device");
+            no_gradients({w});
             norms[j] = data<float>(w);
         }
         require((norms[0] == nullptr) == (norms[1] == nullptr) && (norms[2] == nullptr) == (norms[3] == nullptr),
@@ -224,6 +233,7 @@ PyObject *cache_attn(PyObject *, PyObject *const *o, Py_ssize_t n) {
         const int i = cuda_index(q);
         const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
         require(q.scalar_type() == at::kBFloat16, "cache_attn takes bf16 q");
+        no_gradients({&q});
         const Rows r = head_rows(q, "q");
         const ress_cache c = cache_of(i, r.B, o + 1);
         const at::Tensor *limits = opt(o[7], "limits"), *given = opt(o[9], "out");
@@ -287,6 +297,7 @@ PyObject *int8_quant_rows(PyObject *, PyObject *const *o, Py_ssize_t n) {
         const at::Tensor &x = tensor(o[0], "x");
         const int i = cuda_index(x), dt = dtype_code(x.scalar_type());
         const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
+        no_gradients({&x});
         const at::Tensor rows = rows2d(x);
         const int64_t M = rows.size(0), K = rows.size(1);
         require(M <= INT_MAX && K <= INT_MAX, "x is too large");
@@ -317,6 +328,7 @@ PyObject *int8_linear(PyObject *, PyObject *const *o, Py_ssize_t n) {
         if (PyErr_Occurred()) throw PythonError{};
         const int odt = want < 0 ? dt : (int)want;
         on_device(i, {&w, &ws, bias});
+        no_gradients({&x, &ws, bias});
         require(w.scalar_type() == at::kChar && w.dim() == 2 && w.is_contiguous(), "w8 must be contiguous int8 (N, K)");
         const int64_t N = w.size(0), K = w.size(1);
         require(x.dim() >= 1 && x.size(-1) == K, "x and w8 have unlike numbers of features");

@@ -579,7 +579,8 @@ def qkv_prologue(qkv, H, qn_weight=None, qn_bias=None, kn_weight=None, kn_bias=N
 
 # ----------------------------------------------------------------- streaming
 # These calls are made per token and take the GPU a few microseconds, so their
-# checks, allocations and launches are compiled (csrc/host.cpp).
+# checks, allocations and launches are compiled (csrc/host.cpp).  They have no
+# backward: with gradients enabled, an input that needs one is refused.
 PAGE = 64  # tokens per cache page
 _host = None
 

@@ -295,3 +295,25 @@ def test_fp32_streams_are_not_rounded_to_bf16():
         out = stream.stream_attention_forward(attn, x, pos, cache, FRAME, stream._prologue(attn))
     assert out.dtype == torch.float32
     assert (out != out.bfloat16().float()).float().mean() > 0.9
+
+
+def test_inputs_that_need_gradients_are_refused():
+    """The operators have no backward: no result without history for an input that has one."""
+    x = torch.randn(1, 3, 2, 64, device="cuda", requires_grad=True)
+    flat = torch.randn(4, 64, device="cuda", requires_grad=True)
+    c = stream.StreamCache(1, 2, 64)
+    w8, s = K.int8_quant_rows(torch.randn(8, 64, device="cuda"))
+    q = x.detach().bfloat16().requires_grad_()
+    plain = x.detach()
+    weight = torch.ones(64, device="cuda", requires_grad=True)
+    calls = [lambda: c.append(x, plain), lambda: c.append(plain, x), lambda: c.append(plain, plain, q=x), lambda: c.attend(q),
+             lambda: c.append(plain, plain, kn_weight=weight, kn_bias=weight.detach()),
+             lambda: K.int8_linear(flat, w8, s), lambda: K.int8_linear(flat.detach(), w8, s, weight[:8]),
+             lambda: K.int8_quant_rows(flat)]
+    for f in calls:
+        with pytest.raises(RessError, match="no_grad"):
+            f()
+    with torch.no_grad():
+        for f in calls:
+            f()
+    assert K.check_status() == 0
