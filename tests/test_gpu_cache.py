@@ -527,3 +527,41 @@ def test_append_refuses_a_pool_without_heads():
     k = torch.zeros(1, 3, 0, HD, device="cuda")
     with pytest.raises(RessError):
         K.cache_append(k, k, **none, table=table, lens=ln, q=torch.zeros(1, 3, 4, HD, device="cuda"))
+
+
+@pytest.mark.parametrize("T", [1, 9])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_long_runs_of_a_warp(T, masked):
+    """Few queries of so many streams and heads that pages are not split: 75 pages
+    a warp, whose ids and scales are fetched 32 at a time."""
+    B, H, pages = 20, 16, 600
+    cache, table, _ = _filled(1, [64 * pages], H, seed=16)
+    g = _gen(16)
+    # the streams read one pool, each in its own order
+    table = torch.stack([table[0, torch.randperm(pages, generator=g, device="cuda")] for _ in range(B)]).contiguous()
+    lens = torch.randint(60 * pages, 64 * pages + 1, (B,), device="cuda", generator=g, dtype=torch.int32)
+    limits = None
+    if masked:
+        limits = torch.randint(0, 64 * pages, (B, T), device="cuda", generator=g, dtype=torch.int32)
+    q = torch.randn(B, T, H, HD, device="cuda", generator=g).bfloat16()
+    out = K.cache_attn(q, **cache, table=table, lens=lens, limits=limits, out_bf16=False)
+    torch.cuda.synchronize()
+    assert K.check_status() == 0
+    _close(out, *attention(q, cache, table, lens, limits))
+
+
+@pytest.mark.parametrize("kind", ["whole", "random", "steps"])
+def test_attention_long_runs_of_a_cta(kind):
+    """Many queries of one head: 86 pages a CTA, through every ring several times, without
+    masks, with masks on every page, and with both in turn."""
+    T, pages = 40 * 256, 600
+    cache, table, ln = _filled(1, [64 * pages - 5], 1, seed=17)
+    g = _gen(17)
+    i = torch.arange(T, device="cuda", dtype=torch.int32)
+    limits = {"whole": None, "random": torch.randint(0, 64 * pages, (1, T), device="cuda", generator=g, dtype=torch.int32),
+              "steps": (i // 256 * 960 + 100)[None].contiguous()}[kind]
+    q = torch.randn(1, T, 1, HD, device="cuda", generator=g).bfloat16()
+    out = K.cache_attn(q, **cache, table=table, lens=ln, limits=limits, out_bf16=False)
+    torch.cuda.synchronize()
+    assert K.check_status() == 0
+    _close(out, *attention(q, cache, table, ln, limits))

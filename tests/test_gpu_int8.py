@@ -176,3 +176,54 @@ def test_rows_that_no_copy_engine_takes():
         assert torch.equal(K.int8_linear(rows, w8, sw, bias), K.int8_linear(plain, w8, sw, bias))
         for a, b in zip(K.int8_quant_rows(rows), K.int8_quant_rows(plain)):
             assert a.shape == b.shape and torch.equal(a, b)
+
+
+# The tile that each size takes, without and with GELU (a pair's 256 x 256, one
+# CTA's 128 x 128 or 128 x 64), and the passes of its busiest CTA.  Odd widths
+# are stored by plain instructions, the others by TMA.
+TILES = [
+    (1374, 4096, 1024, "128: one pass of 32 slices"),
+    (300, 1024, 4096, "128: one pass"),
+    (257, 1024, 4097, "128: one pass, plain stores"),
+    (3000, 256, 1500, "128: two passes of 2 slices; 64 with GELU: four"),
+    (3000, 256, 1501, "the same, plain stores"),
+    (2200, 2064, 1022, "pair: one pass of 17 slices, plain bf16 stores; 128 with GELU"),
+    (700, 1024, 1024, "64: one pass"),
+    (165, 1536, 3001, "64: one pass of 12 slices, plain stores"),
+    (2100, 144, 2000, "128: two passes of 2 slices; 64 with GELU: four"),
+    (5000, 1040, 1001, "pair: two passes, plain stores"),
+    (9999, 1024, 1001, "pair: three passes, plain stores"),
+    (12001, 1008, 1024, "pair: three passes"),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k,n,tile", TILES)
+def test_linear_tiles(m, k, n, tile, dtype):
+    """Every tile in both output types: remainders of rows, channels and K, one pass and several, both ways of storing."""
+    x, w, bias = _inputs(m, k, n, dtype, seed=m + k + n)
+    w8, sw = K.int8_quant_rows(w)
+    x8, sx = quant_rows(x)
+    for b, act in ((bias, None), (None, "gelu")):
+        out = K.int8_linear(x, w8, sw, b, act=act)
+        torch.cuda.synchronize()
+        assert K.check_status() == 0
+        _check(out, x8, sx, w8, sw, b, act)
+        # the same bits in another tile
+        assert torch.equal(K.int8_linear(x[-20:], w8, sw, b, act=act), out[-20:])
+
+
+def test_a_graph_of_linears():
+    """Captured and replayed on new tokens: the quantiser and the product of both, back to back."""
+    for m in (1, 64, 1500):
+        x, w, bias = _inputs(m, 512, 512, torch.bfloat16, seed=m)
+        w8, sw = K.int8_quant_rows(w)
+        want = K.int8_linear(K.int8_linear(x, w8, sw, bias, act="gelu"), w8, sw)
+        held, graph = torch.zeros_like(x), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = K.int8_linear(K.int8_linear(held, w8, sw, bias, act="gelu"), w8, sw)
+        for _ in range(3):
+            held.copy_(x)
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
