@@ -59,7 +59,7 @@ enum {
     RESS_STATUS_CACHE_RANGE = 8          /* a cache length or page number out of range */
 };
 
-enum { RESS_F32 = 0, RESS_BF16 = 1 };
+enum { RESS_F32 = 0, RESS_BF16 = 1, RESS_BF16_NORMS = 256 /* ress_append_args: beside RESS_BF16 */ };
 
 int ress_version(void);
 
@@ -376,7 +376,8 @@ typedef struct {
  *   b*sb + t*st + head*sh (elements; rows 16-byte aligned), RESS_F32 or
  *   RESS_BF16; k and v have the cache's heads, q a multiple of them.
  *   q and k: LayerNorm over the head dims where weight and bias are given
- *   (fp32, 64 values, 16-byte aligned; NULL: none), then the 2-D rotary embedding as in
+ *   (fp32, or bf16 with dtype RESS_BF16 | RESS_BF16_NORMS; 64 values, 16-byte
+ *   aligned; NULL: none), then the 2-D rotary embedding as in
  *   ress_qkv_prologue when rope_cos is given (tables (rope_len, 32) in the
  *   input's type, pos (streams, tokens, 2) int64), all in fp32 without
  *   intermediate rounding.  q_out (streams, tokens, q_heads, 64) contiguous in
@@ -394,7 +395,7 @@ typedef struct {
     void *q_out;
     int64_t dtype, tokens, q_heads;
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
-    const float *qn_weight, *qn_bias, *kn_weight, *kn_bias;
+    const void *qn_weight, *qn_bias, *kn_weight, *kn_bias;
     double eps;
     const int64_t *pos;
     const void *rope_cos, *rope_sin;

@@ -37,7 +37,7 @@ struct AppendArgs {
     long long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;  // elements
     void *q_out;  // (B, T, Hq, 64) contiguous
     int T, group;
-    const float *qw, *qb, *kw, *kb;
+    const void *qw, *qb, *kw, *kb;
     float eps;
     const long long *pos;
     const void *cos, *sin;
@@ -101,11 +101,16 @@ __device__ __forceinline__ void put(float *p, const f32x2 (&x)[4]) {
         *reinterpret_cast<float4 *>(p + 16 * i) = v;
     }
 }
-// four floats of a norm's weight or bias
+// four values of a norm's weight or bias
 __device__ __forceinline__ void affine4(const float *p, f32x2 &a, f32x2 &b) {
     const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
     a = f2_pack(v.x, v.y);
     b = f2_pack(v.z, v.w);
+}
+__device__ __forceinline__ void affine4(const __nv_bfloat16 *p, f32x2 &a, f32x2 &b) {
+    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
+    a = f2_pack(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u));
+    b = f2_pack(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
 }
 // the sum of both lanes of x over the eight threads of a row
 __device__ __forceinline__ float row_sum(f32x2 x) {
@@ -121,8 +126,9 @@ __device__ __forceinline__ f32x2 twice(float x) { return f2_pack(x, x); }
 // LayerNorm (where w is given) and rotation of a thread's rows, unrounded.  All
 // lanes of the warp take part.  sn holds sin of dims 16..19 on, and -sin of
 // dims 0..3.
-__device__ __forceinline__ void norm_rotate(f32x2 (&x)[ROWS][4], int d, float eps, const float *w, const float *b,
-                                            bool rope, const f32x2 (&cs)[ROWS][4], const f32x2 (&sn)[ROWS][4]) {
+template <typename W>
+__device__ __forceinline__ void norm_rotate(f32x2 (&x)[ROWS][4], int d, float eps, const W *w, const W *b, bool rope,
+                                            const f32x2 (&cs)[ROWS][4], const f32x2 (&sn)[ROWS][4]) {
     if (w != nullptr) {
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -202,8 +208,9 @@ __device__ __noinline__ void move_codes(uint8_t *p, float f) {
     store_codes(p, x, f);
 }
 
+// T, W: types of the rows and of the norms.
 // heads: of the cache; the CTA takes [blockIdx.x * per, .. + per) of them.
-template <typename T>
+template <typename T, typename W>
 __global__ void __launch_bounds__(APP_NT, 2) append_kernel(const AppendArgs a, int heads, int per) {
     constexpr int WARPS = APP_NT / 32;
     __shared__ uint32_t red[2][2][WARPS];
@@ -230,6 +237,8 @@ __global__ void __launch_bounds__(APP_NT, 2) append_kernel(const AppendArgs a, i
     const T *kp = reinterpret_cast<const T *>(a.k) + b * a.k_sb + t0 * a.k_st + d;
     const T *vp = reinterpret_cast<const T *>(a.v) + b * a.v_sb + t0 * a.v_st + d;
     const T *qp = reinterpret_cast<const T *>(a.q) + b * a.q_sb + t0 * a.q_st + d;
+    const W *const qw = reinterpret_cast<const W *>(a.qw), *const qb = reinterpret_cast<const W *>(a.qb);
+    const W *const kw = reinterpret_cast<const W *>(a.kw), *const kb = reinterpret_cast<const W *>(a.kb);
     const bool has_q = a.q != nullptr, rope = a.cos != nullptr;
     Raw<T> rk[ROWS], rv[ROWS], rq[ROWS];
 #pragma unroll
@@ -293,7 +302,7 @@ __global__ void __launch_bounds__(APP_NT, 2) append_kernel(const AppendArgs a, i
             ask_k(h + 1);
             if (AHEAD) ask_v(h + 1);
         }
-        norm_rotate(x, d, a.eps, a.kw, a.kb, rope, cs, sn);
+        norm_rotate(x, d, a.eps, kw, kb, rope, cs, sn);
         uint32_t (*red_h)[WARPS] = red[h & 1];  // the other one may still be read
         uint32_t mk = 0, mv = 0;
 #pragma unroll
@@ -347,7 +356,7 @@ __global__ void __launch_bounds__(APP_NT, 2) append_kernel(const AppendArgs a, i
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) rq[r].get(x[r]);
             if (AHEAD && g + 1 == a.group && h + 1 < h1) ask_q((long long)(h + 1) * a.group);
-            norm_rotate(x, d, a.eps, a.qw, a.qb, rope, cs, sn);
+            norm_rotate(x, d, a.eps, qw, qb, rope, cs, sn);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
                 if (row[r]) put(qo + r * (PAGE / ROWS) * q_row, x[r]);
@@ -372,9 +381,10 @@ extern "C" int ress_cache_append(const ress_cache *cache, const ress_append_args
         return RESS_E_ARG;
     if ((g.rope_cos == nullptr) != (g.rope_sin == nullptr) || (g.rope_cos != nullptr && (!g.pos || g.rope_len <= 0)))
         return RESS_E_ARG;
-    if (g.dtype != RESS_BF16 && g.dtype != RESS_F32) return RESS_E_DTYPE;
+    const bool bf16 = (g.dtype & ~(int64_t)RESS_BF16_NORMS) == RESS_BF16, bf16_norms = (g.dtype & RESS_BF16_NORMS) != 0;
+    if (!bf16 && g.dtype != RESS_F32) return RESS_E_DTYPE;
     // loads of up to 16 bytes
-    const int size = g.dtype == RESS_BF16 ? 2 : 4;
+    const int size = bf16 ? 2 : 4;
     if (((uintptr_t)g.q | (uintptr_t)g.k | (uintptr_t)g.v | (uintptr_t)g.q_out | (uintptr_t)g.rope_cos |
          (uintptr_t)g.rope_sin | (uintptr_t)g.qn_weight | (uintptr_t)g.qn_bias | (uintptr_t)g.kn_weight |
          (uintptr_t)g.kn_bias) & 15)
@@ -419,9 +429,9 @@ extern "C" int ress_cache_append(const ress_cache *cache, const ress_append_args
     }
     const int heads = (int)cache->heads;
     const dim3 grid((unsigned)((heads + per - 1) / per), (unsigned)pages, (unsigned)cache->streams);
-    if (g.dtype == RESS_BF16)
-        cache::append_kernel<__nv_bfloat16><<<grid, cache::APP_NT, 0, (cudaStream_t)stream>>>(a, heads, per);
-    else
-        cache::append_kernel<float><<<grid, cache::APP_NT, 0, (cudaStream_t)stream>>>(a, heads, per);
+    auto kern = !bf16        ? cache::append_kernel<float, float>
+                : bf16_norms ? cache::append_kernel<__nv_bfloat16, __nv_bfloat16>
+                             : cache::append_kernel<__nv_bfloat16, float>;
+    kern<<<grid, cache::APP_NT, 0, (cudaStream_t)stream>>>(a, heads, per);
     return cudaGetLastError() == cudaSuccess ? RESS_OK : RESS_E_LAUNCH;
 }

@@ -181,15 +181,29 @@ PyObject *cache_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
             require(n_new->scalar_type() == at::kInt && n_new->dim() == 1 && n_new->size(0) == rk.B && n_new->is_contiguous(),
                     "n_new holds one contiguous int32 per stream");
         a.n_new = data<int32_t>(n_new);
-        const float *norms[4];
+        const void *norms[4];
+        at::Tensor wide[4];  // fp32 copies of bf16 norms, where the rows or another norm are fp32 or one is not aligned
+        int n_f32 = 0, n_bf16 = 0;
+        bool aligned = true;
         for (int j = 0; j < 4; ++j) {
             const at::Tensor *w = opt(o[10 + j], "a norm's weight");
-            require(w == nullptr || (w->is_cuda() && w->get_device() == i && w->scalar_type() == at::kFloat && w->dim() == 1 &&
+            require(w == nullptr || (w->is_cuda() && w->get_device() == i &&
+                                     (w->scalar_type() == at::kFloat || w->scalar_type() == at::kBFloat16) && w->dim() == 1 &&
                                      w->size(0) == HD && w->is_contiguous()),
-                    "norm weights and biases are contiguous fp32 (64,) on the call's device");
+                    "norm weights and biases are contiguous fp32 or bf16 (64,) on the call's device");
             no_gradients({w});
-            norms[j] = data<float>(w);
+            norms[j] = data<void>(w);
+            if (w != nullptr) ++(w->scalar_type() == at::kFloat ? n_f32 : n_bf16);
+            aligned &= (reinterpret_cast<uintptr_t>(norms[j]) & 15) == 0;
         }
+        if (n_bf16 > 0 && n_f32 == 0 && aligned && dtype == at::kBFloat16)
+            a.dtype |= RESS_BF16_NORMS;
+        else if (n_bf16 > 0 || !aligned)
+            for (int j = 0; j < 4; ++j)
+                if (norms[j] != nullptr) {
+                    wide[j] = opt(o[10 + j], "")->to(at::kFloat, /*non_blocking=*/false, /*copy=*/true);
+                    norms[j] = data<void>(&wide[j]);
+                }
         require((norms[0] == nullptr) == (norms[1] == nullptr) && (norms[2] == nullptr) == (norms[3] == nullptr),
                 "a norm has both weight and bias");
         a.qn_weight = norms[0], a.qn_bias = norms[1], a.kn_weight = norms[2], a.kn_bias = norms[3];

@@ -602,7 +602,7 @@ def cache_append(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, *, q=Non
     with a contiguous last dim (views of a qkv Linear's output).  They come
     behind the lens[b] tokens that stream b holds (lens (B,) int32, not
     changed); n_new (B,) int32 of the T count, all by default.  q and k are
-    normalised over the head dims where weight and bias (fp32) are given, and
+    normalised over the head dims where weight and bias (fp32 or bf16) are given, and
     rotated where rope_cos, rope_sin (positions, 32) and pos (B, T, 2) int64
     are; k and v are quantised into their pages, at the smallest power of two
     per page and head that they fit.  Returns q's rows (B, T, Hq, 64), or None

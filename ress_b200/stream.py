@@ -150,7 +150,9 @@ def _prologue(attn) -> dict:
         if not isinstance(norm, nn.LayerNorm) or tuple(norm.normalized_shape) != (K.HD,) or norm.weight is None or \
                 norm.bias is None:
             raise RessError("streaming takes q/k LayerNorms over 64 head dims, with weight and bias, or none")
-        args[name + "_weight"], args[name + "_bias"] = norm.weight.detach().float(), norm.bias.detach().float()
+        for part in ("weight", "bias"):
+            p = getattr(norm, part).detach()
+            args[f"{name}_{part}"] = p if p.dtype in (torch.float32, torch.bfloat16) else p.float()
         if args.setdefault("eps", norm.eps) != norm.eps:
             raise RessError("streaming takes q/k LayerNorms of one eps")
     rope = getattr(attn, "rope", None)

@@ -565,3 +565,26 @@ def test_attention_long_runs_of_a_cta(kind):
     torch.cuda.synchronize()
     assert K.check_status() == 0
     _close(out, *attention(q, cache, table, ln, limits))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_norms_of_either_type(dtype):
+    """bf16 norms, norms of both types and norms off a 16-byte boundary give the bits of the same values in fp32."""
+    g = _gen(18)
+    names = ("qn_weight", "qn_bias", "kn_weight", "kn_bias")
+    norms = [w.bfloat16() for w in _affine(g) + _affine(g)]
+    q, k, v = torch.randn(2, 70, 6, HD, device="cuda", generator=g).to(dtype).split([2, 2, 2], 2)
+    table, lens = shuffled_table(2, 2, 5, seed=18), _i32(0, 30)
+
+    def off(w):
+        return torch.cat([w[:1], w])[1:]
+
+    results = []
+    for kinds in ([w.float() for w in norms], norms, [norms[0], norms[1].float(), norms[2], norms[3].float()],
+                  [off(w) for w in norms], [off(w.float()) for w in norms]):
+        cache = make_cache(5, 2)
+        rows = K.cache_append(k, v, **cache, table=table, lens=lens, q=q, **dict(zip(names, kinds)))
+        results.append([rows] + [_u8(t) for t in cache.values()])
+    assert K.check_status() == 0
+    for r in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, results[0]))
