@@ -410,7 +410,10 @@ int ress_cache_append(const ress_cache *cache, const ress_append_args *args, int
  * over the cache: softmax(q k^T * sm_scale) v (sm_scale >= 0) over stream b's tokens below
  * min(lens[b], limits[b*tokens + t]) (limits NULL: lens[b] for all).  Query
  * heads are consecutive groups of q_heads / heads per key/value head.  Sums
- * and softmax statistics are fp32.  A query that sees no token gives zeros.
+ * and softmax statistics are fp32; probabilities are rounded to 16 bits for
+ * their product with v (fp16 up to 32 rows a key/value head, else bf16), fp32
+ * output included.  A query that sees no token gives zeros.  A NaN code or
+ * scale reaches the queries that see it, and no others.
  * out (strides in elements, rows 16-byte aligned): bf16 when out_bf16, else
  * fp32.  A length outside [0, 64*table_width] is clamped, a page number
  * outside [0, n_pages) counts as a page of NaN; both set

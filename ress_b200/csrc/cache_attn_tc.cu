@@ -6,9 +6,12 @@
 //   warp 0       loads pages: K blocks (TMA, 64B-swizzled), V blocks (bulk);
 //   warp 1       issues S = Q K^T, tcgen05.mma kind::f8f6f4.  K's codes are an
 //                operand as they lie in the cache.  q is split into two e4m3
-//                parts, q = hi + lo (4 + 4 significant bits, as many as bf16
-//                has), so S takes four K = 32 steps: hi and lo against the same
-//                K, which is what bf16 would take.  Scales are applied to S.
+//                parts, q = hi + lo, so S takes four K = 32 steps: hi and lo
+//                against the same K, which is what bf16 would take.  4 + 4
+//                significant bits are as many as bf16 has, down to 2^-9 of the
+//                row's largest element; smaller ones meet e4m3's subnormals and
+//                err by up to 2^-17 of it, which over 64 dims is below what P is
+//                rounded by.  Scales are applied to S.
 //   warp 2       issues O += P V, kind::f16 in bf16, P from tensor memory (an
 //                MMA of 128 x 80 x 16 takes 40 cycles so, 52 with P in shared
 //                memory).  N = 80: sixteen columns of ones give the row sums.
@@ -35,8 +38,10 @@
 // 1835 with steps of 128 keys; 2070 with the next page's scores loaded ahead;
 // 1845 with the two tiles' exponentials taking turns; a polynomial for a part
 // of the exponentials gained nothing.)
-// P is rounded to bf16 for the MMA, numerator and denominator alike;
-// everything else is fp32.
+// P is rounded to bf16 (2^-9) for the MMA, numerator and denominator alike: tf32
+// has half the rate and takes twice P's way to tensor memory, and fp16 has not
+// the range of V's scales.  Against 64 bits that is 0.55e-3 of an output, whose
+// own rounding to bf16 is 1.6e-3; everything else is fp32.
 // When the tiles are too few for the GPU the pages are split over several
 // CTAs; the one that finishes last joins the pieces in page order, so the
 // result does not depend on the order of arrival.  (With a piece's rows each

@@ -60,6 +60,13 @@ inline int cuda_index(const at::Tensor &t) {
     require(t.is_cuda(), "ress_b200 kernels run on CUDA tensors only (no CPU fallback)");
     return (int)t.get_device();
 }
+// Makes device i current where it is not.
+struct Current {
+    c10::cuda::OptionalCUDAGuard guard;
+    explicit Current(int i) {
+        if (c10::cuda::current_device() != i) guard.set_index((c10::DeviceIndex)i);
+    }
+};
 inline void on_device(int i, std::initializer_list<const at::Tensor *> ts) {
     for (const at::Tensor *t : ts)
         require(t == nullptr || (t->is_cuda() && t->get_device() == i), "all tensors of a call are on one CUDA device");
@@ -160,7 +167,7 @@ PyObject *cache_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
         count(n, 18);
         const at::Tensor &k = tensor(o[0], "k"), &v = tensor(o[1], "v");
         const int i = cuda_index(k);
-        const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
+        const Current current(i);
         const at::Tensor *q = opt(o[8], "q"), *n_new = opt(o[9], "n_new"), *pos = opt(o[15], "pos"),
                          *cos = opt(o[16], "rope_cos"), *sin = opt(o[17], "rope_sin");
         const at::ScalarType dtype = k.scalar_type();
@@ -246,7 +253,7 @@ PyObject *cache_attn(PyObject *, PyObject *const *o, Py_ssize_t n) {
         count(n, 11);
         const at::Tensor &q = tensor(o[0], "q");
         const int i = cuda_index(q);
-        const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
+        const Current current(i);
         require(q.scalar_type() == at::kBFloat16, "cache_attn takes bf16 q");
         no_gradients({&q});
         const Rows r = head_rows(q, "q");
@@ -311,7 +318,7 @@ PyObject *int8_quant_rows(PyObject *, PyObject *const *o, Py_ssize_t n) {
         count(n, 1);
         const at::Tensor &x = tensor(o[0], "x");
         const int i = cuda_index(x), dt = dtype_code(x.scalar_type());
-        const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
+        const Current current(i);
         no_gradients({&x});
         const at::Tensor rows = rows2d(x);
         const int64_t M = rows.size(0), K = rows.size(1);
@@ -337,7 +344,7 @@ PyObject *int8_linear(PyObject *, PyObject *const *o, Py_ssize_t n) {
         const at::Tensor &x = tensor(o[0], "x"), &w = tensor(o[1], "w8"), &ws = tensor(o[2], "w_scale");
         const at::Tensor *bias = opt(o[3], "bias");
         const int i = cuda_index(x), dt = dtype_code(x.scalar_type());
-        const c10::cuda::CUDAGuard current((c10::DeviceIndex)i);
+        const Current current(i);
         const int gelu = PyObject_IsTrue(o[4]);
         const long want = PyLong_AsLong(o[5]);
         if (PyErr_Occurred()) throw PythonError{};

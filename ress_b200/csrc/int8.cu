@@ -658,8 +658,11 @@ __global__ void __launch_bounds__(384, 1) gemm_kernel(const __grid_constant__ CU
             fence_before();
             __syncwarp();
             if (lane == 0) {
-                // only tensor memory changes hands: a releasing arrive would wait for the
-                // loads asked ahead (2,000 to 2,900 cycles of a tile's 10,000)
+                // Only tensor memory changes hands: this warp's reads of it are complete
+                // (tcgen05.wait::ld) and fence::before_thread_sync orders them before the
+                // arrival, which the issuer's wait and fence::after_thread_sync take up;
+                // ordinary memory needs no order.  A releasing arrive would wait for the
+                // loads asked ahead (2,000 to 2,900 cycles of a tile's 10,000).
                 if constexpr (CG == 2)
                     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
                                      leader_addr(smem_u32(&B.acc_free[buf])))
