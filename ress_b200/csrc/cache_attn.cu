@@ -48,7 +48,7 @@ using namespace tc;
 // 16 streams of 11 to 44 thousand tokens, 24 heads on 8: 86 us, 5.2 TB/s of the
 // 6.45 that a copy reaches.  One token, 16 heads, 10,992 tokens: 11.2 us for 22.5
 // MB: a launch, and three pages in turn on each warp, which is bound by the
-// latency of its about 850 instructions a page.
+// latency of its about 580 instructions a page (two groups: 810).
 constexpr int FEW_ROWS = 16, FEW_WARPS = 8, FEW_RING = 3, FEW_SPLITS = 16;
 constexpr int FEW_NT = FEW_WARPS * 32;
 constexpr int FEW_SMEM = FEW_WARPS * FEW_RING * BLOCK_BYTES;

@@ -31,8 +31,8 @@
 // which queue behind the other's exponentials, and the supply of instructions:
 // what is rare is out of line, and the loop over pages is kept short.
 // 5,496 queries x 43,968 tokens x 16 heads, each frame seeing those up to its
-// own: 1639 us, 575 TFLOP/s of the products that no mask hides; 1374 x 10,992:
-// 141 us, 440 (a CTA's start and join weigh more).
+// own: 1644 us, 573 TFLOP/s of the products that no mask hides; 1374 x 10,992:
+// 143 us, 435 (a CTA's start and join weigh more).
 // (Measured on the first at one and the same split: 1684 us so; 1782 with the
 // masked path in the loop; 1860 with the scores read again in pieces of 16;
 // 1835 with steps of 128 keys; 2070 with the next page's scores loaded ahead;
