@@ -31,7 +31,7 @@ using namespace tc;
 // heads: its operands take more instructions than these conversions.)
 // The running maximum, sums and O are fp32.  q is scaled by a power of two that
 // brings the row's largest element to [1, 2), and is exact in fp16 down to 2^-17
-// of it (below, it errs by 2^-25 of it).  P is rounded to fp16 (2^-12), since the
+// of it (below, it errs by 2^-25 of it).  P is rounded to fp16 (2^-11), since the
 // products take 16-bit operands: a page's
 // probabilities count against the page's own maximum, times 2^14, so that small
 // ones keep their bits; the page's weight among the others and its V scale are

@@ -38,7 +38,7 @@
 // 1835 with steps of 128 keys; 2070 with the next page's scores loaded ahead;
 // 1845 with the two tiles' exponentials taking turns; a polynomial for a part
 // of the exponentials gained nothing.)
-// P is rounded to bf16 (2^-9) for the MMA, numerator and denominator alike: tf32
+// P is rounded to bf16 (2^-8) for the MMA, numerator and denominator alike: tf32
 // has half the rate and takes twice P's way to tensor memory, and fp16 has not
 // the range of V's scales.  Against 64 bits that is 0.55e-3 of an output, whose
 // own rounding to bf16 is 1.6e-3; everything else is fp32.

@@ -181,7 +181,7 @@ def stream_attention_forward(attn, x, pos, cache: StreamCache, frame_tokens: int
         ends = (torch.arange(T, device=x.device, dtype=torch.int32) // frame_tokens + 1) * frame_tokens
         limits = (cache.lens[:, None] + ends).contiguous()
     q = cache.append(lin[:, :, 1], lin[:, :, 2], q=lin[:, :, 0], **kw)
-    # fp32 queries are rounded to bf16, which the kernels take: 2^-9 of an element, beside the
+    # fp32 queries are rounded to bf16, which the kernels take: 2^-8 of an element, beside the
     # 2^-4 of the keys' codes.  What comes out keeps the projection's type.
     o = cache.attend(q if q.dtype == torch.bfloat16 else q.bfloat16(), limits=limits,
                      out_bf16=lin.dtype == torch.bfloat16)
